@@ -14,6 +14,8 @@ LIB_PATH = os.path.join(_HERE, "libcpmi355.so")
 
 CP_ERR_NOMEM = -3          # include/cpmi355.h
 CP_F32, CP_F64 = 0, 1
+CP_BF16, CP_F16, CP_E4M3, CP_E5M2 = 2, 3, 4, 5
+CP_QUANT_POW2 = 1
 CP_CD_RECIPROCAL = 1
 CP_CD_DELTA = 2
 CP_REFIT_PRECOMPUTE = 4
@@ -52,6 +54,25 @@ class PruneJob(ctypes.Structure):
                 ("lbound", _c_dbl), ("rbound", _c_dbl), ("seeds", _vp), ("max_fits", ctypes.c_int32),
                 ("max_iter", ctypes.c_int32), ("tol", _c_dbl), ("flags", ctypes.c_int32), ("reserved", ctypes.c_int32),
                 ("ridge", _c_dbl), ("mask_out", _vp), ("W_out", _vp), ("b_out", _vp)]
+
+
+class BlocksStruct(ctypes.Structure):
+    """cp_blocks: a matrix held in 8-bit floating point with a scale per block of 128 (see Blocks)."""
+    _fields_ = [("q", _vp), ("scale", _vp), ("rows", _c_i64), ("cols", _c_i64), ("ld", _c_i64), ("lds", _c_i64),
+                ("fmt", ctypes.c_int32), ("tile", ctypes.c_int32)]
+
+
+class OrthoJob(ctypes.Structure):
+    """cp_ortho_job: one matrix of cp_orthogonalise."""
+    _fields_ = [("G", _vp), ("O", _vp), ("ldg", _c_i64), ("ldo", _c_i64), ("rows", ctypes.c_int32), ("cols", ctypes.c_int32),
+                ("g_dtype", ctypes.c_int32), ("o_dtype", ctypes.c_int32)]
+
+
+class OrthoStepJob(ctypes.Structure):
+    """cp_ortho_step_job: one layer's weights in cp_ortho_step."""
+    _fields_ = [("G", _vp), ("M", _vp), ("W", _vp), ("ldg", _c_i64), ("ldm", _c_i64), ("ldw", _c_i64),
+                ("rows", ctypes.c_int32), ("cols", ctypes.c_int32), ("g_dtype", ctypes.c_int32), ("w_dtype", ctypes.c_int32),
+                ("gamma", _c_dbl)]
 
 
 class CpError(RuntimeError):
@@ -114,6 +135,14 @@ SIGNATURES = {
     "cp_prune_layers": (_c_int, [_c_int, ctypes.POINTER(_vp), _vp, _vp]),
     "cp_result_host": (_c_int, [_vp, ctypes.POINTER(_vp), ctypes.POINTER(_vp), ctypes.POINTER(_c_int),
                                 ctypes.POINTER(_c_int)]),
+    "cp_blocks_check": (_c_int, [_vp]),
+    "cp_quant_blocks": (_c_int, [_vp, _vp, _c_int, _c_i64, _c_i64, _c_i64, _c_int, _vp, _vp]),
+    "cp_matmul_blocks": (_c_int, [_vp, _vp, _vp, _vp, _vp, _c_int, _c_i64, _vp, ctypes.c_size_t]),
+    "cp_matmul_blocks_workspace": (_c_int, [_vp, _vp, _c_int, _c_i64, ctypes.POINTER(ctypes.c_size_t)]),
+    "cp_orthogonalise": (_c_int, [_vp, _c_int, _vp, _c_int, _vp, _c_dbl, _vp, ctypes.c_size_t]),
+    "cp_orthogonalise_workspace": (_c_int, [_c_int, _vp, _c_int, _vp, _c_dbl, ctypes.POINTER(ctypes.c_size_t)]),
+    "cp_ortho_step": (_c_int, [_vp, _c_int, _vp, _c_dbl, _c_dbl, _c_int, _c_dbl, _c_int, _vp, _c_dbl, _vp, ctypes.c_size_t]),
+    "cp_ortho_step_workspace": (_c_int, [_c_int, _vp, _c_int, _vp, _c_dbl, ctypes.POINTER(ctypes.c_size_t)]),
     "cp_probe_mfma_f64": (_c_int, [_vp, ctypes.POINTER(_c_dbl)]),
     "cp_probe_mfma_f64_clock": (_c_int, [_vp, ctypes.POINTER(_c_dbl), ctypes.POINTER(_c_dbl), ctypes.POINTER(_c_dbl)]),
     "cp_probe_hbm_copy": (_c_int, [_vp, ctypes.c_size_t, ctypes.POINTER(_c_dbl)]),
@@ -178,6 +207,125 @@ def _ptr(x):
     if hasattr(x, "data_ptr"):
         return x.data_ptr()
     return int(x)
+
+
+_TORCH_NAMES = {CP_F32: "torch.float32", CP_F64: "torch.float64", CP_BF16: "torch.bfloat16", CP_F16: "torch.float16"}
+
+
+def _matrix(x, dtype, rows, cols, ld, name):
+    """(pointer, row stride in elements, device index or None) of a device matrix.  A torch tensor is held to the dtype code,
+    the shape and unit column stride, and gives its own row stride; a DevBuf to its size; an int is taken as it is."""
+    if hasattr(x, "data_ptr"):
+        if tuple(x.shape) != (rows, cols) or (cols > 1 and rows and x.stride(1) != 1):
+            raise ValueError("%s: a [%d, %d] tensor with unit column stride is needed, got %s, strides %s"
+                             % (name, rows, cols, tuple(x.shape), tuple(x.stride())))
+        if str(x.dtype) != _TORCH_NAMES.get(dtype):
+            raise ValueError("%s: dtype code %r does not fit a tensor of %s" % (name, dtype, x.dtype))
+        if not x.is_cuda:
+            raise ValueError("%s: a tensor on the device is needed" % name)
+        own = x.stride(0) if rows > 1 else max(cols, 1)
+        if ld is not None and rows > 1 and ld != own:
+            raise ValueError("%s: row stride %d does not fit the tensor's %d" % (name, ld, own))
+        return x.data_ptr(), own if ld is None else ld, x.device.index
+    ld = max(cols, 1) if ld is None else int(ld)
+    if isinstance(x, DevBuf):
+        if rows and cols and ((rows - 1) * ld + cols) * (8 if dtype == CP_F64 else 4 if dtype == CP_F32 else 2) > x.nbytes:
+            raise ValueError("%s: the buffer holds %d bytes, too few for [%d, %d]" % (name, x.nbytes, rows, cols))
+        return x.ptr, ld, x.ctx.device
+    return _ptr(x), ld, None
+
+
+class Blocks:
+    """A matrix [rows, cols] held in 8-bit floating point (cp_blocks): bytes q [rows, ld] and float32 scales
+    [ceil(cols / 128), lds], one per 128 columns of a row (tile=1) or of 128 rows (tile=128).  q / scale: torch tensors
+    (two-dimensional: their row strides are ld / lds), DevBufs or device addresses; kept alive by this object.  The bytes of a
+    row from cols to the next multiple of 128 have to be zero."""
+
+    def __init__(self, q, scale, rows, cols, fmt, tile, ld=None, lds=None):
+        rows, cols, tile = int(rows), int(cols), int(tile)
+        kb, up = -(-cols // 128), -(-cols // 128) * 128
+        tall = rows if tile == 1 else -(-rows // 128)
+        self.device = None
+        for t, name, dts, need in ((q, "q", ("torch.uint8", "torch.float8_e4m3fn", "torch.float8_e5m2"), (rows, up)),
+                                   (scale, "scale", ("torch.float32",), (kb, tall))):
+            if not hasattr(t, "data_ptr"):
+                continue
+            if t.dim() != 2 or str(t.dtype) not in dts or not t.is_cuda:
+                raise ValueError("%s: a two-dimensional device tensor of %s is needed" % (name, " / ".join(dts)))
+            if t.shape[0] < need[0] or t.shape[1] < need[1] or (t.shape[1] > 1 and t.stride(1) != 1):
+                raise ValueError("%s: at least %s with unit column stride is needed, got %s" % (name, need, tuple(t.shape)))
+            if self.device not in (None, t.device.index):
+                raise ValueError("q and scale are on different devices")
+            self.device = t.device.index
+        if ld is None:
+            ld = q.stride(0) if hasattr(q, "data_ptr") and q.shape[0] > 1 else max(up, 128)
+        if lds is None:
+            lds = scale.stride(0) if hasattr(scale, "data_ptr") and scale.shape[0] > 1 else max(tall, 1)
+        for b, name, need in ((q, "q", (rows - 1) * ld + up if rows else 0), (scale, "scale", 4 * ((kb - 1) * lds + tall) if kb else 0)):
+            if isinstance(b, DevBuf):
+                self.device = b.ctx.device
+                if b.nbytes < need:
+                    raise ValueError("%s: the buffer holds %d bytes, %d needed" % (name, b.nbytes, need))
+        self.q, self.scale, self.rows, self.cols, self.fmt, self.tile = q, scale, rows, cols, fmt, tile
+        self.ld, self.lds = int(ld), int(lds)
+        self.c = BlocksStruct(_ptr(q), _ptr(scale), rows, cols, self.ld, self.lds, fmt, tile)
+        rc = load().cp_blocks_check(ctypes.byref(self.c))
+        if rc != 0:
+            raise CpError(rc, "cp_blocks_check", "rows %d, cols %d, ld %d, lds %d, fmt %d, tile %d"
+                          % (rows, cols, self.ld, self.lds, fmt, tile))
+
+    @classmethod
+    def empty(cls, ctx, rows, cols, fmt, tile):
+        """A matrix with memory of its own on ctx (contents undefined until cp_quant_blocks writes them)."""
+        kb = -(-cols // 128)
+        return cls(ctx.empty(max(rows * kb * 128, 16)), ctx.empty(max(4 * kb * (rows if tile == 1 else -(-rows // 128)), 16)),
+                   rows, cols, fmt, tile)
+
+
+class _Jobs:
+    """An array of job records and what keeps their memory alive."""
+
+    def __init__(self, struct, n):
+        self.n, self.keep, self.device = n, [], None
+        self.c = (struct * max(n, 1))()
+
+    def _take(self, x, dtype, rows, cols, ld, name):
+        ptr, ld, dev = _matrix(x, dtype, rows, cols, ld, name)
+        if dev is not None:
+            if self.device not in (None, dev):
+                raise ValueError("%s is on another device than the job before it" % name)
+            self.device = dev
+        self.keep.append(x)
+        return ptr, ld
+
+
+class OrthoJobs(_Jobs):
+    """The matrices of Context.orthogonalise: a list of (G, g_dtype, rows, cols, O, o_dtype) or with (.., ldg, ldo)."""
+
+    def __init__(self, jobs):
+        jobs = list(jobs)
+        _Jobs.__init__(self, OrthoJob, len(jobs))
+        for a, (G, gd, rows, cols, O, od, *lds) in zip(self.c, jobs):
+            ldg, ldo = lds or (None, None)
+            a.rows, a.cols, a.g_dtype, a.o_dtype = int(rows), int(cols), gd, od
+            a.G, a.ldg = self._take(G, gd, rows, cols, ldg, "G")
+            a.O, a.ldo = self._take(O, od, rows, cols, ldo, "O")
+
+
+class OrthoStepJobs(_Jobs):
+    """The layers of Context.ortho_step: a list of (G, g_dtype, rows, cols, M, W, w_dtype), with (.., gamma) or with
+    (.., gamma, ldg, ldm, ldw).  gamma: the layer's factor on the learning rate; None = sqrt(max(1, rows / cols))."""
+
+    def __init__(self, jobs):
+        jobs = list(jobs)
+        _Jobs.__init__(self, OrthoStepJob, len(jobs))
+        for a, (G, gd, rows, cols, M, W, wd, *more) in zip(self.c, jobs):
+            gamma, ldg, ldm, ldw = (more + [None] * 4)[:4]
+            a.rows, a.cols, a.g_dtype, a.w_dtype = int(rows), int(cols), gd, wd
+            a.gamma = max(1.0, rows / max(cols, 1)) ** 0.5 if gamma is None else float(gamma)
+            a.G, a.ldg = self._take(G, gd, rows, cols, ldg, "G")
+            a.M, a.ldm = self._take(M, CP_F32, rows, cols, ldm, "M")
+            a.W, a.ldw = self._take(W, wd, rows, cols, ldw, "W")
 
 
 class DevBuf:
@@ -443,6 +591,83 @@ class Context:
             for bfr in (Ad, Bd, Cd):
                 bfr.free()
 
+    # -- 8-bit matrices ----------------------------------------------------------------------
+    def _here(self, device, name):
+        if device is not None and device != self.device:
+            raise ValueError("%s is on device %d, the context on %d" % (name, device, self.device))
+
+    @staticmethod
+    def _ws(ws):
+        if ws is None:
+            return None, 0
+        return _ptr(ws), int(ws.nbytes)
+
+    def quant_blocks(self, x, x_dtype, out=None, out_t=None, ldx=None, flags=0):
+        """x [rows, cols] -> the 8-bit matrices out [rows, cols] and / or out_t [cols, rows] (Blocks), in one read of x
+        (cp_quant_blocks)."""
+        if out is None and out_t is None:
+            raise ValueError("no output")
+        rows, cols = (out.rows, out.cols) if out is not None else (out_t.cols, out_t.rows)
+        p, ldx, dev = _matrix(x, x_dtype, rows, cols, ldx, "x")
+        self._here(dev, "x")
+        for m in (out, out_t):
+            if m is not None:
+                self._here(m.device, "an output")
+        self._check(self.lib.cp_quant_blocks(self.h, p, x_dtype, rows, cols, ldx, flags,
+                                             ctypes.byref(out.c) if out is not None else None,
+                                             ctypes.byref(out_t.c) if out_t is not None else None), "cp_quant_blocks")
+
+    def matmul_blocks(self, A, B, C, c_dtype, bias=None, ldc=None, ws=None):
+        """C [M, N] = A [M, K] B [N, K]^T (+ bias float32 [N]) of two Blocks (cp_matmul_blocks).  ws: None or a device buffer
+        of matmul_blocks_workspace() bytes (needed under stream capture)."""
+        p, ldc, dev = _matrix(C, c_dtype, A.rows, B.rows, ldc, "C")
+        for d, name in ((dev, "C"), (A.device, "A"), (B.device, "B")):
+            self._here(d, name)
+        if hasattr(bias, "data_ptr"):
+            if tuple(bias.shape) != (B.rows,) or str(bias.dtype) != "torch.float32" or not bias.is_contiguous() or not bias.is_cuda:
+                raise ValueError("bias: a contiguous float32 tensor [%d] on the device is needed" % B.rows)
+            self._here(bias.device.index, "bias")
+        w, wb = self._ws(ws)
+        self._check(self.lib.cp_matmul_blocks(self.h, ctypes.byref(A.c), ctypes.byref(B.c), _ptr(bias), p, c_dtype, ldc, w, wb),
+                    "cp_matmul_blocks")
+
+    def matmul_blocks_workspace(self, A, B, c_dtype, ldc=None):
+        n = ctypes.c_size_t()
+        self._check(self.lib.cp_matmul_blocks_workspace(ctypes.byref(A.c), ctypes.byref(B.c), c_dtype,
+                                                        max(B.rows, 1) if ldc is None else ldc, ctypes.byref(n)),
+                    "cp_matmul_blocks_workspace")
+        return n.value
+
+    # -- orthogonalised updates ------------------------------------------------------------------
+    @staticmethod
+    def _coef(coef, steps):
+        if coef is None:
+            return None
+        coef = np.ascontiguousarray(np.broadcast_to(np.asarray(coef, dtype=np.float64), (steps, 3)))
+        return coef
+
+    def orthogonalise(self, jobs, steps=5, coef=None, eps=1e-7, ws=None):
+        """O = the Newton-Schulz approximation of G's orthogonal polar factor, for every matrix of an OrthoJobs list in common
+        launches (cp_orthogonalise).  coef: (a, b, c) or one row per step; None = (3.4445, -4.7750, 2.0315)."""
+        self._here(jobs.device, "a job")
+        q = self._coef(coef, steps)
+        w, wb = self._ws(ws)
+        self._check(self.lib.cp_orthogonalise(self.h, jobs.n, jobs.c, steps, None if q is None else q.ctypes.data, eps, w, wb),
+                    "cp_orthogonalise")
+
+    def ortho_step(self, jobs, lr, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coef=None, eps=1e-7, ws=None):
+        """One optimiser step on every layer of an OrthoStepJobs list: momentum, orthogonalisation, decay, weights
+        (cp_ortho_step).  G is read, M and W are updated."""
+        self._here(jobs.device, "a job")
+        q = self._coef(coef, steps)
+        w, wb = self._ws(ws)
+        self._check(self.lib.cp_ortho_step(self.h, jobs.n, jobs.c, lr, momentum, int(nesterov), weight_decay, steps,
+                                           None if q is None else q.ctypes.data, eps, w, wb), "cp_ortho_step")
+
+    def ortho_workspace(self, jobs, steps=5, coef=None, eps=1e-7):
+        """Bytes of scratch that a call on these jobs (OrthoJobs or OrthoStepJobs) needs."""
+        return ortho_workspace(jobs, steps, coef, eps)
+
     def itq_iterate(self, feature, gt_feature, rank, iters=(30, 20), lambdas=(0.1, 1.0), pinv_cond=1e-6):
         """The alternations of ITQ_decompose on the device -> (T[n, n], Y_mean[n], U_mean[n]) as host arrays."""
         F = np.ascontiguousarray(feature, dtype=np.float64)
@@ -609,6 +834,18 @@ class Context:
         begin = (ctypes.c_float * CP_MAX_STAGES)()
         self._check(self.lib.cp_last_stage_spans(self.h, epoch_of.h, ctypes.byref(cnt), ms, begin), "cp_last_stage_spans")
         return [(self.lib.cp_stage_name(self.h, i).decode(), float(ms[i]), float(begin[i])) for i in range(cnt.value)]
+
+
+def ortho_workspace(jobs, steps=5, coef=None, eps=1e-7):
+    """Context.ortho_workspace without a context: checks the jobs like the call itself, needs no device."""
+    n = ctypes.c_size_t()
+    q = Context._coef(coef, steps)
+    lib = load()
+    fn = lib.cp_orthogonalise_workspace if isinstance(jobs, OrthoJobs) else lib.cp_ortho_step_workspace
+    rc = fn(jobs.n, jobs.c, steps, None if q is None else q.ctypes.data, eps, ctypes.byref(n))
+    if rc != 0:
+        raise CpError(rc, fn.__name__)
+    return n.value
 
 
 def device_count():

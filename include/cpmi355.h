@@ -42,6 +42,11 @@ extern "C" {
 
 #define CP_F32 0
 #define CP_F64 1
+/* the next four only where an entry point names them */
+#define CP_BF16 2
+#define CP_F16 3
+#define CP_E4M3 4 /* 8 bits, 4 of exponent, largest value 448, no infinity */
+#define CP_E5M2 5 /* 8 bits, 5 of exponent, largest value 57344 */
 
 typedef struct cp_ctx cp_ctx;
 
@@ -241,6 +246,80 @@ int cp_vh_project(cp_ctx *ctx, const void *X, int x_dtype, int64_t N, int c, int
 /* C[m,n] = A^T B, A DEVICE [k,m], B DEVICE [k,n], C DEVICE [m,n] (row-major f64, any sizes): the small
  * reconstructions V.dot(H) of decompose.py:114, 139. */
 int cp_matmul_tn(cp_ctx *ctx, const double *A, const double *B, int m, int n, int k, double *C);
+
+/* ---- 8-bit matrices with a scale per block, and their product --------------------------- */
+/* A matrix [rows, cols] held in 8-bit floating point, for the layers that a refit leaves: training passes and serving.
+ * Element (i, j) stands for q[i * ld + j] (fmt: CP_E4M3 or CP_E5M2) times the scale of its block, which is 128 consecutive
+ * columns of one row (tile = 1: activations, gradients) or of 128 rows (tile = 128: weights).  The last blocks may be cut.
+ *   q      DEVICE bytes, 16-byte aligned; ld: a multiple of 128, >= cols, < 2^22.  The bytes of a row from cols to the next
+ *          multiple of 128 have to be zero (cp_quant_blocks writes them); what lies behind them is not touched.
+ *   scale  DEVICE f32 [ceil(cols / 128)][lds], column block by column block; lds >= rows (tile 1) or ceil(rows / 128).
+ * No reference counterpart (Caffe layers are float32). */
+typedef struct cp_blocks {
+    void *q;
+    float *scale;
+    int64_t rows, cols, ld, lds;
+    int32_t fmt, tile;
+} cp_blocks;
+#define CP_QUANT_POW2 1 /* scales are rounded up to powers of two */
+/* Checks a description without a device (CP_OK, CP_ERR_ARG; q / scale may be null when rows or cols is 0). */
+int cp_blocks_check(const cp_blocks *m);
+/* x DEVICE [rows, cols] (x_dtype F32, F64, BF16 or F16, row stride ldx elements) -> out [rows, cols] and / or out_t
+ * [cols, rows], the transpose, from one read of x (either may be NULL).  Per block, in float32:
+ *   amax  = the largest |x| of its finite values, at least 2^-100;   scale = amax / fmax,  inverse = fmax / amax
+ *   (CP_QUANT_POW2: scale = the smallest power of two >= amax / fmax, inverse = 1 / scale);
+ *   q = x * inverse cut to +-fmax, rounded to nearest even.  A NaN or an infinity becomes NaN.
+ * F64 is rounded to float32 first.  Asynchronous on the context's stream, no workspace; can be captured. */
+int cp_quant_blocks(cp_ctx *ctx, const void *x, int x_dtype, int64_t rows, int64_t cols, int64_t ldx, int flags,
+                    const cp_blocks *out, const cp_blocks *out_t);
+/* C[i, j] = sum_k A[i, k] B[j, k] (+ bias[j]): A [M, K], B [N, K], C DEVICE [M, N] (c_dtype F32, BF16 or F16, row stride
+ * ldc elements), bias DEVICE f32 [N] or NULL.  With x [M, c k^2], w [n, c k^2], dy [M, n]: y = x w^T, dx = dy (w^T)^T,
+ * dw = dy^T (x^T)^T, the operands in the orientation that cp_quant_blocks' out / out_t give.  The products of a block are
+ * summed in float32 and joined in float32 times both scales; one rounding to c_dtype at the end.  (For BF16 the matrix unit
+ * adds products eight at a time, each cut below 2^-13 of the largest; F32 and F16 results keep all of float32.)  The order of the sums
+ * depends on the shape alone.  C must not overlap the operands.  K = 0: C = bias (or 0).  Asynchronous.
+ * ws: DEVICE scratch of cp_matmul_blocks_workspace() bytes, 256-byte aligned, or NULL: the context's own, which a call under
+ * stream capture refuses (a graph outlives it) -- give every captured call a workspace that no concurrent replay uses. */
+int cp_matmul_blocks(cp_ctx *ctx, const cp_blocks *A, const cp_blocks *B, const float *bias, void *C, int c_dtype,
+                     int64_t ldc, void *ws, size_t ws_bytes);
+/* The scratch that this product needs (0: none).  Checks the arguments like the call itself; needs no device. */
+int cp_matmul_blocks_workspace(const cp_blocks *A, const cp_blocks *B, int c_dtype, int64_t ldc, size_t *bytes);
+
+/* ---- orthogonalised updates ------------------------------------------------------------- */
+/* O = the Newton-Schulz approximation of the orthogonal polar factor of G (cp_svd_rows' U V^T without the SVD):
+ *   X = G / (|G|_F + eps);   `steps` times  X <- a X + b (X X^T) X + c (X X^T)^2 X
+ * coef HOST [steps][3] = (a, b, c) per step, or NULL: (3.4445, -4.7750, 2.0315), which brings singular values into about
+ * [0.7, 1.2].  G DEVICE [rows, cols] (g_dtype F32, BF16 or F16, row stride ldg), O DEVICE [rows, cols] (o_dtype likewise; may
+ * be G itself).  All jobs of a call run in common launches.  Products are carried with 22 bits of mantissa where the result
+ * is F32 or F16 and with 11 where it is BF16 (8), sums in float32, the norm in float64.  G = 0 gives O = 0; a NaN or an
+ * infinity in G makes that job's O NaN.  coef must keep |x| <= 1 below 16 in every step (checked), steps 1..32.  Outputs of
+ * a call must not overlap each other.  Asynchronous on the context's stream; ws as in cp_matmul_blocks. */
+typedef struct cp_ortho_job {
+    const void *G;
+    void *O;
+    int64_t ldg, ldo;
+    int32_t rows, cols, g_dtype, o_dtype;
+} cp_ortho_job;
+int cp_orthogonalise(cp_ctx *ctx, int n_jobs, const cp_ortho_job *jobs, int steps, const double *coef, double eps, void *ws,
+                     size_t ws_bytes);
+int cp_orthogonalise_workspace(int n_jobs, const cp_ortho_job *jobs, int steps, const double *coef, double eps, size_t *bytes);
+/* One optimiser step on a set of layers' weights:
+ *   M <- momentum M + G;   U = nesterov ? G + momentum M : M;   W <- (1 - lr weight_decay) W - lr gamma O(U)
+ * G DEVICE (g_dtype F32, BF16 or F16), M DEVICE f32 in/out, W DEVICE (w_dtype F32, BF16 or F16) in/out, all [rows, cols];
+ * gamma: the job's factor on lr (sqrt(max(1, rows / cols)) is usual).  O(U) as above, carried for W's type.  G, M and W must
+ * not overlap, nor the jobs' M and W each other.  Nothing is kept between calls but M. */
+typedef struct cp_ortho_step_job {
+    const void *G;
+    float *M;
+    void *W;
+    int64_t ldg, ldm, ldw;
+    int32_t rows, cols, g_dtype, w_dtype;
+    double gamma;
+} cp_ortho_step_job;
+int cp_ortho_step(cp_ctx *ctx, int n_jobs, const cp_ortho_step_job *jobs, double lr, double momentum, int nesterov,
+                  double weight_decay, int steps, const double *coef, double eps, void *ws, size_t ws_bytes);
+int cp_ortho_step_workspace(int n_jobs, const cp_ortho_step_job *jobs, int steps, const double *coef, double eps,
+                            size_t *bytes);
 
 /* ---- f2: ITQ_decompose (channel decomposition, lib/decompose.py:163-319) ---------------------------- */
 /* The 30 + 20 alternations of decompose.py:163-246 on the device: G = Y - mean, PGGt = pinv(G^T G, cond) G^T,

@@ -1,0 +1,315 @@
+"""Orthogonalised updates against float64.
+
+Tolerance.  The library rounds X, A and B of every step to `bits` of mantissa (11 where the result is bfloat16, 22 otherwise).
+`iterate(bits=)` does the same in float64 at the same places, with no kernel involved; its distance from the unrounded
+iteration is what that choice costs on these inputs, and the kernel's roundings, others of the same size, may cost four times
+that.  Its sums are float32 in an accumulator that the matrix unit cuts instead of rounding: a sum over K takes ceil(K / 32)
+additions (three times as many for pairs), each of which loses up to a step, 2^-23, of the partial sum, always towards zero, so
+that the losses of a diagonal entry add up: `iterate(loss=)` shortens every product by that much.  The error's root mean square
+is held to the sum of both and half a step of the output type, and no element may be twelve times as far (a Gaussian's largest
+of 10^7 lies at 5.3)."""
+import ctypes
+
+import numpy as np
+import pytest
+
+from cpmi355 import capi
+from lowbits import HALF, TYPES, Mat, from_bits, to_bits
+
+gpu = pytest.mark.gpu
+COEF = (3.4445, -4.7750, 2.0315)
+
+
+def cut(x, bits):
+    """x rounded to `bits` of mantissa, element by element."""
+    if bits is None:
+        return x
+    m, e = np.frexp(x)
+    return np.ldexp(np.rint(np.ldexp(m, bits)), e - bits)
+
+
+def iterate(U, steps=5, coef=None, eps=1e-7, bits=None, loss=0):
+    keep = lambda K: 1 - loss * -(-K // 32) * 2.0 ** -23
+    U = np.asarray(U, dtype=np.float64)
+    norm = np.sqrt((U * U).sum()) + eps
+    X = cut(U / norm if norm > 0 else U * 0, bits)
+    tall = X.shape[0] > X.shape[1]
+    X = X.T if tall else X
+    for k in range(steps):
+        a, b, c = COEF if coef is None else coef[k]
+        A = cut(X @ X.T * keep(X.shape[1]), bits)
+        B = cut(a * np.eye(len(A)) + b * A + c * (A @ A) * keep(len(A)), bits)
+        X = B @ X * keep(len(A))
+        if k + 1 < steps:
+            X = cut(X, bits)
+    return X.T if tall else X
+
+
+def bits_of(kind):
+    return 11 if kind == "bf16" else 22
+
+
+def distance(U, kind, **more):
+    """(the iteration in float64, how far the root mean square of the error may be, per element)"""
+    want = iterate(U, **more)
+    rms = lambda x: np.sqrt(((x - want) ** 2).mean())
+    return want, 4 * rms(iterate(U, bits=bits_of(kind), **more)) + rms(iterate(U, loss=1 if kind == "bf16" else 3, **more))
+
+
+def gradient(rs, rows, cols, scale=1e-3):
+    r = min(8, rows, cols)
+    return scale * (0.3 * rs.randn(rows, r) @ rs.randn(r, cols) + rs.randn(rows, cols))
+
+
+def within(got, want, far, kind):
+    assert got.shape == want.shape and np.isfinite(got).all()
+    rms = np.sqrt((want ** 2).mean())
+    err = got - want
+    half = HALF[kind] * np.abs(want) + 2.0 ** -25
+    assert np.sqrt((err ** 2).mean()) <= far + HALF[kind] * rms + 2.0 ** -25, (np.sqrt((err ** 2).mean()) / rms, far / rms)
+    assert (np.abs(err) <= 12 * far + half).all(), float((np.abs(err) - half).max() / max(far, 1e-300))
+
+
+# ---- refusals, no device -------------------------------------------------------------------------------------------------
+
+
+def job(rows=4, cols=6, G=4096, O=8192, gd=capi.CP_F32, od=capi.CP_F32, ldg=None, ldo=None):
+    return (G, gd, rows, cols, O, od, ldg or max(cols, 1), ldo or max(cols, 1))
+
+
+def step_job(rows=4, cols=6, G=4096, M=8192, W=16384, gd=capi.CP_F32, wd=capi.CP_F32, gamma=1.0, ldm=None):
+    return (G, gd, rows, cols, M, W, wd, gamma, None, ldm, None)
+
+
+def refuses(make, jobs, **kw):
+    with pytest.raises(capi.CpError):
+        capi.ortho_workspace(make(jobs), **kw)
+
+
+def test_jobs_are_checked():
+    O = capi.OrthoJobs
+    assert capi.ortho_workspace(O([job()])) > 0 and capi.ortho_workspace(O([])) == 0
+    assert capi.ortho_workspace(O([job(0, 6), job(4, 0)])) == 0
+    for bad in (job(rows=-1), job(gd=capi.CP_F64), job(od=capi.CP_E4M3), job(ldg=5), job(ldo=5), job(G=None), job(O=None),
+                job(G=4098), job(O=8193, od=capi.CP_BF16), job(rows=1 << 21), job(rows=70000, cols=70000)):
+        refuses(O, [bad])
+    refuses(O, [job(), job()])                                            # the same output twice
+    refuses(O, [job(), job(O=8192 + 4 * 23)])                             # its last element
+    capi.ortho_workspace(O([job(), job(O=8192 + 4 * 24)]))
+    capi.ortho_workspace(O([job(ldo=12), job(O=8192 + 4 * 6, ldo=12)]))   # two column halves of one matrix
+    refuses(O, [job(ldo=12), job(O=8192 + 4 * 5, ldo=12)])
+    capi.ortho_workspace(O([job(), job(O=4096)]))                         # one job's output is another's input: read first
+    for kw in (dict(steps=0), dict(steps=33), dict(eps=-1.0), dict(eps=np.nan), dict(coef=(np.nan, 0, 0)), dict(coef=(40.0, 0, 0)),
+               dict(coef=(3.4445, 4.7750, 2.0315))):
+        refuses(O, [job()], **kw)
+    for kw in (dict(steps=32), dict(coef=(1.5, -0.5, 0.0)), dict(coef=(1.875, -1.25, 0.375)), dict(coef=[(3, -3, 1)] * 5)):
+        assert capi.ortho_workspace(O([job()]), **kw) > 0
+    lib = capi.load()
+    assert lib.cp_orthogonalise_workspace(1, None, 5, None, 0.0, ctypes.byref(ctypes.c_size_t())) == -1
+    assert lib.cp_orthogonalise_workspace(-1, None, 5, None, 0.0, ctypes.byref(ctypes.c_size_t())) == -1
+    assert lib.cp_orthogonalise_workspace(0, None, 5, None, 0.0, None) == -1
+    assert lib.cp_orthogonalise(None, 0, None, 5, None, 0.0, None, 0) == -1
+    assert lib.cp_ortho_step(None, 0, None, 0.1, 0.9, 1, 0.0, 5, None, 0.0, None, 0) == -1
+
+
+def test_step_jobs_are_checked():
+    S = capi.OrthoStepJobs
+    assert capi.ortho_workspace(S([step_job()])) > 0
+    for bad in (step_job(M=None), step_job(W=None), step_job(M=8194), step_job(wd=capi.CP_F64), step_job(gamma=np.inf), step_job(ldm=5),
+                step_job(M=4096), step_job(W=4096), step_job(W=8192), step_job(G=8192 + 8)):
+        refuses(S, [bad])
+    refuses(S, [step_job(), step_job(M=32768)])
+    refuses(S, [step_job(), step_job(W=32768)])
+    capi.ortho_workspace(S([step_job(), step_job(M=32768, W=65536)]))     # one gradient, two layers
+    assert capi.OrthoStepJobs([(0, 0, 8, 2, 0, 0, 0)]).c[0].gamma == 2.0 and capi.OrthoStepJobs([(0, 0, 2, 8, 0, 0, 0)]).c[0].gamma == 1.0
+
+
+# ---- orthogonalise ---------------------------------------------------------------------------------------------------------
+
+SHAPES = [(1, 1), (1, 300), (300, 1), (2, 3), (27, 64), (64, 27), (63, 65), (64, 576), (128, 128), (129, 200), (200, 129), (55, 1000),
+          (512, 130), (257, 700)]
+
+
+@gpu
+@pytest.mark.parametrize("rows,cols", SHAPES)
+@pytest.mark.parametrize("gk,ok", [("f32", "f32"), ("bf16", "bf16"), ("f16", "f16"), ("bf16", "f32"), ("f32", "bf16")])
+def test_orthogonalise(ctx, rows, cols, gk, ok):
+    rs = np.random.RandomState(rows * 7 + cols)
+    G = Mat(ctx, gradient(rs, rows, cols, 1.0), gk, ld=cols + 3, lead=1)
+    O = Mat(ctx, np.zeros((rows, cols)), ok, ld=cols + 1, lead=5)
+    U = G.get()
+    ctx.orthogonalise(capi.OrthoJobs([(G.ptr, TYPES[gk], rows, cols, O.ptr, TYPES[ok], G.ld, O.ld)]))
+    within(O.get(), *distance(U, ok), ok)
+    assert O.untouched() and np.array_equal(G.raw(), G.before)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_many_matrices_in_one_call(ctx, kind):
+    """More than one launch's table, of mixed sizes and types, against each on its own: equal bits."""
+    rs = np.random.RandomState(3)
+    shapes = [(int(rs.randint(1, 150)), int(rs.randint(1, 200))) for _ in range(30)] + [(140, 400), (0, 5), (5, 0), (300, 150)]
+    kinds = [kind if i % 5 else "f16" for i in range(len(shapes))]
+    Gs = [Mat(ctx, gradient(rs, *s), k) for s, k in zip(shapes, kinds)]
+    together = [Mat(ctx, np.zeros(s), k) for s, k in zip(shapes, kinds)]
+    ctx.orthogonalise(capi.OrthoJobs([(G.ptr, TYPES[k], s[0], s[1], O.ptr, TYPES[k]) for G, O, s, k in zip(Gs, together, shapes, kinds)]))
+    for G, O, s, k in zip(Gs, together, shapes, kinds):
+        if not (s[0] and s[1]):
+            continue
+        one = Mat(ctx, np.zeros(s), k)
+        ctx.orthogonalise(capi.OrthoJobs([(G.ptr, TYPES[k], s[0], s[1], one.ptr, TYPES[k])]))
+        within(O.get(), *distance(G.get(), k), k)
+        assert np.array_equal(one.raw(), O.raw())
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("scale", [1e-30, 1e-12, 1.0, 1e18])
+def test_magnitudes(ctx, kind, scale):
+    rs = np.random.RandomState(4)
+    for rows, cols in ((40, 90), (150, 70)):
+        G, O = Mat(ctx, gradient(rs, rows, cols, scale), kind), Mat(ctx, np.zeros((rows, cols)), kind)
+        ctx.orthogonalise(capi.OrthoJobs([(G.ptr, TYPES[kind], rows, cols, O.ptr, TYPES[kind])]), eps=0.0)
+        within(O.get(), *distance(G.get(), kind, eps=0.0), kind)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_special_matrices(ctx, kind):
+    rs = np.random.RandomState(5)
+    zero = np.zeros((70, 130))
+    lowrank = rs.randn(70, 2) @ rs.randn(2, 130)
+    gone = gradient(rs, 70, 130)
+    gone[::3], gone[:, ::5] = 0, 0                              # rows and columns of channels that were pruned
+    spread = rs.randn(70, 130) * np.logspace(0, -6, 70)[:, None]
+    for a in (lowrank, gone, spread, np.eye(70, 130)):
+        for G in (a, a.T):
+            g, o = Mat(ctx, G, kind), Mat(ctx, np.ones(G.shape), kind)
+            ctx.orthogonalise(capi.OrthoJobs([(g.ptr, TYPES[kind], G.shape[0], G.shape[1], o.ptr, TYPES[kind])]))
+            within(o.get(), *distance(g.get(), kind), kind)
+            if a is gone:
+                assert (o.get()[g.get() == 0].reshape(-1)[:1] == 0).all() and (np.abs(o.get()[(g.get() == 0).all(1)]) == 0).all()
+    for eps in (0.0, 1e-7):
+        g, o = Mat(ctx, zero, kind), Mat(ctx, np.ones(zero.shape), kind)
+        ctx.orthogonalise(capi.OrthoJobs([(g.ptr, TYPES[kind], 70, 130, o.ptr, TYPES[kind])]), eps=eps)
+        assert (o.get() == 0).all()
+    for v in (np.nan, np.inf, -np.inf):
+        bad = gradient(rs, 70, 130)
+        bad[3, 100] = v
+        g, o = Mat(ctx, bad, kind), Mat(ctx, np.zeros(bad.shape), kind)
+        g2, o2 = Mat(ctx, gone, kind), Mat(ctx, np.zeros(gone.shape), kind)
+        ctx.orthogonalise(capi.OrthoJobs([(g.ptr, TYPES[kind], 70, 130, o.ptr, TYPES[kind]), (g2.ptr, TYPES[kind], 70, 130, o2.ptr, TYPES[kind])]))
+        assert np.isnan(o.get()).all() and np.isfinite(o2.get()).all()
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("steps,coef", [(1, None), (2, None), (10, None), (12, (1.5, -0.5, 0.0)), (8, (1.875, -1.25, 0.375)), (3, (0.0, 0.0, 1.0)),
+                                        (2, (4.0, -1.0, 0.0))])
+def test_steps_and_coefficients(ctx, kind, steps, coef):
+    rs = np.random.RandomState(6)
+    coef = None if coef is None else [coef] * steps
+    for rows, cols in ((60, 100), (140, 90)):
+        G, O = Mat(ctx, gradient(rs, rows, cols), kind), Mat(ctx, np.zeros((rows, cols)), kind)
+        ctx.orthogonalise(capi.OrthoJobs([(G.ptr, TYPES[kind], rows, cols, O.ptr, TYPES[kind])]), steps=steps, coef=coef)
+        within(O.get(), *distance(G.get(), kind, steps=steps, coef=coef), kind)
+
+
+@gpu
+def test_converged_factor_is_the_polar_factor(ctx):
+    """With coefficients that converge, U V^T of the singular value decomposition: 20 cubic steps bring 1e-2 to one."""
+    rs = np.random.RandomState(7)
+    G = rs.randn(96, 160)
+    g, o = Mat(ctx, G, "f32"), Mat(ctx, np.zeros(G.shape), "f32")
+    ctx.orthogonalise(capi.OrthoJobs([(g.ptr, 0, 96, 160, o.ptr, 0)]), steps=20, coef=(1.5, -0.5, 0.0))
+    u, _, v = np.linalg.svd(g.get(), full_matrices=False)
+    _, far = distance(g.get(), "f32", steps=20, coef=[(1.5, -0.5, 0.0)] * 20)
+    within(o.get(), u @ v, far + 1e-9, "f32")
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_in_place_and_shared_input(ctx, kind):
+    rs = np.random.RandomState(8)
+    for rows, cols in ((50, 80), (150, 140)):
+        G, O, P = (Mat(ctx, gradient(rs, rows, cols), kind) for _ in range(3))
+        U = G.get()
+        T = TYPES[kind]
+        ctx.orthogonalise(capi.OrthoJobs([(G.ptr, T, rows, cols, O.ptr, T), (G.ptr, T, rows, cols, P.ptr, T), (O.ptr, T, rows, cols, G.ptr, T)]))
+        assert np.array_equal(O.raw(), P.raw())
+        within(O.get(), *distance(U, kind), kind)
+        H = Mat(ctx, U, kind)
+        ctx.orthogonalise(capi.OrthoJobs([(H.ptr, T, rows, cols, H.ptr, T)]))
+        assert np.array_equal(H.get(), O.get())
+
+
+@gpu
+def test_repeats_its_bits_on_any_workspace(ctx):
+    rs = np.random.RandomState(9)
+    G, O, P = (Mat(ctx, gradient(rs, 260, 500), "f32") for _ in range(3))
+    jo, jp = (capi.OrthoJobs([(G.ptr, 0, 260, 500, o.ptr, 0)]) for o in (O, P))
+    need = ctx.ortho_workspace(jp)
+    ws = ctx.to_device(np.full(need, 0xff, dtype=np.uint8))               # every number of it a NaN
+    ctx.orthogonalise(jo)
+    ctx.orthogonalise(jp, ws=ws)
+    assert np.array_equal(O.raw(), P.raw())
+    lib = ctx.lib
+    assert lib.cp_orthogonalise(ctx.h, 1, jp.c, 5, None, 0.0, ws.ptr, need - 1) == -1
+    assert lib.cp_orthogonalise(ctx.h, 1, jp.c, 5, None, 0.0, ws.ptr + 128, need) == -1
+
+
+# ---- the step --------------------------------------------------------------------------------------------------------------
+
+
+def step(G, M, W, kind, lr, momentum, nesterov, decay, gamma, **more):
+    """-> (M, W, how far W's root mean square may be)"""
+    M = momentum * M + G
+    U = G + momentum * M if nesterov else M
+    O, far = distance(U, kind, **more)
+    return M, (1 - lr * decay) * W - lr * gamma * O, abs(lr * gamma) * far
+
+
+@gpu
+@pytest.mark.parametrize("rows,cols", [(1, 1), (5, 300), (300, 5), (64, 495), (130, 140), (257, 130)])
+@pytest.mark.parametrize("gk,wk", [("f32", "f32"), ("bf16", "bf16"), ("bf16", "f32"), ("f16", "f16")])
+@pytest.mark.parametrize("nesterov", [True, False])
+def test_step(ctx, rows, cols, gk, wk, nesterov):
+    rs = np.random.RandomState(rows + 3 * cols)
+    G, M = Mat(ctx, gradient(rs, rows, cols), gk, ld=cols + 2), Mat(ctx, gradient(rs, rows, cols), "f32", ld=cols + 1, lead=1)
+    W = Mat(ctx, 0.05 * rs.randn(rows, cols), wk, ld=cols + 4, lead=3)
+    g, m, w = G.get(), M.get(), W.get()
+    jobs = capi.OrthoStepJobs([(G.ptr, TYPES[gk], rows, cols, M.ptr, W.ptr, TYPES[wk], None, G.ld, M.ld, W.ld)])
+    for _ in range(2):
+        m2, w2, far = step(g, m, w, wk, 0.02, 0.95, nesterov, 0.1, max(1, rows / cols) ** 0.5)
+        ctx.ortho_step(jobs, 0.02, momentum=0.95, nesterov=nesterov, weight_decay=0.1)
+        # one fused multiply-add in float32, of a float32 factor
+        assert (np.abs(M.get() - m2) <= 2.0 ** -24 * np.abs(m2) + 2.0 ** -24 * np.abs(m) + 1e-30).all()
+        # W: two float32 factors (each off by half a step), a product and a fused multiply-add, and the type's rounding
+        slack = 4 * 2.0 ** -24 * (np.abs(w) + np.abs(w2))
+        err = np.abs(W.get() - w2)
+        assert (err <= 12 * far + slack + HALF[wk] * np.abs(w2) + 2.0 ** -25).all()
+        assert np.sqrt((err ** 2).mean()) <= far + np.sqrt(((slack + HALF[wk] * np.abs(w2)) ** 2).mean()) + 2.0 ** -25
+        m, w = M.get(), W.get()
+    assert M.untouched() and W.untouched() and np.array_equal(G.raw(), G.before)
+
+
+@gpu
+def test_pruned_channels_stay_zero(ctx):
+    """Zero rows and columns in G, M and W (channels that were taken out) are zero after the step."""
+    rs = np.random.RandomState(2)
+    a = gradient(rs, 60, 90)
+    a[::4], a[:, 1::3] = 0, 0
+    G, M, W = Mat(ctx, a, "f32"), Mat(ctx, a * 2, "f32"), Mat(ctx, a * 50, "f32")
+    ctx.ortho_step(capi.OrthoStepJobs([(G.ptr, 0, 60, 90, M.ptr, W.ptr, 0)]), 0.1, weight_decay=0.01)
+    assert (W.get()[a == 0] == 0).all() and (M.get()[a == 0] == 0).all() and (W.get()[a != 0] != 0).any()
+
+
+@gpu
+def test_step_of_nothing_changes_only_by_decay(ctx):
+    W = Mat(ctx, np.full((3, 4), 0.5), "f32")
+    G, M = Mat(ctx, np.zeros((3, 4)), "f32"), Mat(ctx, np.zeros((3, 4)), "f32")
+    ctx.ortho_step(capi.OrthoStepJobs([(G.ptr, 0, 3, 4, M.ptr, W.ptr, 0)]), 0.5, weight_decay=0.5)
+    assert (W.get() == 0.375).all() and (M.get() == 0).all()
+    ctx.ortho_step(capi.OrthoStepJobs([]), 0.5)
+    with pytest.raises(capi.CpError):
+        ctx.ortho_step(capi.OrthoStepJobs([]), np.inf)
