@@ -1,5 +1,6 @@
 // Matrices held in 8-bit floating point with one scale per block of 128 (cp_blocks), the cast that makes them and their product.
 #include <cfloat>
+#include <cmath>
 
 #include "cp_common.h"
 #include "nt_mfma.h"
@@ -202,98 +203,205 @@ struct Product {
     void *c;
     int64_t sa_step, sb_step, ldc;   // scale strides per block column
     uint32_t lda, ldb;
-    int M, N, steps, tiles_m, tiles_n;
+    int M, N, steps, tiles_m, tiles_n, pieces;
     int a_shift, b_shift;            // row -> scale: 0 (one per row) or 7
     int c_dtype, c_vec;
+    float *parts;
+    int *counts;
 };
 
-__device__ __forceinline__ void store_c(const Product &p, int64_t i, int j, f4 v) {
-    if (p.bias) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (j + r < p.N) v[r] += p.bias[j + r];
-    }
+__device__ __forceinline__ void store4(const Product &p, int64_t i, int j, f4 v) {
     const int64_t at = i * p.ldc + j;
-    if (p.c_vec && j + 4 <= p.N) {
-        if (p.c_dtype == CP_F32) {
-            *reinterpret_cast<f4 *>(static_cast<float *>(p.c) + at) = v;
-        } else if (p.c_dtype == CP_BF16) {
-            typedef __bf16 b4 __attribute__((ext_vector_type(4)));
-            *reinterpret_cast<b4 *>(static_cast<__bf16 *>(p.c) + at) = __builtin_convertvector(v, b4);
-        } else {
-            *reinterpret_cast<nt::h4 *>(static_cast<_Float16 *>(p.c) + at) = __builtin_convertvector(v, nt::h4);
+    if (p.c_dtype == CP_F32) {
+        *reinterpret_cast<f4 *>(static_cast<float *>(p.c) + at) = v;
+    } else if (p.c_dtype == CP_BF16) {
+        typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+        *reinterpret_cast<b4 *>(static_cast<__bf16 *>(p.c) + at) = __builtin_convertvector(v, b4);
+    } else {
+        *reinterpret_cast<nt::h4 *>(static_cast<_Float16 *>(p.c) + at) = __builtin_convertvector(v, nt::h4);
+    }
+}
+__device__ __forceinline__ void store1(const Product &p, int64_t i, int j, float v) {
+    const int64_t at = i * p.ldc + j;
+    if (p.c_dtype == CP_F32) static_cast<float *>(p.c)[at] = v;
+    else if (p.c_dtype == CP_BF16) static_cast<__bf16 *>(p.c)[at] = __bf16(v);
+    else static_cast<_Float16 *>(p.c)[at] = _Float16(v);
+}
+
+// A wave's part of C [16 WI rows from i0, 16 WJ columns from j0].  Where four neighbours cannot be stored at once, sixteen rows
+// at a time go through LDS (`own`: the wave's), so that lanes hold neighbours: single stores of 16 lanes' different rows took
+// 126 us more on a 20000 x 4005 product in bfloat16.
+template <int WI, int WJ>
+__device__ __forceinline__ void write_c(const Product &p, const f4 (&acc)[WI][WJ], float *own, int i0, int j0, int lane) {
+    if (p.c_vec) {
+        f4 bias[WJ];
+#pragma unroll
+        for (int wj = 0; wj < WJ; ++wj) {
+            const int j = j0 + wj * 16 + (lane >> 4) * 4;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) bias[wj][r] = p.bias && j + r < p.N ? p.bias[j + r] : 0.f;
+        }
+#pragma unroll
+        for (int wi = 0; wi < WI; ++wi) {
+            const int i = i0 + wi * 16 + (lane & 15);
+            if (i >= p.M) continue;
+#pragma unroll
+            for (int wj = 0; wj < WJ; ++wj) {
+                const int j = j0 + wj * 16 + (lane >> 4) * 4;
+                const f4 v = acc[wi][wj] + bias[wj];
+                if (j + 4 <= p.N) store4(p, i, j, v);
+                else
+                    for (int r = 0; r < 3; ++r)
+                        if (j + r < p.N) store1(p, i, j + r, v[r]);
+            }
         }
         return;
     }
+    constexpr int W = WJ * 16, LD = W + 4, AT_ONCE = 64 / W, N = 16 / AT_ONCE;
+    const int j = j0 + lane % W;
+    const float bias = p.bias && j < p.N ? p.bias[j] : 0.f;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        if (j + r >= p.N) return;
-        if (p.c_dtype == CP_F32) static_cast<float *>(p.c)[at + r] = v[r];
-        else if (p.c_dtype == CP_BF16) static_cast<__bf16 *>(p.c)[at + r] = __bf16(v[r]);
-        else static_cast<_Float16 *>(p.c)[at + r] = _Float16(v[r]);
+    for (int wi = 0; wi < WI; ++wi) {
+        const int i = i0 + wi * 16 + lane / W;
+        if (i0 + wi * 16 >= p.M) break;
+#pragma unroll
+        for (int wj = 0; wj < WJ; ++wj) *reinterpret_cast<f4 *>(own + (lane & 15) * LD + wj * 16 + (lane >> 4) * 4) = acc[wi][wj];
+#pragma unroll
+        for (int r = 0; r < N; ++r) {
+            const float v = own[(r * AT_ONCE + lane / W) * LD + lane % W] + bias;
+            if (i + r * AT_ONCE < p.M && j < p.N) store1(p, i + r * AT_ONCE, j, v);
+        }
     }
 }
 
-template <int BM, int BN, int NWM, int NWN, int FA, int FB, bool COMMON, bool WIDE>
-__global__ void __launch_bounds__(64 * NWM * NWN) k_matmul_blocks(Product p) {
-    constexpr int T = 64 * NWM * NWN, WI = BM / NWM / 16, WJ = BN / NWN / 16;
-    static_assert((BM + BN) / 64 == NWM * NWN, "one wave per 64 scales");
-    static_assert(!COMMON || (128 % (16 * WJ) == 0 && BN % 128 == 0), "a wave's columns share their scale");
-    __shared__ alignas(1024) char a0[BM * 128], a1[BM * 128], b0[BN * 128], b1[BN * 128];
-    __shared__ alignas(1024) float s0[BM + BN], s1[BM + BN];
+template <class CFG, int FA, int FB, bool COMMON, bool WIDE>
+__global__ void __launch_bounds__(CFG::T) k_matmul_blocks(Product p) {
+    constexpr int BM = CFG::BM, BN = CFG::BN, T = CFG::T, WI = CFG::WI, WJ = CFG::WJ;
+    static_assert((BM + BN) / 64 <= CFG::NWM * CFG::NWN, "one wave per 64 scales");
+    static_assert(!COMMON || 128 % (16 * WJ) == 0, "a wave's columns share their scale");
+    static_assert(CFG::NWM * CFG::NWN * 16 * (WJ * 16 + 4) * 4 <= CFG::STAGE, "LDS");
+    NT_STAGES(st, CFG::STAGES, CFG::STAGE + (BM + BN) * 4);
+    __shared__ int flag;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wm = wave / NWN, wn = wave % NWN;
-    const int tile = nt::xcd_order(blockIdx.x, p.tiles_m * p.tiles_n);
-    const int tm = tile % p.tiles_m, tn = tile / p.tiles_m;
+    const int wm = wave / CFG::NWN, wn = wave % CFG::NWN;
+    const int at = nt::xcd_order(blockIdx.x, gridDim.x), tiles = p.tiles_m * p.tiles_n, piece = at / tiles, tile = at % tiles;
+    const int k0 = int(int64_t(p.steps) * piece / p.pieces), k1 = int(int64_t(p.steps) * (piece + 1) / p.pieces);
+    int tm, tn;
+    nt::tile_at(tile, p.tiles_m, p.tiles_n, tm, tn);
     const int i0 = tm * BM, j0 = tn * BN;
 
     nt::Loader<BM, T> la;
     nt::Loader<BN, T> lb;
-    la.init(p.a + int64_t(i0) * p.lda, p.lda, p.M - i0, tid);
-    lb.init(p.b + int64_t(j0) * p.ldb, p.ldb, p.N - j0, tid);
-    const bool for_a = wave < BM / 64;
+    la.init(p.a + int64_t(i0) * p.lda + int64_t(k0) * 128, p.lda, p.M - i0, tid);
+    lb.init(p.b + int64_t(j0) * p.ldb + int64_t(k0) * 128, p.ldb, p.N - j0, tid);
+    // the step's scales, 64 to a wave; waves without any load the last ones again (every wave waits for as many loads)
+    const int sw = wave < (BM + BN) / 64 ? wave : (BM + BN) / 64 - 1;
     const float *sp;
     int64_t s_step;
-    if (for_a) {
-        const int r = i0 + wave * 64 + lane;
+    if (sw < BM / 64) {
+        const int r = i0 + sw * 64 + lane;
         sp = p.sa + ((r < p.M ? r : p.M - 1) >> p.a_shift);
         s_step = p.sa_step;
     } else {
-        const int r = j0 + (wave - BM / 64) * 64 + lane;
+        const int r = j0 + (sw - BM / 64) * 64 + lane;
         sp = p.sb + ((r < p.N ? r : p.N - 1) >> p.b_shift);
         s_step = p.sb_step;
     }
+    sp += k0 * s_step;
     f4 acc[WI][WJ];
 #pragma unroll
     for (int i = 0; i < WI; ++i)
 #pragma unroll
         for (int j = 0; j < WJ; ++j) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
     const int ra = wm * WI * 16, rb = wn * WJ * 16;
+    if (k1 > k0) nt::pipeline<CFG::STAGES, CFG::LOADS + 1, CFG::PARTS>(
+        st, k1 - k0,
+        [&](int k, char *s, int part, int parts) {
+            if (part == 0) nt::load_lds4(sp + k * s_step, reinterpret_cast<float *>(s + CFG::STAGE) + sw * 64);
+            la.issue(k, s, wave, part, parts);
+            lb.issue(k, s + BM * 128, wave, part, parts);
+        },
+        [&](const char *s, auto between) {
+            const float *sc = reinterpret_cast<const float *>(s + CFG::STAGE);
+            nt::products8<WI, WJ, FA, FB, COMMON, WIDE>(s + ra * 128, s + (BM + rb) * 128, sc + ra, sc + BM + rb, lane, acc, between);
+        });
+    if (p.pieces > 1 && !nt::join<T>(acc, piece, p.pieces, p.parts + int64_t(tile) * (BM * BN), tiles, p.counts + tile, &flag, tid)) return;
+    write_c<WI, WJ>(p, acc, reinterpret_cast<float *>(st[0]) + wave * 16 * (WJ * 16 + 4), i0 + ra, j0 + rb, lane);
+}
 
-    auto fetch = [&](int k, char *a, char *b, float *s) {
-        la.issue(k, a, wave);
-        lb.issue(k, b, wave);
-        nt::load_lds4(sp + k * s_step, s + wave * 64);
-    };
-    auto compute = [&](const char *a, const char *b, const float *s) {
-        nt::products8<WI, WJ, FA, FB, COMMON, WIDE>(a + ra * 128, b + rb * 128, s + ra, s + BM + rb, lane, acc);
-    };
-    if (p.steps > 0) fetch(0, a0, b0, s0);
-    for (int k = 0; k < p.steps; k += 2) {
-        nt::stage_barrier();
-        if (k + 1 < p.steps) fetch(k + 1, a1, b1, s1);
-        compute(a0, b0, s0);
-        if (k + 1 >= p.steps) break;
-        nt::stage_barrier();
-        if (k + 2 < p.steps) fetch(k + 2, a0, b0, s0);
-        compute(a1, b1, s1);
+// Few rows of A: bound by reading B once.  A workgroup takes sixteen rows of B and its eight waves an eighth of k each, straight
+// from memory into the matrix instruction's registers (a lane holds 32 bytes of one row: the K order within a block is the same
+// for A and B, and that is all that a sum needs); their sums are added in the order of k.
+template <int MT, int FA, int FB, bool COMMON, bool WIDE>
+__global__ void __launch_bounds__(512) k_matmul_blocks_rows(Product p) {
+    __shared__ alignas(16) float sum[8][MT][64][4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int j0 = blockIdx.x * 16, jr = j0 + (lane & 15), o = (lane >> 4) * 16;
+    const char *b = p.b + int64_t(jr < p.N ? jr : p.N - 1) * p.ldb + o;
+    const char *a[MT];
+    const float *sa[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        const int i = min(m * 16 + (lane & 15), p.M - 1);
+        a[m] = p.a + int64_t(i) * p.lda + o;
+        sa[m] = p.sa + (i >> p.a_shift);
+    }
+    const float *sb[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) sb[r] = p.sb + (min(j0 + (lane >> 4) * 4 + r, p.N - 1) >> p.b_shift);
+    const int k0 = p.steps * wave / 8, k1 = p.steps * (wave + 1) / 8;
+    f4 acc[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[m] = f4{0.f, 0.f, 0.f, 0.f};
+    constexpr int U = MT == 1 ? 4 : 2;   // blocks whose loads are under way together
+    for (int k = k0; k < k1; k += U) {
+        nt::i4v qb[U][2], qa[U][MT][2];
+        float sj[U][4], si[U][MT];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t kb = k + u < k1 ? k + u : k1 - 1;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) qb[u][h] = *reinterpret_cast<const nt::i4v *>(b + kb * 128 + h * 64);
+#pragma unroll
+            for (int r = 0; r < (COMMON ? 1 : 4); ++r) sj[u][r] = sb[r][kb * p.sb_step];
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) qa[u][m][h] = *reinterpret_cast<const nt::i4v *>(a[m] + kb * 128 + h * 64);
+                si[u][m] = sa[m][kb * p.sa_step];
+            }
+        }
+        NT_STAY();
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (k + u >= k1) break;
+            nt::Frag8<FB, WIDE> fb;
+            fb.set(qb[u][0], qb[u][1]);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                nt::Frag8<FA, WIDE> fa;
+                fa.set(qa[u][m][0], qa[u][m][1]);
+                const f4 t = nt::block_product<FA, FB, WIDE>(fa, fb);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[m][r] = fmaf(t[r], si[u][m] * sj[u][COMMON ? 0 : r], acc[m][r]);
+            }
+        }
     }
 #pragma unroll
-    for (int i = 0; i < WI; ++i) {
-        const int row = i0 + ra + i * 16 + (lane & 15);
-        if (row >= p.M) continue;
+    for (int m = 0; m < MT; ++m) *reinterpret_cast<f4 *>(sum[wave][m][lane]) = acc[m];
+    __syncthreads();
+    for (int u = tid; u < MT * 64; u += 512) {
+        const int m = u >> 6, l = u & 63, i = m * 16 + (l & 15), j = j0 + (l >> 4) * 4;
+        f4 v = *reinterpret_cast<const f4 *>(sum[0][m][l]);
+        for (int w = 1; w < 8; ++w) v += *reinterpret_cast<const f4 *>(sum[w][m][l]);
+        if (i >= p.M) continue;
 #pragma unroll
-        for (int j = 0; j < WJ; ++j) store_c(p, row, j0 + rb + j * 16 + (lane >> 4) * 4, acc[i][j]);
+        for (int r = 0; r < 4; ++r)
+            if (p.bias && j + r < p.N) v[r] += p.bias[j + r];
+        if (p.c_vec && j + 4 <= p.N) store4(p, i, j, v);
+        else
+            for (int r = 0; r < 4; ++r)
+                if (j + r < p.N) store1(p, i, j + r, v[r]);
     }
 }
 
@@ -304,21 +412,74 @@ int check_product(cp_ctx *ctx, const cp_blocks *A, const cp_blocks *B, int c_dty
         return cp_set_error(ctx, CP_ERR_ARG, "A has %lld columns, B %lld", (long long)A->cols, (long long)B->cols);
     if (c_dtype != CP_F32 && c_dtype != CP_BF16 && c_dtype != CP_F16) return cp_set_error(ctx, CP_ERR_ARG, "c_dtype %d", c_dtype);
     if (ldc < B->rows) return cp_set_error(ctx, CP_ERR_ARG, "ldc %lld < %lld", (long long)ldc, (long long)B->rows);
-    if (((A->rows + 127) / 128) * ((B->rows + 127) / 128) >= (int64_t(1) << 31))
-        return cp_set_error(ctx, CP_ERR_UNSUPPORTED, "C is too large");
+    if (((A->rows + 63) / 64) * ((B->rows + 63) / 64) >= (int64_t(1) << 31)) return cp_set_error(ctx, CP_ERR_UNSUPPORTED, "C is too large");
     return CP_OK;
 }
 
+// How a product is formed: by its shape, its types and C's type alone
+struct Form {
+    int cfg;             // 0 Large, 1 Medium, 2 Small, 3 few rows
+    int tiles_m, tiles_n, pieces;
+    size_t counts, parts;   // bytes
+};
+constexpr int kMaxJoined = 16384;   // workgroups of a launch that joins pieces
+constexpr int kChip = 256;          // CUs that a split is planned for
+
+bool wide_form(int c_dtype) { return c_dtype != CP_BF16; }   // what the 8-bit matrix instructions drop is below bfloat16's rounding only
+
+Form form_of(const cp_blocks *A, const cp_blocks *B, int c_dtype) {
+    // us per step and workgroup on a full chip / with at most one to a CU, beside the steps, and for a join; [wide][cfg]
+    static const double full[2][3] = {{2.2, 1.1, 0.36}, {1e3, 1.75, 0.6}}, alone[2][3] = {{1.9, 0.85, 0.26}, {1e3, 1.4, 0.45}};
+    static const double extra[3] = {8.0, 5.0, 3.5}, joined[3] = {12.0, 5.0, 3.0};
+    const int64_t steps = (A->cols + 127) / 128;
+    const bool wide = wide_form(c_dtype);
+    Form best = {};
+    const int forced = cp_knob(CP_KNOB_NT_TILE);
+    if (A->rows <= 32 && !forced) return {3, 0, 0, 1, 0, 0};
+    double least = 1e300;
+    for (int cfg = wide ? 1 : 0; cfg < 3; ++cfg) {
+        if (forced && forced - 1 != cfg && !(wide && forced == 1 && cfg == 1)) continue;
+        const int64_t edge = 256 >> cfg, tm = (A->rows + edge - 1) / edge, tn = (B->rows + edge - 1) / edge;
+        for (int p = 1; p <= 32 && (p == 1 || (steps / p >= 4 && tm * tn * p <= kMaxJoined)); ++p) {
+            const double groups = double(tm) * tn * p, rounds = std::ceil(groups / (cfg == 0 ? kChip : 2 * kChip));
+            const double step = groups > kChip ? full[wide][cfg] : alone[wide][cfg];
+            const double cost = rounds * ((steps + p - 1) / p * step + extra[cfg] + (p > 1 ? joined[cfg] : 0.0));
+            if (cost < 0.97 * least) {
+                least = cost;
+                best = {cfg, int(tm), int(tn), p, 0, 0};
+                if (p > 1) {
+                    best.counts = cp_align_up(size_t(tm * tn) * sizeof(int), 256);
+                    best.parts = size_t(tm * tn * p) * edge * edge * sizeof(float);
+                }
+            }
+        }
+    }
+    return best;
+}
+
+__global__ void __launch_bounds__(256) k_zero(int *p, int n) {
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < n; i += gridDim.x * 256) p[i] = 0;
+}
+
 template <int FA, int FB, bool COMMON, bool WIDE>
-void launch_product(cp_ctx *ctx, const Product &p) {
-    k_matmul_blocks<128, 128, 2, 2, FA, FB, COMMON, WIDE><<<p.tiles_m * p.tiles_n, 256, 0, ctx->stream>>>(p);
+void launch_product(cp_ctx *ctx, const Product &p, const Form &f) {
+    const int n = f.tiles_m * f.tiles_n * f.pieces;
+    if (f.cfg == 3) {
+        if (p.M <= 16) k_matmul_blocks_rows<1, FA, FB, COMMON, WIDE><<<(p.N + 15) / 16, 512, 0, ctx->stream>>>(p);
+        else k_matmul_blocks_rows<2, FA, FB, COMMON, WIDE><<<(p.N + 15) / 16, 512, 0, ctx->stream>>>(p);
+        return;
+    }
+    if constexpr (!WIDE)   // the widened fragments of 256 x 256 do not fit into registers
+        if (f.cfg == 0) return (void)(k_matmul_blocks<nt::Large, FA, FB, COMMON, WIDE><<<n, nt::Large::T, 0, ctx->stream>>>(p));
+    if (f.cfg <= 1) k_matmul_blocks<nt::Medium, FA, FB, COMMON, WIDE><<<n, nt::Medium::T, 0, ctx->stream>>>(p);
+    else k_matmul_blocks<nt::Small, FA, FB, COMMON, WIDE><<<n, nt::Small::T, 0, ctx->stream>>>(p);
 }
 
 template <int FA, int FB>
-void launch_product(cp_ctx *ctx, const Product &p) {
-    const bool wide = p.c_dtype != CP_BF16;   // what the 8-bit matrix instructions drop is below bfloat16's rounding only
-    if (p.b_shift) wide ? launch_product<FA, FB, true, true>(ctx, p) : launch_product<FA, FB, true, false>(ctx, p);
-    else wide ? launch_product<FA, FB, false, true>(ctx, p) : launch_product<FA, FB, false, false>(ctx, p);
+void launch_product(cp_ctx *ctx, const Product &p, const Form &f) {
+    const bool wide = wide_form(p.c_dtype);
+    if (p.b_shift) wide ? launch_product<FA, FB, true, true>(ctx, p, f) : launch_product<FA, FB, true, false>(ctx, p, f);
+    else wide ? launch_product<FA, FB, false, true>(ctx, p, f) : launch_product<FA, FB, false, false>(ctx, p, f);
 }
 
 }  // namespace
@@ -360,7 +521,8 @@ extern "C" int cp_quant_blocks(cp_ctx *ctx, const void *x, int x_dtype, int64_t 
 extern "C" int cp_matmul_blocks_workspace(const cp_blocks *A, const cp_blocks *B, int c_dtype, int64_t ldc, size_t *bytes) {
     if (!bytes) return CP_ERR_ARG;
     CP_TRY(check_product(nullptr, A, B, c_dtype, ldc));
-    *bytes = 0;
+    const Form f = form_of(A, B, c_dtype);
+    *bytes = f.counts + f.parts;
     return CP_OK;
 }
 
@@ -371,8 +533,19 @@ extern "C" int cp_matmul_blocks(cp_ctx *ctx, const cp_blocks *A, const cp_blocks
     if (!A->rows || !B->rows) return CP_OK;
     const size_t size = c_dtype == CP_F32 ? 4 : 2;
     if (!C || uintptr_t(C) % size || uintptr_t(bias) % 4) return cp_set_error(ctx, CP_ERR_ARG, "C is null or misaligned");
-    (void)ws, (void)ws_bytes;
     CP_HIP(ctx, hipSetDevice(ctx->device));
+    const Form f = form_of(A, B, c_dtype);
+    char *scratch = nullptr;
+    if (f.pieces > 1) {
+        CP_TRY(cp_scratch(ctx, ws, ws_bytes, f.counts + f.parts, &scratch));
+        if (!ws && !ctx->nt_cnt) {   // the context's own counters are zero between launches
+            int *c = nullptr;
+            CP_HIP(ctx, hipMalloc(reinterpret_cast<void **>(&c), kMaxJoined * sizeof(int)));
+            k_zero<<<16, 256, 0, ctx->stream>>>(c, kMaxJoined);
+            ctx->nt_cnt = c;
+        }
+        if (ws) k_zero<<<1, 256, 0, ctx->stream>>>(reinterpret_cast<int *>(scratch), f.tiles_m * f.tiles_n);
+    }
     Product p = {};
     p.a = static_cast<const char *>(A->q);
     p.b = static_cast<const char *>(B->q);
@@ -388,17 +561,20 @@ extern "C" int cp_matmul_blocks(cp_ctx *ctx, const cp_blocks *A, const cp_blocks
     p.M = int(A->rows);
     p.N = int(B->rows);
     p.steps = int((A->cols + 127) / 128);
-    p.tiles_m = (p.M + 127) / 128;
-    p.tiles_n = (p.N + 127) / 128;
+    p.tiles_m = f.tiles_m;
+    p.tiles_n = f.tiles_n;
+    p.pieces = f.pieces;
+    p.counts = ws ? reinterpret_cast<int *>(scratch) : ctx->nt_cnt;
+    p.parts = reinterpret_cast<float *>(scratch + f.counts);
     p.a_shift = A->tile == 1 ? 0 : 7;
     p.b_shift = B->tile == 1 ? 0 : 7;
     p.c_dtype = c_dtype;
     p.c_vec = ldc % 4 == 0 && uintptr_t(C) % (4 * size) == 0;
     const bool a5 = A->fmt == CP_E5M2, b5 = B->fmt == CP_E5M2;
-    if (a5 && b5) launch_product<1, 1>(ctx, p);
-    else if (a5) launch_product<1, 0>(ctx, p);
-    else if (b5) launch_product<0, 1>(ctx, p);
-    else launch_product<0, 0>(ctx, p);
+    if (a5 && b5) launch_product<1, 1>(ctx, p, f);
+    else if (a5) launch_product<1, 0>(ctx, p, f);
+    else if (b5) launch_product<0, 1>(ctx, p, f);
+    else launch_product<0, 0>(ctx, p, f);
     CP_LAUNCH_CHECK(ctx);
     return CP_OK;
 }

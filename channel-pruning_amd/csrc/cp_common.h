@@ -108,6 +108,7 @@ struct cp_ctx {
     int cu_count = 256;
     int *gemm_cnt = nullptr;          // arrival counters of the split tiles of cp_gemm_tn_f64 (a ring of regions, zero between launches)
     int gemm_cnt_next = 0;
+    int *nt_cnt = nullptr;            // arrival counters of cp_matmul_blocks, zero between launches
     bool defer_refit_wait = false;    // cp_prune_layers: enqueue the refit, the caller waits once for the whole batch
     bool refit_pending = false;       // set by a deferred refit: factor + solve still to be launched by the batch
     cp_refit_deferred deferred = {};
@@ -128,7 +129,9 @@ struct cp_ctx {
 };
 
 // process-wide experiment switches (cp_debug_knob; cp_ctx.hip): plain ints, 0 by default, read when work is enqueued
-enum { CP_KNOB_SPLIT_XTY = 0, CP_KNOB_CHOL_PHASES = 1, CP_KNOB_CHOL_WG = 2, CP_KNOB_COUNT = 8 };
+enum { CP_KNOB_SPLIT_XTY = 0, CP_KNOB_CHOL_PHASES = 1, CP_KNOB_CHOL_WG = 2,
+       CP_KNOB_NT_TILE = 3,   // ortho.hip, blocks8.hip: 1 + the tile shape of every product (0: by rule)
+       CP_KNOB_COUNT = 8 };
 int cp_knob(int id);
 
 int cp_set_error(cp_ctx *ctx, int code, const char *fmt, ...);
@@ -168,6 +171,9 @@ static inline T *cp_arena_take_t(cp_ctx *ctx, size_t count) {
 }
 static inline size_t cp_align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 int cp_pinned_reserve(cp_ctx *ctx, size_t bytes);
+// the scratch of a call that takes a workspace: the caller's (checked), or the context's arena, which a captured call must not
+// use (a graph outlives what the arena holds now)
+int cp_scratch(cp_ctx *ctx, void *ws, size_t ws_bytes, size_t need, char **out);
 
 // stage timing -----------------------------------------------------------------------
 void cp_stage_begin(cp_ctx *ctx);                   // start of a top-level call

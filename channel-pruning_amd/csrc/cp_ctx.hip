@@ -137,6 +137,7 @@ extern "C" int cp_ctx_destroy(cp_ctx *ctx) {
     if (ctx->layer_ws) hipFree(ctx->layer_ws);
     if (ctx->cd_box) hipFree(ctx->cd_box);
     if (ctx->gemm_cnt) hipFree(ctx->gemm_cnt);
+    if (ctx->nt_cnt) hipFree(ctx->nt_cnt);
     if (ctx->pinned) hipHostFree(ctx->pinned);
     if (ctx->stage) hipHostFree(ctx->stage);
     if (ctx->ev_upload) hipEventDestroy(ctx->ev_upload);
@@ -236,6 +237,22 @@ void *cp_arena_take(cp_ctx *ctx, size_t bytes) {
     if (off + bytes > ctx->arena_bytes) return nullptr;
     ctx->arena_used = off + bytes;
     return ctx->arena + off;
+}
+
+int cp_scratch(cp_ctx *ctx, void *ws, size_t ws_bytes, size_t need, char **out) {
+    if (ws) {
+        if (uintptr_t(ws) % 256) return cp_set_error(ctx, CP_ERR_ARG, "workspace is not 256-byte aligned");
+        if (ws_bytes < need) return cp_set_error(ctx, CP_ERR_ARG, "workspace of %zu bytes, %zu needed", ws_bytes, need);
+        *out = static_cast<char *>(ws);
+        return CP_OK;
+    }
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    CP_HIP(ctx, hipStreamIsCapturing(ctx->stream, &st));
+    if (st != hipStreamCaptureStatusNone)
+        return cp_set_error(ctx, CP_ERR_ARG, "a captured call needs a workspace of its own (%zu bytes)", need);
+    CP_TRY(cp_arena_reserve(ctx, need));
+    *out = static_cast<char *>(cp_arena_take(ctx, need));
+    return *out ? CP_OK : cp_set_error(ctx, CP_ERR_NOMEM, "arena");
 }
 
 int cp_pinned_reserve(cp_ctx *ctx, size_t bytes) {

@@ -11,13 +11,19 @@
 // The accumulators come out of the matrix instruction as (four consecutive rows, one column) per lane, so B feeds its row side
 // and A its column side: a lane then owns four consecutive j of one i, a vector store in row-major C.
 //
-// Two LDS stages, each in its own __shared__ array so that the compiler can tell a load into one from reads of the other (and
-// inserts no wait between them); one barrier per K step, after which the next step's loads are issued before this step's
-// products: they have a whole step (2000 cycles at 256 x 256) to arrive.
+// STAGES LDS stages, each in its own __shared__ array so that the compiler can tell a load into one from reads of the others
+// (and inserts no wait between them); one barrier per K step, behind which the loads of a step STAGES - 1 ahead are issued.
+// A tile that fills the chip alone needs two stages (a step of 256 x 256 takes 2000 cycles); few small tiles are bound by the
+// latency of their loads (0.8 us from a cold L2) and take more.
+//
+// A tile with a long k and few tiles beside it is cut into pieces of k (their number follows from the product's shape alone)
+// that several workgroups form; the one that arrives last adds them in the order of k.  The result does not depend on who
+// that is, and nobody waits for anybody.
 #pragma once
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 namespace nt {
 
@@ -36,13 +42,65 @@ __device__ __forceinline__ void load_lds4(const float *g, float *l) {
                                      (__attribute__((address_space(3))) void *)l, 4, 0, 0);
 }
 
-// every load into LDS that this wave issued has landed, its LDS reads are done, and so are the other waves'
+// at most N of this wave's loads are still under way, its LDS reads are done, and both hold for the other waves
+template <int N>
 __device__ __forceinline__ void stage_barrier() {
+    static_assert(N < 64, "vmcnt has six bits");
     asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x0070);   // vmcnt(0) lgkmcnt(0)
+    __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | ((N >> 4) << 14));   // vmcnt(N) lgkmcnt(0)
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
+template <int STAGES, int U, class Step>
+__device__ __forceinline__ void rest(int n, Step step) {
+    if constexpr (U < STAGES - 1) {
+        if (n <= U) return;
+        step(std::integral_constant<int, U>());
+        rest<STAGES, U + 1>(n, step);
+    }
+}
+
+// `steps` K steps: fetch(k, stage, part, parts) issues a share of a step's loads (LOADS per thread in all), compute(stage,
+// between) uses a step's and calls between(i) among its products, where the first PARTS calls issue the shares.  Ends with a barrier.
+// Every path through the loop issues the same loads (the last step's again where there is no further one): the compiler
+// counts them along paths, not values, and would wait for all of them otherwise.
+template <int STAGES, int LOADS, int PARTS, class Fetch, class Compute>
+__device__ __forceinline__ void pipeline(char *const (&st)[8], int steps, Fetch fetch, Compute compute) {
+    const int last = steps - 1;
+    auto step = [&](int k, int u) {
+        stage_barrier<LOADS *(STAGES - 2)>();
+        const int next = k + STAGES - 1, n = next < last ? next : last;
+        compute(st[u], [&](int i) { if (i < PARTS) fetch(n, st[(u + STAGES - 1) % STAGES], i, PARTS); });
+    };
+#pragma unroll
+    for (int u = 0; u < STAGES - 1; ++u) fetch(u < last ? u : last, st[u], 0, 1);
+    int k = 0;
+    // whole rounds of the stages, then the rest: a loop that can be left in its middle keeps the accumulators twice
+    for (; k + STAGES <= steps; k += STAGES) {
+#pragma unroll
+        for (int u = 0; u < STAGES; ++u) step(k + u, u);
+    }
+    rest<STAGES, 0>(steps - k, [&](auto u) { step(k + u.value, u.value); });
+    stage_barrier<0>();
+}
+// the stages' arrays, `bytes` each
+#define NT_STAGES(name, n, bytes)                                                                                        \
+    __shared__ alignas(1024) char name##0[bytes], name##1[(n) > 1 ? (bytes) : 16], name##2[(n) > 2 ? (bytes) : 16],      \
+        name##3[(n) > 3 ? (bytes) : 16], name##4[(n) > 4 ? (bytes) : 16], name##5[(n) > 5 ? (bytes) : 16],               \
+        name##6[(n) > 6 ? (bytes) : 16], name##7[(n) > 7 ? (bytes) : 16];                                                \
+    char *const name[8] = {name##0, name##1, name##2, name##3, name##4, name##5, name##6, name##7}
+
+// A tile shape: BM x BN by NWM x NWN waves
+template <int BM_, int BN_, int NWM_, int NWN_, int STAGES_>
+struct Tile {
+    static constexpr int BM = BM_, BN = BN_, NWM = NWM_, NWN = NWN_, STAGES = STAGES_;
+    static constexpr int T = 64 * NWM * NWN, WI = BM / NWM / 16, WJ = BN / NWN / 16;
+    static constexpr int STAGE = (BM + BN) * 128, LOADS = STAGE / 16 / T;
+    static constexpr int PARTS = WI >= 8 ? 4 : 1;
+};
+typedef Tile<256, 256, 2, 4, 2> Large;    // 132 KB of LDS, one workgroup to a CU
+typedef Tile<128, 128, 2, 2, 2> Medium;   // 64 KB, two
+typedef Tile<64, 64, 2, 2, 4> Small;      // 64 KB, two
 
 // One operand's share of the loads: ROWS rows of 128 bytes by THREADS threads, 16 bytes each
 template <int ROWS, int THREADS>
@@ -62,42 +120,58 @@ struct Loader {
             off[i] = uint32_t(r) * ld + chunk * 16;
         }
     }
-    __device__ __forceinline__ void issue(int64_t step, char *lds, int wave) const {
+    // the part-th of `parts` shares of a step's loads
+    __device__ __forceinline__ void issue(int64_t step, char *lds, int wave, int part, int parts) const {
         const char *g = base + step * 128;
 #pragma unroll
-        for (int i = 0; i < N; ++i) load_lds16(g + off[i], lds + (i * THREADS + wave * 64) * 16);
+        for (int i = 0; i < N; ++i)
+            if (i * parts / N == part) load_lds16(g + off[i], lds + (i * THREADS + wave * 64) * 16);
     }
 };
 
 // per-lane byte offset of chunk (lane >> 4) + 4 h of row (lane & 15) of a 16-row group
 __device__ __forceinline__ int frag_off(int lane, int h) { return (lane & 15) * 128 + ((((lane >> 4) + 4 * h) ^ (lane & 7)) << 4); }
 
-template <int WI, int WJ>
-__device__ __forceinline__ void products16(const char *a, const char *b, int lane, f4 (&acc)[WI][WJ], bool split) {
+// A step's products.  A row group's fragments are read one group ahead of their use, and the next step's loads are issued
+// among the products (`between`): the barriers of the compiler's scheduler keep both where they stand, or it gathers the reads
+// at the top of the step, where both waves of a SIMD then wait for them at once (1.7 us instead of ... a 256 x 256 step).
+#define NT_STAY() __builtin_amdgcn_sched_barrier(0)
+
+template <int WI, int WJ, bool SPLIT, class Between>
+__device__ __forceinline__ void products16(const char *a, const char *b, int lane, f4 (&acc)[WI][WJ], Between between) {
     const int o0 = frag_off(lane, 0), o1 = frag_off(lane, 1);
-    h8 b0[WJ], b1[WJ];
+    h8 b0[WJ], b1[WJ], a0[2], a1[2];
+    a0[0] = *reinterpret_cast<const h8 *>(a + o0);
+    a1[0] = *reinterpret_cast<const h8 *>(a + o1);
 #pragma unroll
     for (int j = 0; j < WJ; ++j) {
         b0[j] = *reinterpret_cast<const h8 *>(b + j * 2048 + o0);
         b1[j] = *reinterpret_cast<const h8 *>(b + j * 2048 + o1);
     }
+    NT_STAY();
 #pragma unroll
     for (int i = 0; i < WI; ++i) {
-        const h8 a0 = *reinterpret_cast<const h8 *>(a + i * 2048 + o0);
-        const h8 a1 = *reinterpret_cast<const h8 *>(a + i * 2048 + o1);
-        if (split) {   // (high + low) (high + low) without low * low, which is below the pair's own rounding
+        const int u = i & 1;
+        if (i + 1 < WI) {
+            a0[u ^ 1] = *reinterpret_cast<const h8 *>(a + (i + 1) * 2048 + o0);
+            a1[u ^ 1] = *reinterpret_cast<const h8 *>(a + (i + 1) * 2048 + o1);
+        }
+        between(i);
+        NT_STAY();
+        if (SPLIT) {   // (high + low) (high + low) without low * low, which is below the pair's own rounding
 #pragma unroll
-            for (int j = 0; j < WJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b1[j], a0, acc[i][j], 0, 0, 0);
+            for (int j = 0; j < WJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b1[j], a0[u], acc[i][j], 0, 0, 0);
 #pragma unroll
-            for (int j = 0; j < WJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b0[j], a1, acc[i][j], 0, 0, 0);
+            for (int j = 0; j < WJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b0[j], a1[u], acc[i][j], 0, 0, 0);
 #pragma unroll
-            for (int j = 0; j < WJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b0[j], a0, acc[i][j], 0, 0, 0);
+            for (int j = 0; j < WJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b0[j], a0[u], acc[i][j], 0, 0, 0);
         } else {
 #pragma unroll
-            for (int j = 0; j < WJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b0[j], a0, acc[i][j], 0, 0, 0);
+            for (int j = 0; j < WJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b0[j], a0[u], acc[i][j], 0, 0, 0);
 #pragma unroll
-            for (int j = 0; j < WJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b1[j], a1, acc[i][j], 0, 0, 0);
+            for (int j = 0; j < WJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b1[j], a1[u], acc[i][j], 0, 0, 0);
         }
+        NT_STAY();
     }
 }
 
@@ -123,7 +197,9 @@ struct Frag8 {
     i8v v;
     h8 w[4];
     __device__ __forceinline__ void load(const char *rows, int o0, int o1) {
-        const i4v c0 = *reinterpret_cast<const i4v *>(rows + o0), c1 = *reinterpret_cast<const i4v *>(rows + o1);
+        set(*reinterpret_cast<const i4v *>(rows + o0), *reinterpret_cast<const i4v *>(rows + o1));
+    }
+    __device__ __forceinline__ void set(i4v c0, i4v c1) {
         if (WIDE) {
             widen<FMT>(c0, reinterpret_cast<h8(&)[2]>(w[0]));
             widen<FMT>(c1, reinterpret_cast<h8(&)[2]>(w[2]));
@@ -133,42 +209,143 @@ struct Frag8 {
     }
 };
 
+// the products of one block of sixteen rows of A and of B, from zero
+template <int FA, int FB, bool WIDE>
+__device__ __forceinline__ f4 block_product(const Frag8<FA, WIDE> &a, const Frag8<FB, WIDE> &b) {
+    f4 z = {0.f, 0.f, 0.f, 0.f};
+    if (WIDE) {
+#pragma unroll
+        for (int h = 0; h < 4; ++h) z = __builtin_amdgcn_mfma_f32_16x16x32_f16(b.w[h], a.w[h], z, 0, 0, 0);
+    } else {
+        z = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b.v, a.v, z, FB, FA, 0, 0, 0, 0);
+    }
+    return z;
+}
+
 // The 8-bit step: the products of one block of 128 start from zero and join the accumulators times both blocks' scales.
 // sa [16 WI] and sb ([16 WJ], or one value where COMMON) are this wave's scales of the step.
 // WIDE: the 8-bit matrix instructions align the eight products of a group to the largest and drop what lies below 2^-13 of
 // its power of two (measured: 2^16 + 4 gives 2^16 within a group, 2^16 + 8 is exact, and across groups all of float32 counts).
 // A bfloat16 result rounds off 2^-8 and takes them as they are; float32 and fp16 results are formed with the fp16
 // instructions, which keep float32's bits at half the rate.
-template <int WI, int WJ, int FA, int FB, bool COMMON, bool WIDE>
+template <int WI, int WJ, int FA, int FB, bool COMMON, bool WIDE, class Between>
 __device__ __forceinline__ void products8(const char *a, const char *b, const float *sa, const float *sb, int lane,
-                                          f4 (&acc)[WI][WJ]) {
+                                          f4 (&acc)[WI][WJ], Between between) {
     const int o0 = frag_off(lane, 0), o1 = frag_off(lane, 1);
     Frag8<FB, WIDE> bf[WJ];
-    f4 sj[WJ];
+    Frag8<FA, WIDE> af[2];
+    f4 sj[WJ], t[2][WJ];
+    float si[2];
+    const float common = COMMON ? sb[0] : 1.f;
+    auto join = [&](int i) {   // a row group's products join the accumulators while the next one's are formed
+#pragma unroll
+        for (int j = 0; j < WJ; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                acc[i][j][r] = fmaf(t[i & 1][j][r], COMMON ? si[i & 1] : si[i & 1] * sj[j][r], acc[i][j][r]);
+    };
+    af[0].load(a, o0, o1);
+    si[0] = sa[lane & 15] * common;
 #pragma unroll
     for (int j = 0; j < WJ; ++j) {
         bf[j].load(b + j * 2048, o0, o1);
         if (!COMMON) sj[j] = *reinterpret_cast<const f4 *>(sb + j * 16 + (lane >> 4) * 4);
     }
-    const float common = COMMON ? sb[0] : 1.f;
+    NT_STAY();
 #pragma unroll
     for (int i = 0; i < WI; ++i) {
-        Frag8<FA, WIDE> af;
-        af.load(a + i * 2048, o0, o1);
-        const float si = sa[i * 16 + (lane & 15)] * common;
+        const int u = i & 1;
+        if (i + 1 < WI) af[u ^ 1].load(a + (i + 1) * 2048, o0, o1);
+        between(i);
+        NT_STAY();
 #pragma unroll
-        for (int j = 0; j < WJ; ++j) {
-            f4 t = {0.f, 0.f, 0.f, 0.f};
-            if (WIDE) {
-#pragma unroll
-                for (int h = 0; h < 4; ++h) t = __builtin_amdgcn_mfma_f32_16x16x32_f16(bf[j].w[h], af.w[h], t, 0, 0, 0);
-            } else {
-                t = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bf[j].v, af.v, t, FB, FA, 0, 0, 0, 0);
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(t[r], COMMON ? si : si * sj[j][r], acc[i][j][r]);
-        }
+        for (int j = 0; j < WJ; ++j) t[u][j] = block_product<FA, FB, WIDE>(af[u], bf[j]);
+        if (i > 0) join(i - 1);
+        if (i + 1 < WI) si[u ^ 1] = sa[(i + 1) * 16 + (lane & 15)] * common;
+        NT_STAY();
     }
+    join(WI - 1);
+}
+
+// ---- tiles that several workgroups share ---------------------------------------------------------------------------------
+// Parts are stored through to where every XCD sees them (sc1), waited for, and announced by a relaxed counter; the last to
+// arrive reads them the same way.  No fence is needed around these.
+typedef unsigned int u4v __attribute__((ext_vector_type(4)));
+constexpr int kSc1 = 16;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t slot_of(float *p, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(p, 0, bytes, 0x00027000);
+}
+__device__ __forceinline__ void put(__amdgpu_buffer_rsrc_t slot, int at, f4 v) {
+    u4v q;
+    __builtin_memcpy(&q, &v, 16);
+    __builtin_amdgcn_raw_buffer_store_b128(q, slot, at, 0, kSc1);
+}
+__device__ __forceinline__ f4 take(__amdgpu_buffer_rsrc_t slot, int at) {
+    const u4v q = __builtin_amdgcn_raw_buffer_load_b128(slot, at, 0, kSc1);
+    f4 v;
+    __builtin_memcpy(&v, &q, 16);
+    return v;
+}
+
+// This workgroup's acc is one of n pieces of a tile; piece q's slot lies at parts + q * apart tiles' sizes.  Returns whether
+// this workgroup holds the whole tile in acc now.  `flag`: one int of LDS, `count`: the tile's counter, zero before and after.
+template <int T, int WI, int WJ>
+__device__ __forceinline__ bool join(f4 (&acc)[WI][WJ], int piece, int n, float *parts, int64_t apart, int *count, int *flag, int tid) {
+    constexpr int SLOT = T * WI * WJ * 4;   // numbers
+    const __amdgpu_buffer_rsrc_t mine = slot_of(parts + piece * apart * SLOT, SLOT * 4);
+#pragma unroll
+    for (int i = 0; i < WI; ++i)
+#pragma unroll
+        for (int j = 0; j < WJ; ++j) put(mine, ((i * WJ + j) * T + tid) * 16, acc[i][j]);
+    stage_barrier<0>();
+    if (tid == 0) {
+        const int seen = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const bool last = seen == n - 1;
+        if (last) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *flag = last;
+    }
+    __syncthreads();
+    const bool last = *flag != 0;
+    __syncthreads();
+    if (!last) return false;
+    for (int q = 0; q < n; ++q) {
+        const __amdgpu_buffer_rsrc_t p = slot_of(parts + q * apart * SLOT, SLOT * 4);
+#pragma unroll
+        for (int i = 0; i < WI; ++i)
+#pragma unroll
+            for (int j = 0; j < WJ; ++j) {
+                const f4 v = take(p, ((i * WJ + j) * T + tid) * 16);
+                acc[i][j] = q == 0 ? v : acc[i][j] + v;
+            }
+    }
+    return true;
+}
+
+// ---- the order of tiles --------------------------------------------------------------------------------------------------
+// Neighbours in the order share operand rows in their XCD's L2: bands of eight tile rows, column by column
+__device__ __forceinline__ void tile_at(int t, int tiles_m, int tiles_n, int &tm, int &tn) {
+    const int band = t / (8 * tiles_n), first = band * 8, h = tiles_m - first < 8 ? tiles_m - first : 8;
+    const int r = t - first * tiles_n;
+    tm = first + r % h;
+    tn = r / h;
+}
+// the tiles on and below the diagonal: bands of four rows, column by column.  Band b begins at tile 8 b^2 + 2 b.
+__device__ __forceinline__ void lower_tile_at(int t, int tiles, int &tm, int &tn) {
+    int b = int((sqrtf(8.f * t + 1.f) - 1.f) * 0.125f);
+    while (b > 0 && 8 * b * b + 2 * b > t) --b;
+    while (8 * (b + 1) * (b + 1) + 2 * (b + 1) <= t) ++b;
+    const int first = 4 * b, h = tiles - first < 4 ? tiles - first : 4;
+    int r = t - (8 * b * b + 2 * b);
+    if (r < first * h) {
+        tm = first + r % h;
+        tn = r / h;
+        return;
+    }
+    r -= first * h;
+    int c = 0;
+    while (r >= h - c) r -= h - c++;
+    tn = first + c;
+    tm = tn + r;
 }
 
 // Workgroups are handed to the eight XCDs in turn; this maps the launch order so that each XCD works on a run of

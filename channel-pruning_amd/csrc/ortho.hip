@@ -21,10 +21,11 @@ using nt::f4;
 using nt::h4;
 using nt::h8;
 
-constexpr int kJobs = 24;        // jobs of one launch: their table travels in the kernel's arguments (4 KB)
+constexpr int kJobs = 20;        // jobs whose records one launch carries in its arguments (4 KB)
 constexpr int kMaxSteps = 32;
-constexpr int kPartials = 256;   // partial sums of |U|_F^2 per job
-constexpr int kTile = 128;
+constexpr int kCus = 256;        // the chip's CUs: what the split of a launch is planned for (results do not depend on the real number)
+constexpr int kPartials = 512;   // partial sums of |U|_F^2 per job, at most
+constexpr int kPad = 64;         // both sides are padded to this (and the tiles' loads repeat the last row beyond it)
 constexpr double kDefault[3] = {3.4445, -4.7750, 2.0315};
 
 struct Job {
@@ -34,18 +35,44 @@ struct Job {
     char *x, *xt0, *xt1, *a, *b; // X [mp][np], X^T [np][mp] twice, A and B [mp][mp]
     double *part;
     int64_t ldg, ldm, ldo;
+    int64_t sum_cols;            // |U|: a row's length, the whole matrix' where it is contiguous
     uint32_t ldn, lds;           // bytes of a row of np / of mp numbers
     int rows, cols, mp, np;
-    int g_dtype, o_dtype;
+    int sum_rows, rows_per, width, chunks;   // |U|: rows, and rows, columns that a workgroup sums, chunks of columns
+    int16_t g_dtype, o_dtype;
+    int16_t vec_in, vec_sum, vec_out;   // whether eight numbers of G and M / four of the output can be moved at once
     float lr;                    // lr * gamma
-    int first_sym, first_apply, first_load;   // this job's first workgroup of the phase
+};
+
+// The phases' launches: job k's first workgroup of each, and the pieces of k that its tiles are cut into
+enum { LOAD, GRAM, POLY, APPLY, PHASES };
+struct Place {
+    int first[PHASES];
+    int16_t pieces[PHASES];
+};
+
+// A call's jobs in its workspace.  The first kernel carries them in its arguments and writes them there.
+struct Table {
+    Job *job;
+    int *first[PHASES];
+    int *pieces[PHASES];
+    int n;
 };
 
 struct Jobs {
-    int n, total_sym, total_apply, total_load;
+    int n, base;                 // job[0] is the call's job `base`
+    int first[kJobs];            // this job's first workgroup of the launch
+    Place place[kJobs];
     Job job[kJobs];
 };
 static_assert(sizeof(Jobs) <= 3900, "kernel arguments");
+
+// the job whose workgroups include `at`; every wave looks for itself
+__device__ __forceinline__ int find_job(const int *first, int n, int at) {
+    int k = 0;
+    for (int i = threadIdx.x & 63; i - int(threadIdx.x & 63) < n; i += 64) k += __popcll(__ballot(i < n && first[i] <= at));
+    return __builtin_amdgcn_readfirstlane(k - 1);
+}
 
 __device__ __forceinline__ float load_as_float(const void *p, int dtype, int64_t at) {
     if (dtype == CP_F32) return static_cast<const float *>(p)[at];
@@ -57,38 +84,103 @@ __device__ __forceinline__ void store_as(void *p, int dtype, int64_t at, float v
     else if (dtype == CP_BF16) static_cast<__bf16 *>(p)[at] = __bf16(v);
     else static_cast<_Float16 *>(p)[at] = _Float16(v);
 }
+typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f4 load4_as_float(const void *p, int dtype, int64_t at) {
+    if (dtype == CP_F32) return *reinterpret_cast<const f4 *>(static_cast<const float *>(p) + at);
+    if (dtype == CP_BF16) return __builtin_convertvector(*reinterpret_cast<const b4 *>(static_cast<const __bf16 *>(p) + at), f4);
+    return __builtin_convertvector(*reinterpret_cast<const h4 *>(static_cast<const _Float16 *>(p) + at), f4);
+}
+__device__ __forceinline__ void store4_as(void *p, int dtype, int64_t at, f4 v) {
+    if (dtype == CP_F32) *reinterpret_cast<f4 *>(static_cast<float *>(p) + at) = v;
+    else if (dtype == CP_BF16) *reinterpret_cast<b4 *>(static_cast<__bf16 *>(p) + at) = __builtin_convertvector(v, b4);
+    else *reinterpret_cast<h4 *>(static_cast<_Float16 *>(p) + at) = __builtin_convertvector(v, h4);
+}
+
+// eight numbers of a row from column c, zero from `cols` on
+__device__ __forceinline__ void load8(const void *row, int dtype, int c, int cols, bool vec, float (&v)[8]) {
+    if (vec && c + 8 <= cols) {
+        if (dtype == CP_F32) {
+            const f4 *p = reinterpret_cast<const f4 *>(static_cast<const float *>(row) + c);
+            const f4 a = p[0], b = p[1];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = a[e], v[e + 4] = b[e];
+        } else if (dtype == CP_BF16) {
+            typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+            const b8 a = *reinterpret_cast<const b8 *>(static_cast<const __bf16 *>(row) + c);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = float(a[e]);
+        } else {
+            const h8 a = *reinterpret_cast<const h8 *>(static_cast<const _Float16 *>(row) + c);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = float(a[e]);
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? load_as_float(row, dtype, c + e) : 0.f;
+}
+
+__device__ __forceinline__ const void *row_of(const void *p, int dtype, int64_t at) {
+    return static_cast<const char *>(p) + at * (dtype == CP_F32 ? 4 : 2);
+}
 
 __device__ __forceinline__ double wave_sum(double v) {
     for (int s = 32; s; s >>= 1) v += __shfl_xor(v, s);
     return v;
 }
 
-// ---- |U|_F, and the momentum -----------------------------------------------------------------------------------------------
-__global__ void __launch_bounds__(256) k_ortho_norm(Jobs js, float momentum, int nesterov) {
-    const Job &j = js.job[blockIdx.y];
-    double sum = 0.0;
-    for (int r = blockIdx.x; r < j.rows; r += kPartials)
-        for (int c = threadIdx.x; c < j.cols; c += 256) {
-            float u = load_as_float(j.G, j.g_dtype, r * j.ldg + c);
-            if (j.M) {
-                float *m = j.M + r * j.ldm + c;
-                const float v = fmaf(momentum, *m, u);
-                *m = v;
-                u = nesterov ? fmaf(momentum, v, u) : v;
-            }
-            sum += double(u) * double(u);
+// ---- |U|_F, and the momentum: one pass over G (and M), bound by HBM -----------------------------------------------------------
+// A workgroup sums rows_per rows of a chunk of `width` columns; the partial sums are added in one order by whoever needs the
+// norm.  Contiguous matrices are one row: their own rows' lengths would leave most of them unaligned.
+__global__ void __launch_bounds__(256) k_ortho_norm(Jobs js, Table t, float momentum, int nesterov, int *counts, int n_counts) {
+    int which = 0;
+#pragma unroll
+    for (int i = 1; i < kJobs; ++i) which += i < js.n && js.first[i] <= int(blockIdx.x);
+    const Job &j = js.job[which];
+    const int id = blockIdx.x - js.first[which];
+    if (id == 0) {   // this job's record, for the kernels that follow
+        const int *from = reinterpret_cast<const int *>(&j);
+        int *to = reinterpret_cast<int *>(t.job + js.base + which);
+        for (int i = threadIdx.x; i < int(sizeof(Job) / 4); i += 256) to[i] = from[i];
+        if (threadIdx.x < PHASES) {
+            t.first[threadIdx.x][js.base + which] = js.place[which].first[threadIdx.x];
+            t.pieces[threadIdx.x][js.base + which] = js.place[which].pieces[threadIdx.x];
         }
+    }
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < n_counts; i += gridDim.x * 256) counts[i] = 0;
+    const int r0 = id / j.chunks * j.rows_per, r1 = min(r0 + j.rows_per, j.sum_rows);
+    const int64_t c0 = int64_t(id % j.chunks) * j.width;
+    const int wide = int(min(j.sum_cols - c0, int64_t(j.width))), eights = (wide + 7) / 8;
+    double sum = 0.0;
+    for (int u = threadIdx.x; u < (r1 - r0) * eights; u += 256) {
+        const int k = r1 - r0 > 1 ? u / eights : 0, r = r0 + k, c = (u - k * eights) * 8;
+        float v[8];
+        load8(row_of(j.G, j.g_dtype, r * j.ldg + c0), j.g_dtype, c, wide, j.vec_sum, v);
+        if (j.M) {
+            float *row = j.M + r * j.ldm + c0, m[8];
+            load8(row, CP_F32, c, wide, j.vec_sum, m);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                m[e] = fmaf(momentum, m[e], v[e]);
+                v[e] = nesterov ? fmaf(momentum, m[e], v[e]) : m[e];
+            }
+            if (j.vec_sum && c + 8 <= wide) {
+                *reinterpret_cast<f4 *>(row + c) = f4{m[0], m[1], m[2], m[3]};
+                *reinterpret_cast<f4 *>(row + c + 4) = f4{m[4], m[5], m[6], m[7]};
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (c + e < wide) row[c + e] = m[e];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = fma(double(v[e]), double(v[e]), sum);
+    }
     __shared__ double s[4];
     sum = wave_sum(sum);
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = sum;
     __syncthreads();
-    if (threadIdx.x == 0) j.part[blockIdx.x] = (s[0] + s[1]) + (s[2] + s[3]);
-}
-
-__device__ __forceinline__ int find_job(const Jobs &js, int id, int Job::*first) {
-    int k = js.n - 1;
-    while (k > 0 && js.job[k].*first > id) --k;
-    return k;
+    if (threadIdx.x == 0) j.part[id] = (s[0] + s[1]) + (s[2] + s[3]);
 }
 
 // sixteen numbers of a row, from column k (a multiple of 16), as fp16 or as pairs
@@ -117,13 +209,6 @@ __device__ __forceinline__ void store4(char *row, int k, f4 v) {
     if (SPLIT) *reinterpret_cast<h4 *>(p + 64) = __builtin_convertvector(v - __builtin_convertvector(hi, f4), h4);
 }
 template <bool SPLIT>
-__device__ __forceinline__ void store1(char *row, int k, float v) {
-    char *p = row + (SPLIT ? (k >> 5) * 128 + (k & 31) * 2 : k * 2);
-    const _Float16 hi = _Float16(v);
-    *reinterpret_cast<_Float16 *>(p) = hi;
-    if (SPLIT) *reinterpret_cast<_Float16 *>(p + 64) = _Float16(v - float(hi));
-}
-template <bool SPLIT>
 __device__ __forceinline__ f4 load4(const char *row, int k) {
     const char *p = row + (SPLIT ? (k >> 5) * 128 + (k & 31) * 2 : k * 2);
     f4 v = __builtin_convertvector(*reinterpret_cast<const h4 *>(p), f4);
@@ -131,42 +216,90 @@ __device__ __forceinline__ f4 load4(const char *row, int k) {
     return v;
 }
 
-// ---- X = U / (|U|_F + eps) in both orientations, zero outside ---------------------------------------------------------------
+template <int CTRL>
+__device__ __forceinline__ float from_quad(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+// the 4 x 4 numbers of four neighbouring lanes, transposed: lane q's v[r] becomes lane r's v[q]
+__device__ __forceinline__ f4 transpose4(f4 v, int lane) {
+    const bool odd = lane & 1, high = lane & 2;
+    const float a = from_quad<0xB1>(odd ? v[0] : v[1]), b = from_quad<0xB1>(odd ? v[2] : v[3]);
+    if (odd) v[0] = a, v[2] = b;
+    else v[1] = a, v[3] = b;
+    const float c = from_quad<0x4E>(high ? v[0] : v[2]), d = from_quad<0x4E>(high ? v[1] : v[3]);
+    if (high) v[0] = c, v[1] = d;
+    else v[2] = c, v[3] = d;
+    return v;
+}
+
+// ---- X = U / (|U|_F + eps) in both orientations, zero in the padding: one 64 x 64 tile of G to a workgroup --------------------
+// sixteen of a tile's numbers as a thread reads them: of one row where rows are aligned, else of one column's 64 lanes
+__device__ __forceinline__ void load_tile(const void *p, int dtype, int64_t ld, const Job &j, int r0, int c0, int tid, float (&v)[16]) {
+    if (j.vec_in) {
+        const int r = r0 + (tid >> 2), c = c0 + (tid & 3) * 16;
+        float a[8] = {}, b[8] = {};
+        if (r < j.rows) {
+            load8(row_of(p, dtype, r * ld), dtype, c, j.cols, true, a);
+            load8(row_of(p, dtype, r * ld), dtype, c + 8, j.cols, true, b);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = a[e], v[e + 8] = b[e];
+        return;
+    }
+    const int c = c0 + (tid & 63), r = r0 + (tid >> 6);
+    const int64_t at = int64_t(r) * ld + c;
+    const bool in = c < j.cols;
+    if (dtype == CP_F32) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = in && r + 4 * e < j.rows ? static_cast<const float *>(p)[at + 4 * e * ld] : 0.f;
+    } else if (dtype == CP_BF16) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = in && r + 4 * e < j.rows ? float(static_cast<const __bf16 *>(p)[at + 4 * e * ld]) : 0.f;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = in && r + 4 * e < j.rows ? float(static_cast<const _Float16 *>(p)[at + 4 * e * ld]) : 0.f;
+    }
+}
+
 template <bool SPLIT>
-__global__ void __launch_bounds__(256) k_ortho_load(Jobs js, float momentum, int nesterov, double eps, float x_scale) {
-    const Job &j = js.job[find_job(js, blockIdx.x, &Job::first_load)];
+__global__ void __launch_bounds__(256) k_ortho_load(Table tab, float momentum, int nesterov, double eps, float x_scale) {
+    const int which = find_job(tab.first[LOAD], tab.n, blockIdx.x);
+    const Job j = tab.job[which];
     const bool tall = j.rows > j.cols;
-    const int pr = tall ? j.np : j.mp, pc = tall ? j.mp : j.np;   // padded rows / columns of G as it lies
-    const int id = blockIdx.x - j.first_load, tiles_c = pc / 64;
+    const int id = blockIdx.x - tab.first[LOAD][which], tiles_c = (tall ? j.mp : j.np) / 64;
     const int r0 = id / tiles_c * 64, c0 = id % tiles_c * 64;
-    (void)pr;
     __shared__ double s[4];
     __shared__ float t[64][65];
-    const int tid = threadIdx.x;
-    const double part = wave_sum(j.part[tid]);
+    const int tid = threadIdx.x, line = tid >> 2, k = (tid & 3) * 16;
+    float v[16];
+    if (j.M) {
+        load_tile(j.M, CP_F32, j.ldm, j, r0, c0, tid, v);
+        if (nesterov) {
+            float u[16];
+            load_tile(j.G, j.g_dtype, j.ldg, j, r0, c0, tid, u);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = fmaf(momentum, v[e], u[e]);
+        }
+    } else {
+        load_tile(j.G, j.g_dtype, j.ldg, j, r0, c0, tid, v);
+    }
+    const int n_part = (j.sum_rows + j.rows_per - 1) / j.rows_per * j.chunks;
+    double part = 0.0;
+    for (int i = tid; i < n_part; i += 256) part += j.part[i];
+    part = wave_sum(part);
     if ((tid & 63) == 0) s[tid >> 6] = part;
     __syncthreads();
     const double norm = sqrt((s[0] + s[1]) + (s[2] + s[3])) + eps;
     const double inv = norm > 0.0 || norm != norm ? double(x_scale) / norm : 0.0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const int r = i * 4 + (tid >> 6), c = tid & 63;
-        float v = 0.f;
-        if (r0 + r < j.rows && c0 + c < j.cols) {
-            float u = load_as_float(j.G, j.g_dtype, int64_t(r0 + r) * j.ldg + c0 + c);
-            if (j.M) {
-                const float m = j.M[int64_t(r0 + r) * j.ldm + c0 + c];
-                u = nesterov ? fmaf(momentum, m, u) : m;
-            }
-            v = float(double(u) * inv);
-        }
-        t[r][c] = v;
+    for (int e = 0; e < 16; ++e) {
+        const float x = float(double(v[e]) * inv);
+        if (j.vec_in) t[line][k + e] = x;
+        else t[(tid >> 6) + 4 * e][tid & 63] = x;
     }
     __syncthreads();
     char *n = tall ? j.xt0 : j.x, *o = tall ? j.x : j.xt0;
     const uint32_t ldn = tall ? j.lds : j.ldn, ldo = tall ? j.ldn : j.lds;
-    const int line = tid >> 2, k = (tid & 3) * 16;
-    float v[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) v[e] = t[line][k + e];
     store16<SPLIT>(n + int64_t(r0 + line) * ldn, c0 + k, v);
@@ -176,7 +309,7 @@ __global__ void __launch_bounds__(256) k_ortho_load(Jobs js, float momentum, int
 }
 
 // ---- the products ------------------------------------------------------------------------------------------------------------
-enum { GRAM, POLY, APPLY, LAST };
+constexpr int LAST = PHASES;   // the step's third product where it is the call's last: writes O or W
 
 struct Factors {
     float acc, a, diag;   // what the accumulator, A's entry and the diagonal count for in the result
@@ -184,58 +317,88 @@ struct Factors {
     int xt;               // which X^T is read
 };
 
-template <int PHASE, bool SPLIT>
-__global__ void __launch_bounds__(256) k_ortho_product(Jobs js, Factors f) {
-    constexpr int BM = kTile, BN = kTile, T = 256, WI = 4, WJ = 4;
+// A wave's part of O or W where rows are not aligned: sixteen rows at a time go through LDS (its own), so that lanes hold
+// neighbours of a row.  W is read where it is there, without a branch, and all of a group before the first is written.
+template <typename T, int WI, int WJ>
+__device__ __forceinline__ void write_rows(const Job &j, const Factors &f, const f4 (&acc)[WI][WJ], float *own, int i0, int j0, int lane) {
+    constexpr int W = WJ * 16, LD = W + 4, AT_ONCE = 64 / W, N = 16 / AT_ONCE;
+    T *out = static_cast<T *>(j.out);
+    const int c = j0 + lane % W;
+#pragma unroll
+    for (int wi = 0; wi < WI; ++wi) {
+        const int i = i0 + wi * 16 + lane / W;
+        if (i0 + wi * 16 >= j.rows) break;
+        float w[N];
+        if (j.M) {
+#pragma unroll
+            for (int r = 0; r < N; ++r) w[r] = float(out[int64_t(min(i + r * AT_ONCE, j.rows - 1)) * j.ldo + min(c, j.cols - 1)]);
+        }
+#pragma unroll
+        for (int wj = 0; wj < WJ; ++wj) *reinterpret_cast<f4 *>(own + (lane & 15) * LD + wj * 16 + (lane >> 4) * 4) = acc[wi][wj] * f.acc;
+#pragma unroll
+        for (int r = 0; r < N; ++r) {
+            float o = own[(r * AT_ONCE + lane / W) * LD + lane % W];
+            if (j.M) o = f.keep * w[r] - j.lr * o;
+            if (i + r * AT_ONCE < j.rows && c < j.cols) out[int64_t(i + r * AT_ONCE) * j.ldo + c] = T(o);
+        }
+    }
+}
+
+template <int PHASE, bool SPLIT, class CFG>
+__global__ void __launch_bounds__(CFG::T) k_ortho_product(Table tab, Factors f, float *parts, int *counts) {
+    constexpr int BM = CFG::BM, BN = CFG::BN, T = CFG::T, WI = CFG::WI, WJ = CFG::WJ;
     constexpr bool SYM = PHASE == GRAM || PHASE == POLY;
-    __shared__ alignas(1024) char a0[BM * 128], a1[BM * 128], b0[BN * 128], b1[BN * 128];
+    constexpr int LIST = PHASE == LAST ? APPLY : PHASE;
+    NT_STAGES(st, CFG::STAGES, CFG::STAGE);
+    __shared__ int flag;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wm = wave >> 1, wn = wave & 1;
-    const int id = nt::xcd_order(blockIdx.x, SYM ? js.total_sym : js.total_apply);
-    const Job &j = js.job[find_job(js, id, SYM ? &Job::first_sym : &Job::first_apply)];
+    const int wm = wave / CFG::NWN, wn = wave % CFG::NWN;
+    const int ra = wm * WI * 16, rb = wn * WJ * 16;
+    const int at = nt::xcd_order(blockIdx.x, gridDim.x), which = find_job(tab.first[LIST], tab.n, at);
+    const Job j = tab.job[which];
+    const int first = tab.first[LIST][which], pieces = tab.pieces[LIST][which];
     const bool tall = j.rows > j.cols;
     const bool swap = PHASE == LAST && tall;   // the result's rows are G's rows: four consecutive numbers lie in one of them
     const char *xt = f.xt ? j.xt1 : j.xt0;
     const char *pa = PHASE == GRAM ? j.x : PHASE == POLY ? j.a : swap ? xt : j.b;
     const char *pb = PHASE == GRAM ? j.x : PHASE == POLY ? j.a : swap ? j.b : xt;
     const uint32_t ld = PHASE == GRAM ? j.ldn : j.lds;
-    const int steps = int(ld >> 7);
+    const int rows_a = swap ? j.np : j.mp, rows_b = SYM || swap ? j.mp : j.np;
+    const int tiles_m = (rows_a + BM - 1) / BM, tiles_n = (rows_b + BN - 1) / BN;
+    const int tiles = SYM ? tiles_m * (tiles_m + 1) / 2 : tiles_m * tiles_n;
+    const int piece = (at - first) / tiles, tile = (at - first) % tiles;
+    const int steps = int(ld >> 7), k0 = steps * piece / pieces, k1 = steps * (piece + 1) / pieces;
     int tm, tn;
-    if (SYM) {
-        const int t = id - j.first_sym;
-        tm = int((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
-        while (tm * (tm + 1) / 2 > t) --tm;
-        while ((tm + 1) * (tm + 2) / 2 <= t) ++tm;
-        tn = t - tm * (tm + 1) / 2;
-    } else {
-        const int t = id - j.first_apply, tiles_m = (swap ? j.np : j.mp) / BM;
-        tm = t % tiles_m;
-        tn = t / tiles_m;
-    }
+    if (SYM) nt::lower_tile_at(tile, tiles_m, tm, tn);
+    else nt::tile_at(tile, tiles_m, tiles_n, tm, tn);
     const int i0 = tm * BM, j0 = tn * BN;
     nt::Loader<BM, T> la;
     nt::Loader<BN, T> lb;
-    la.init(pa + int64_t(i0) * ld, ld, BM, tid);
-    lb.init(pb + int64_t(j0) * ld, ld, BN, tid);
+    la.init(pa + int64_t(i0) * ld + k0 * 128, ld, rows_a - i0, tid);
+    lb.init(pb + int64_t(j0) * ld + k0 * 128, ld, rows_b - j0, tid);
     f4 acc[WI][WJ];
 #pragma unroll
     for (int i = 0; i < WI; ++i)
 #pragma unroll
         for (int k = 0; k < WJ; ++k) acc[i][k] = f4{0.f, 0.f, 0.f, 0.f};
-    const int ra = wm * WI * 16, rb = wn * WJ * 16;
-    auto fetch = [&](int k, char *a, char *b) {
-        la.issue(k, a, wave);
-        lb.issue(k, b, wave);
-    };
-    fetch(0, a0, b0);
-    for (int k = 0; k < steps; k += 2) {
-        nt::stage_barrier();
-        if (k + 1 < steps) fetch(k + 1, a1, b1);
-        nt::products16<WI, WJ>(a0 + ra * 128, b0 + rb * 128, lane, acc, SPLIT);
-        if (k + 1 >= steps) break;
-        nt::stage_barrier();
-        if (k + 2 < steps) fetch(k + 2, a0, b0);
-        nt::products16<WI, WJ>(a1 + ra * 128, b1 + rb * 128, lane, acc, SPLIT);
+    nt::pipeline<CFG::STAGES, CFG::LOADS, CFG::PARTS>(
+        st, k1 - k0,
+        [&](int k, char *s, int part, int parts) {
+            la.issue(k, s, wave, part, parts);
+            lb.issue(k, s + BM * 128, wave, part, parts);
+        },
+        [&](const char *s, auto between) {
+            nt::products16<WI, WJ, SPLIT>(s + ra * 128, s + (BM + rb) * 128, lane, acc, between);
+        });
+    if (pieces > 1 && !nt::join<T>(acc, piece, pieces, parts + int64_t(first + tile) * (BM * BN), tiles, counts + first + tile, &flag, tid))
+        return;
+    if (PHASE == LAST && !j.vec_out) {
+        float *own = reinterpret_cast<float *>(st[0]) + wave * 16 * (WJ * 16 + 4);
+        static_assert(CFG::NWM * CFG::NWN * 16 * (WJ * 16 + 4) * 4 <= CFG::STAGE, "LDS");
+        if (j.o_dtype == CP_F32) write_rows<float>(j, f, acc, own, i0 + ra, j0 + rb, lane);
+        else if (j.o_dtype == CP_BF16) write_rows<__bf16>(j, f, acc, own, i0 + ra, j0 + rb, lane);
+        else write_rows<_Float16>(j, f, acc, own, i0 + ra, j0 + rb, lane);
+        return;
     }
 #pragma unroll
     for (int wi = 0; wi < WI; ++wi) {
@@ -243,6 +406,8 @@ __global__ void __launch_bounds__(256) k_ortho_product(Jobs js, Factors f) {
 #pragma unroll
         for (int wj = 0; wj < WJ; ++wj) {
             const int c = j0 + rb + wj * 16 + (lane >> 4) * 4;
+            // the tile's rows and columns beyond the padding are not there (both are multiples of 64: a group of 16 is all in or out)
+            if (i0 + ra + wi * 16 >= rows_a || j0 + rb + wj * 16 >= rows_b) continue;
             f4 v = acc[wi][wj] * f.acc;
             if (PHASE == POLY) {
                 v += load4<SPLIT>(j.a + int64_t(i) * j.lds, c) * f.a;
@@ -250,26 +415,24 @@ __global__ void __launch_bounds__(256) k_ortho_product(Jobs js, Factors f) {
                 for (int r = 0; r < 4; ++r)
                     if (c + r == i) v[r] += f.diag;
             }
-            if (SYM) {
-                char *out = PHASE == GRAM ? j.a : j.b;
-                store4<SPLIT>(out + int64_t(i) * j.lds, c, v);
-                if (tm != tn) {
+            if (PHASE != LAST) {
+                char *out = PHASE == GRAM ? j.a : PHASE == POLY ? j.b : j.x;
+                char *out_t = PHASE == GRAM ? j.a : PHASE == POLY ? j.b : f.xt ? j.xt0 : j.xt1;
+                store4<SPLIT>(out + int64_t(i) * (SYM ? j.lds : j.ldn), c, v);
+                if (!SYM || tm != tn) store4<SPLIT>(out_t + int64_t(c + (lane & 3)) * j.lds, i & ~3, transpose4(v, lane));
+            } else if (i < j.rows && c < j.cols) {
+                const int64_t o = i * j.ldo + c;
+                if (c + 4 <= j.cols) {
+                    if (j.M) v = load4_as_float(j.out, j.o_dtype, o) * f.keep - v * j.lr;
+                    store4_as(j.out, j.o_dtype, o, v);
+                } else {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) store1<SPLIT>(out + int64_t(c + r) * j.lds, i, v[r]);
-                }
-            } else if (PHASE == APPLY) {
-                store4<SPLIT>(j.x + int64_t(i) * j.ldn, c, v);
-                char *out = f.xt ? j.xt0 : j.xt1;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) store1<SPLIT>(out + int64_t(c + r) * j.lds, i, v[r]);
-            } else if (i < j.rows) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    if (c + r >= j.cols) break;
-                    const int64_t at = i * j.ldo + c + r;
-                    float o = v[r];
-                    if (j.M) o = f.keep * load_as_float(j.out, j.o_dtype, at) - j.lr * o;
-                    store_as(j.out, j.o_dtype, at, o);
+                    for (int r = 0; r < 3; ++r) {
+                        if (c + r >= j.cols) break;
+                        float y = v[r];
+                        if (j.M) y = f.keep * load_as_float(j.out, j.o_dtype, o + r) - j.lr * y;
+                        store_as(j.out, j.o_dtype, o + r, y);
+                    }
                 }
             }
         }
@@ -377,7 +540,7 @@ int check_requests(cp_ctx *ctx, const std::vector<Request> &rq, bool step) {
         if (!r.G || !r.out || (step && !r.M)) return cp_set_error(ctx, CP_ERR_ARG, "job %d: null pointer", int(k));
         if (uintptr_t(r.G) % type_size(r.g_dtype) || uintptr_t(r.out) % type_size(r.o_dtype) || uintptr_t(r.M) % 4)
             return cp_set_error(ctx, CP_ERR_ARG, "job %d: alignment", int(k));
-        if (int64_t(std::min(r.rows, r.cols) + 127) / 128 > 512)
+        if (std::min(r.rows, r.cols) > 65536)
             return cp_set_error(ctx, CP_ERR_UNSUPPORTED, "job %d: shorter side above 65536", int(k));
         w.push_back({uintptr_t(r.out), r.ldo, r.rows, r.cols, type_size(r.o_dtype)});
         const Written g = {uintptr_t(r.G), r.ldg, r.rows, r.cols, type_size(r.g_dtype)};
@@ -396,7 +559,7 @@ int check_requests(cp_ctx *ctx, const std::vector<Request> &rq, bool step) {
 
 bool is_split(const Request &r) { return r.o_dtype != CP_BF16; }
 
-int64_t padded(int v) { return (int64_t(v) + kTile - 1) / kTile * kTile; }
+int64_t padded(int64_t v) { return (v + kPad - 1) / kPad * kPad; }
 
 size_t job_bytes(const Request &r) {
     if (!r.rows || !r.cols) return 0;
@@ -405,78 +568,115 @@ size_t job_bytes(const Request &r) {
     return cp_align_up(kPartials * sizeof(double) + e * (3 * mp * np + 2 * mp * mp), 256);
 }
 
-size_t call_bytes(const std::vector<Request> &rq) {
-    size_t b = 0;
-    for (const Request &r : rq) b += job_bytes(r);
-    return b;
+// One launch of a product over a class's jobs: its shape of tile, and the pieces that each job's tiles are cut into
+struct Choice {
+    int cfg;           // 0 Large, 1 Medium, 2 Small
+    int grid;
+    bool joins;
+};
+
+// The jobs of one class (one fp16 a number, or pairs)
+struct Class {
+    bool split;
+    std::vector<Job> jobs;
+    std::vector<Place> places;
+    std::vector<int> sum_groups;   // workgroups of k_ortho_norm
+    Table table;
+    int loads = 0;
+    Choice gram, poly, apply;
+};
+
+constexpr int kEdge[3] = {256, 128, 64};
+
+int64_t tiles_of(const Job &j, int phase, int edge) {
+    const int64_t m = (j.mp + edge - 1) / edge, n = (j.np + edge - 1) / edge;
+    return phase == APPLY ? m * n : m * (m + 1) / 2;
+}
+int64_t steps_of(const Job &j, int phase) { return (phase == GRAM ? j.ldn : j.lds) / 128; }
+
+// What a launch costs in us, from its number of workgroups, their K steps in all and the longest's.
+// Measured: us per step and workgroup where a CU holds as many as fit (Large one, the others two), and where there is at most
+// one to a CU; what a workgroup costs beside its steps (first loads, stores: twice as many where numbers are pairs); a join.
+double cost_of(int cfg, bool split, int64_t groups, int64_t total, int64_t longest, bool joins) {
+    static const double full[2][3] = {{1.55, 1.04, 0.33}, {2.25, 1.35, 0.37}}, alone[2][3] = {{1.35, 0.60, 0.20}, {2.0, 0.75, 0.28}};
+    static const double extra[2][3] = {{14.0, 6.0, 3.5}, {28.0, 11.0, 5.0}}, joined[3] = {14.0, 5.0, 3.0};
+    const int slots = cfg == 0 ? kCus : 2 * kCus;
+    const double step = groups > kCus ? full[split][cfg] : alone[split][cfg], more = extra[split][cfg] + (joins ? joined[cfg] : 0.0);
+    const double mean = double(total) / groups * step + more, most = longest * step + more, rounds = double(groups) / slots;
+    // equal workgroups end together; others fill each other's gaps
+    return std::max(most, mean * (total == longest * groups ? std::ceil(rounds) : rounds + 0.3));
 }
 
-// the scratch of a call: the caller's, or the context's own (which a captured call must not use: the graph outlives it)
-int scratch(cp_ctx *ctx, void *ws, size_t ws_bytes, size_t need, char **out) {
-    if (ws) {
-        if (uintptr_t(ws) % 256) return cp_set_error(ctx, CP_ERR_ARG, "workspace is not 256-byte aligned");
-        if (ws_bytes < need) return cp_set_error(ctx, CP_ERR_ARG, "workspace of %zu bytes, %zu needed", ws_bytes, need);
-        *out = static_cast<char *>(ws);
-        return CP_OK;
-    }
-    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    CP_HIP(ctx, hipStreamIsCapturing(ctx->stream, &st));
-    if (st != hipStreamCaptureStatusNone)
-        return cp_set_error(ctx, CP_ERR_ARG, "a captured call needs a workspace of its own (%zu bytes)", need);
-    CP_TRY(cp_arena_reserve(ctx, need));
-    *out = static_cast<char *>(cp_arena_take(ctx, need));
-    return *out ? CP_OK : cp_set_error(ctx, CP_ERR_NOMEM, "arena");
-}
+constexpr int kLeast = 32;   // K steps of a piece, at least
 
-template <bool SPLIT>
-void launch_all(cp_ctx *ctx, const std::vector<Jobs> &launches, const Plan &pl, float momentum, int nesterov, double eps,
-                float keep) {
-    hipStream_t st = ctx->stream;
-    for (int k = 0; k < pl.steps; ++k) {
-        const double a = pl.coef[k][0], b = pl.coef[k][1], c = pl.coef[k][2];
-        const double sx = pl.sx[k], sa = pl.sa[k], sb = pl.sb[k];
-        Factors f = {};
-        f.xt = k & 1;
-        for (const Jobs &js : launches) {
-            f.acc = float(sa / (sx * sx));
-            k_ortho_product<GRAM, SPLIT><<<js.total_sym, 256, 0, st>>>(js, f);
-        }
-        for (const Jobs &js : launches) {
-            f.acc = float(c * sb / (sa * sa));
-            f.a = float(b * sb / sa);
-            f.diag = float(a * sb);
-            k_ortho_product<POLY, SPLIT><<<js.total_sym, 256, 0, st>>>(js, f);
-        }
-        for (const Jobs &js : launches) {
-            if (k + 1 < pl.steps) {
-                f.acc = float(pl.sx[k + 1] / (sb * sx));
-                k_ortho_product<APPLY, SPLIT><<<js.total_apply, 256, 0, st>>>(js, f);
-            } else {
-                f.acc = float(1.0 / (sb * sx));
-                f.keep = keep;
-                k_ortho_product<LAST, SPLIT><<<js.total_apply, 256, 0, st>>>(js, f);
+// into how many pieces of k a job's tiles are cut: as if it were alone, so that its sums do not depend on the call's other jobs
+int pieces_of(const Job &j, int phase, bool split) {
+    const int64_t steps = steps_of(j, phase);
+    double least = 1e30;
+    int best = 1;
+    for (int cfg = 0; cfg < 3; ++cfg) {
+        const int64_t tiles = tiles_of(j, phase, kEdge[cfg]);
+        for (int p = 1; p <= 16 && (p == 1 || steps / p >= kLeast); ++p) {
+            const double c = cost_of(cfg, split, tiles * p, tiles * steps, (steps + p - 1) / p, p > 1);
+            if (c < 0.97 * least) {
+                least = c;
+                best = p;
             }
         }
     }
+    return best;
 }
 
-int run(cp_ctx *ctx, const std::vector<Request> &rq, const Plan &pl, double lr, double momentum, int nesterov, double decay,
-        double eps, void *ws, size_t ws_bytes) {
-    const size_t need = call_bytes(rq);
-    if (!need) return CP_OK;
-    CP_HIP(ctx, hipSetDevice(ctx->device));
-    char *at = nullptr;
-    CP_TRY(scratch(ctx, ws, ws_bytes, need, &at));
-    std::vector<Jobs> launches[2];
+bool choose(Class &cl, int phase, Choice &best) {
+    double least = 1e300;
+    const int forced = cp_knob(CP_KNOB_NT_TILE);
+    for (int cfg = 0; cfg < 3; ++cfg) {
+        if (forced && forced - 1 != cfg) continue;
+        int64_t groups = 0, total = 0, longest = 0;
+        Choice c = {cfg, 0, false};
+        for (size_t k = 0; k < cl.jobs.size(); ++k) {
+            const int64_t tiles = tiles_of(cl.jobs[k], phase, kEdge[cfg]), steps = steps_of(cl.jobs[k], phase);
+            const int p = cl.places[k].pieces[phase];
+            c.joins |= p > 1;
+            groups += tiles * p;
+            total += tiles * steps;
+            longest = std::max(longest, (steps + p - 1) / p);
+        }
+        if (groups >= (int64_t(1) << 31)) continue;
+        c.grid = int(groups);
+        const double cost = cost_of(cfg, cl.split, groups, total, longest, c.joins);
+        if (cost < least) {
+            least = cost;
+            best = c;
+        }
+    }
+    if (least == 1e300) return false;
+    int at = 0;
+    for (size_t k = 0; k < cl.jobs.size(); ++k) {
+        cl.places[k].first[phase] = at;
+        at += int(tiles_of(cl.jobs[k], phase, kEdge[best.cfg])) * cl.places[k].pieces[phase];
+    }
+    return true;
+}
+
+// The layout of a call in its workspace: | arrival counters | pieces of tiles | tables | the jobs' matrices |
+struct Layout {
+    size_t counts = 0, parts = 0, tables = 0, jobs = 0;   // bytes
+    Class cls[2];
+    size_t all() const { return jobs ? counts + parts + tables + jobs : 0; }
+};
+
+size_t table_bytes(size_t n) { return cp_align_up(n * (sizeof(Job) + 2 * PHASES * sizeof(int)), 256); }
+
+int lay_out(cp_ctx *ctx, const std::vector<Request> &rq, double lr, Layout &lay) {
+    lay.cls[0].split = false;
+    lay.cls[1].split = true;
     for (const Request &r : rq) {
         if (!r.rows || !r.cols) continue;
-        std::vector<Jobs> &ls = launches[is_split(r)];
-        if (ls.empty() || ls.back().n == kJobs) ls.push_back(Jobs());
-        Jobs &js = ls.back();
-        Job &j = js.job[js.n++];
-        j = {};
-        const size_t e = is_split(r) ? 4 : 2;
+        Class &cl = lay.cls[is_split(r)];
+        const size_t e = cl.split ? 4 : 2;
         const size_t mp = padded(std::min(r.rows, r.cols)), np = padded(std::max(r.rows, r.cols));
+        Job j = {};
         j.G = r.G;
         j.M = r.M;
         j.out = r.out;
@@ -489,34 +689,145 @@ int run(cp_ctx *ctx, const std::vector<Request> &rq, const Plan &pl, double lr, 
         j.np = int(np);
         j.ldn = uint32_t(np * e);
         j.lds = uint32_t(mp * e);
-        j.g_dtype = r.g_dtype;
-        j.o_dtype = r.o_dtype;
+        j.g_dtype = int16_t(r.g_dtype);
+        j.o_dtype = int16_t(r.o_dtype);
+        const bool aligned = uintptr_t(r.G) % 16 == 0 && uintptr_t(r.M) % 16 == 0;
+        j.vec_in = aligned && r.ldg * type_size(r.g_dtype) % 16 == 0 && r.ldm % 4 == 0;
+        j.vec_out = uintptr_t(r.out) % (4 * type_size(r.o_dtype)) == 0 && r.ldo % 4 == 0;
         j.lr = float(lr * r.gamma);
-        j.part = reinterpret_cast<double *>(at);
-        j.x = at + kPartials * sizeof(double);
-        j.xt0 = j.x + mp * np * e;
-        j.xt1 = j.xt0 + mp * np * e;
-        j.a = j.xt1 + mp * np * e;
-        j.b = j.a + mp * mp * e;
-        at += job_bytes(r);
-        const int tm = int(mp / kTile), tn = int(np / kTile);
-        j.first_sym = js.total_sym;
-        js.total_sym += tm * (tm + 1) / 2;
-        j.first_apply = js.total_apply;
-        js.total_apply += tm * tn;
-        j.first_load = js.total_load;
-        js.total_load += int((mp / 64) * (np / 64));
+        const bool flat = r.ldg == r.cols && (!r.M || r.ldm == r.cols);
+        j.sum_rows = flat ? 1 : r.rows;
+        j.sum_cols = flat ? int64_t(r.rows) * r.cols : r.cols;
+        j.vec_sum = flat ? aligned : j.vec_in;
+        j.width = flat ? int(std::max<int64_t>(4096, (j.sum_cols / kPartials + 2048) / 2048 * 2048)) : 4096;
+        j.chunks = int((j.sum_cols + j.width - 1) / j.width);
+        j.rows_per = int(std::max<int64_t>(1, 4096 / std::min<int64_t>(j.sum_cols, 4096)));
+        while (int64_t((j.sum_rows + j.rows_per - 1) / j.rows_per) * j.chunks > kPartials) j.rows_per *= 2;
+        j.part = reinterpret_cast<double *>(lay.jobs);   // an offset so far
+        lay.jobs += job_bytes(r);
+        Place p = {};
+        p.first[LOAD] = cl.loads;
+        cl.loads += int((mp / 64) * (np / 64));
+        for (int phase = GRAM; phase < PHASES; ++phase) p.pieces[phase] = int16_t(pieces_of(j, phase, cl.split));
+        cl.sum_groups.push_back((j.sum_rows + j.rows_per - 1) / j.rows_per * j.chunks);
+        cl.jobs.push_back(j);
+        cl.places.push_back(p);
     }
-    for (int s = 0; s < 2; ++s)
-        for (const Jobs &js : launches[s])
-            k_ortho_norm<<<dim3(kPartials, js.n), 256, 0, ctx->stream>>>(js, float(momentum), nesterov);
-    for (const Jobs &js : launches[0])
-        k_ortho_load<false><<<js.total_load, 256, 0, ctx->stream>>>(js, float(momentum), nesterov, eps, float(pl.sx[0]));
-    for (const Jobs &js : launches[1])
-        k_ortho_load<true><<<js.total_load, 256, 0, ctx->stream>>>(js, float(momentum), nesterov, eps, float(pl.sx[0]));
-    const float keep = float(1.0 - lr * decay);
-    launch_all<false>(ctx, launches[0], pl, float(momentum), nesterov, eps, keep);
-    launch_all<true>(ctx, launches[1], pl, float(momentum), nesterov, eps, keep);
+    for (Class &cl : lay.cls) {
+        if (cl.jobs.empty()) continue;
+        if (!choose(cl, GRAM, cl.gram) || !choose(cl, POLY, cl.poly) || !choose(cl, APPLY, cl.apply))
+            return cp_set_error(ctx, CP_ERR_UNSUPPORTED, "a product of more than 2^31 tiles");
+        for (const Choice *c : {&cl.gram, &cl.poly, &cl.apply})
+            if (c->joins) {
+                lay.counts = std::max(lay.counts, cp_align_up(size_t(c->grid) * sizeof(int), 256));
+                lay.parts = std::max(lay.parts, size_t(c->grid) * kEdge[c->cfg] * kEdge[c->cfg] * sizeof(float));
+            }
+        lay.tables += table_bytes(cl.jobs.size());
+    }
+    return CP_OK;
+}
+
+// the offsets become pointers into the workspace
+void place(Layout &lay, char *ws) {
+    char *tables = ws + lay.counts + lay.parts, *jobs = tables + lay.tables;
+    for (Class &cl : lay.cls) {
+        const size_t n = cl.jobs.size();
+        if (!n) continue;
+        cl.table.n = int(n);
+        cl.table.job = reinterpret_cast<Job *>(tables);
+        int *p = reinterpret_cast<int *>(tables + n * sizeof(Job));
+        for (int k = 0; k < PHASES; ++k) {
+            cl.table.first[k] = p + 2 * k * n;
+            cl.table.pieces[k] = p + (2 * k + 1) * n;
+        }
+        tables += table_bytes(n);
+        for (Job &j : cl.jobs) {
+            const size_t mn = size_t(j.mp) * j.ldn, mm = size_t(j.mp) * j.lds;
+            char *q = jobs + reinterpret_cast<size_t>(j.part);
+            j.part = reinterpret_cast<double *>(q);
+            j.x = q + kPartials * sizeof(double);
+            j.xt0 = j.x + mn;
+            j.xt1 = j.xt0 + mn;
+            j.a = j.xt1 + mn;
+            j.b = j.a + mm;
+        }
+    }
+}
+
+struct Call {
+    hipStream_t st;
+    const Layout &lay;
+    char *ws;
+    int *counts() const { return reinterpret_cast<int *>(ws); }
+    float *parts() const { return reinterpret_cast<float *>(ws + lay.counts); }
+};
+
+template <int PHASE, bool SPLIT>
+void launch_product(const Call &call, const Table &t, const Choice &c, const Factors &f) {
+    if (c.cfg == 0) k_ortho_product<PHASE, SPLIT, nt::Large><<<c.grid, nt::Large::T, 0, call.st>>>(t, f, call.parts(), call.counts());
+    else if (c.cfg == 1) k_ortho_product<PHASE, SPLIT, nt::Medium><<<c.grid, nt::Medium::T, 0, call.st>>>(t, f, call.parts(), call.counts());
+    else k_ortho_product<PHASE, SPLIT, nt::Small><<<c.grid, nt::Small::T, 0, call.st>>>(t, f, call.parts(), call.counts());
+}
+
+template <bool SPLIT>
+void launch_steps(const Call &call, const Class &cl, const Plan &pl, float keep) {
+    for (int k = 0; k < pl.steps; ++k) {
+        const double a = pl.coef[k][0], b = pl.coef[k][1], c = pl.coef[k][2];
+        const double sx = pl.sx[k], sa = pl.sa[k], sb = pl.sb[k];
+        Factors f = {};
+        f.xt = k & 1;
+        f.acc = float(sa / (sx * sx));
+        launch_product<GRAM, SPLIT>(call, cl.table, cl.gram, f);
+        f.acc = float(c * sb / (sa * sa));
+        f.a = float(b * sb / sa);
+        f.diag = float(a * sb);
+        launch_product<POLY, SPLIT>(call, cl.table, cl.poly, f);
+        if (k + 1 < pl.steps) {
+            f.acc = float(pl.sx[k + 1] / (sb * sx));
+            launch_product<APPLY, SPLIT>(call, cl.table, cl.apply, f);
+        } else {
+            f.acc = float(1.0 / (sb * sx));
+            f.keep = keep;
+            launch_product<LAST, SPLIT>(call, cl.table, cl.apply, f);
+        }
+    }
+}
+
+int run(cp_ctx *ctx, const std::vector<Request> &rq, const Plan &pl, double lr, double momentum, int nesterov, double decay,
+        double eps, void *given, size_t given_bytes) {
+    Layout lay;
+    CP_TRY(lay_out(ctx, rq, lr, lay));
+    if (!lay.all()) return CP_OK;
+    CP_HIP(ctx, hipSetDevice(ctx->device));
+    char *ws = nullptr;
+    CP_TRY(cp_scratch(ctx, given, given_bytes, lay.all(), &ws));
+    place(lay, ws);
+    const Call call = {ctx->stream, lay, ws};
+    const float mu = float(momentum), keep = float(1.0 - lr * decay), sx = float(pl.sx[0]);
+    // every job's G is read before any output is written: an output may be another job's G
+    for (const Class &cl : lay.cls)
+        for (size_t base = 0; base < cl.jobs.size(); base += kJobs) {
+            Jobs js = {};
+            js.base = int(base);
+            int groups = 0;
+            for (; js.n < kJobs && base + js.n < cl.jobs.size(); ++js.n) {
+                js.first[js.n] = groups;
+                js.job[js.n] = cl.jobs[base + js.n];
+                js.place[js.n] = cl.places[base + js.n];
+                groups += cl.sum_groups[base + js.n];
+            }
+            k_ortho_norm<<<groups, 256, 0, call.st>>>(js, cl.table, mu, nesterov, call.counts(), int(lay.counts / sizeof(int)));
+        }
+    for (const Class &cl : lay.cls) {
+        if (cl.jobs.empty()) continue;
+        if (cl.split) k_ortho_load<true><<<cl.loads, 256, 0, call.st>>>(cl.table, mu, nesterov, eps, sx);
+        else k_ortho_load<false><<<cl.loads, 256, 0, call.st>>>(cl.table, mu, nesterov, eps, sx);
+    }
+    for (const Class &cl : lay.cls) {
+        if (cl.jobs.empty()) continue;
+        if (cl.split) launch_steps<true>(call, cl, pl, keep);
+        else launch_steps<false>(call, cl, pl, keep);
+    }
     CP_LAUNCH_CHECK(ctx);
     return CP_OK;
 }
@@ -547,7 +858,9 @@ int workspace(int n, const J *jobs, int steps, const double *coef, double eps, s
         std::vector<Request> rq;
         CP_TRY(make_plan(nullptr, steps, coef, eps, pl));
         CP_TRY(take_jobs(nullptr, n, jobs, rq));
-        *bytes = call_bytes(rq);
+        Layout lay;
+        CP_TRY(lay_out(nullptr, rq, 0.0, lay));
+        *bytes = lay.all();
         return CP_OK;
     } catch (...) {
         return CP_ERR_NOMEM;

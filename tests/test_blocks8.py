@@ -195,13 +195,31 @@ def check_product(ctx, m, n, k, fa="e4m3", fb="e4m3", ta=1, tb=128, out="f32", b
     return C
 
 
+@pytest.fixture(params=[0, 1, 2, 3])
+def tile_shape(request, ctx):
+    """Every shape of tile in turn (0: the library's choice)."""
+    ctx.lib.cp_debug_knob(3, request.param)
+    yield request.param
+    ctx.lib.cp_debug_knob(3, 0)
+
+
 @gpu
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 16, 128), (1, 1000, 2048), (2, 129, 300), (7, 77, 77), (16, 512, 4005), (17, 64, 640),
                                    (33, 200, 1280), (64, 128, 129), (100, 60, 513), (128, 128, 256), (129, 257, 384), (300, 300, 1000),
                                    (500, 130, 50), (700, 520, 260)])
 @pytest.mark.parametrize("tb", [1, 128])
-def test_product(ctx, m, n, k, tb):
+def test_product(ctx, tile_shape, m, n, k, tb):
     check_product(ctx, m, n, k, tb=tb, bias=m % 2 == 1)
+    check_product(ctx, m, n, k, tb=tb, out="bf16", bias=m % 2 == 0)
+
+
+@gpu
+@pytest.mark.parametrize("m,n,k", [(20, 70, 4000), (129, 65, 6000), (300, 260, 3000)])
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+def test_product_cut_along_k(ctx, tile_shape, m, n, k, out):
+    """Few tiles and a long inner length: several workgroups to a tile, one call after another on the same counters."""
+    A = check_product(ctx, m, n, k, out=out).raw()
+    assert np.array_equal(A, check_product(ctx, m, n, k, out=out).raw())
 
 
 @gpu

@@ -126,6 +126,14 @@ def test_step_jobs_are_checked():
 
 # ---- orthogonalise ---------------------------------------------------------------------------------------------------------
 
+@pytest.fixture(params=[0, 1, 2, 3])
+def tile_shape(request, ctx):
+    """Every shape of tile in turn (0: the library's choice)."""
+    ctx.lib.cp_debug_knob(3, request.param)
+    yield request.param
+    ctx.lib.cp_debug_knob(3, 0)
+
+
 SHAPES = [(1, 1), (1, 300), (300, 1), (2, 3), (27, 64), (64, 27), (63, 65), (64, 576), (128, 128), (129, 200), (200, 129), (55, 1000),
           (512, 130), (257, 700)]
 
@@ -133,7 +141,7 @@ SHAPES = [(1, 1), (1, 300), (300, 1), (2, 3), (27, 64), (64, 27), (63, 65), (64,
 @gpu
 @pytest.mark.parametrize("rows,cols", SHAPES)
 @pytest.mark.parametrize("gk,ok", [("f32", "f32"), ("bf16", "bf16"), ("f16", "f16"), ("bf16", "f32"), ("f32", "bf16")])
-def test_orthogonalise(ctx, rows, cols, gk, ok):
+def test_orthogonalise(ctx, tile_shape, rows, cols, gk, ok):
     rs = np.random.RandomState(rows * 7 + cols)
     G = Mat(ctx, gradient(rs, rows, cols, 1.0), gk, ld=cols + 3, lead=1)
     O = Mat(ctx, np.zeros((rows, cols)), ok, ld=cols + 1, lead=5)
@@ -141,6 +149,17 @@ def test_orthogonalise(ctx, rows, cols, gk, ok):
     ctx.orthogonalise(capi.OrthoJobs([(G.ptr, TYPES[gk], rows, cols, O.ptr, TYPES[ok], G.ld, O.ld)]))
     within(O.get(), *distance(U, ok), ok)
     assert O.untouched() and np.array_equal(G.raw(), G.before)
+
+
+@gpu
+@pytest.mark.parametrize("rows,cols", [(70, 6000), (5000, 130), (300, 4500)])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_long_matrices(ctx, tile_shape, rows, cols, kind):
+    """The first product's tiles cut along k, several workgroups to a tile."""
+    rs = np.random.RandomState(11)
+    G, O = Mat(ctx, gradient(rs, rows, cols), kind), Mat(ctx, np.zeros((rows, cols)), kind)
+    ctx.orthogonalise(capi.OrthoJobs([(G.ptr, TYPES[kind], rows, cols, O.ptr, TYPES[kind])]), steps=3)
+    within(O.get(), *distance(G.get(), kind, steps=3), kind)
 
 
 @gpu
