@@ -38,10 +38,26 @@ struct Held {
     int fmt, tile;
 };
 
-__device__ __forceinline__ float to_float(float v) { return v; }
-__device__ __forceinline__ float to_float(double v) { return float(v); }
-__device__ __forceinline__ float to_float(__bf16 v) { return float(v); }
-__device__ __forceinline__ float to_float(_Float16 v) { return float(v); }
+// eight neighbours, at any element's address
+__device__ __forceinline__ void load8(const float *p, float (&v)[8]) {
+    const f4 a = *reinterpret_cast<const nt::f4u *>(p), b = *reinterpret_cast<const nt::f4u *>(p + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = a[e], v[e + 4] = b[e];
+}
+__device__ __forceinline__ void load8(const double *p, float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = float(p[e]);
+}
+__device__ __forceinline__ void load8(const __bf16 *p, float (&v)[8]) {
+    const nt::b8 a = *reinterpret_cast<const nt::b8u *>(p);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = float(a[e]);
+}
+__device__ __forceinline__ void load8(const _Float16 *p, float (&v)[8]) {
+    const nt::h8 a = *reinterpret_cast<const nt::h8u *>(p);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = float(a[e]);
+}
 
 __device__ __forceinline__ float finite_abs(float v) {
     const float a = fabsf(v);
@@ -80,8 +96,8 @@ __device__ __forceinline__ uint32_t pack4(const float (&y)[4], int fmt) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) k_quant_blocks(const T *__restrict__ x, int64_t rows, int64_t cols, int64_t ldx, int vec,
-                                                      int pow2, Held o, Held t) {
+__global__ void __launch_bounds__(256) k_quant_blocks(const T *__restrict__ x, int64_t rows, int64_t cols, int64_t ldx, int pow2,
+                                                      Held o, Held t) {
     __shared__ float rmax[2][128], cmax[2][128];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int lr = (wave >> 1) * 64 + (lane >> 3) * 8, lc = (wave & 1) * 64 + (lane & 7) * 8;
@@ -92,16 +108,11 @@ __global__ void __launch_bounds__(256) k_quant_blocks(const T *__restrict__ x, i
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const T *p = x + (row + i) * ldx + col;
-        if (vec && row + i < rows && col + 8 <= cols) {
-            struct alignas(16) Eight {
-                T e[8];
-            };
-            const Eight e = *reinterpret_cast<const Eight *>(p);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = to_float(e.e[j]);
+        if (row + i < rows && col + 8 <= cols) {
+            load8(p, v[i]);
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = row + i < rows && col + j < cols ? to_float(p[j]) : 0.f;
+            for (int j = 0; j < 8; ++j) v[i][j] = row + i < rows && col + j < cols ? float(p[j]) : 0.f;
         }
     }
 #pragma unroll
@@ -190,9 +201,8 @@ Held held(const cp_blocks *m) {
 template <typename T>
 void launch_quant(cp_ctx *ctx, const void *x, int64_t rows, int64_t cols, int64_t ldx, int flags, const cp_blocks *out,
                   const cp_blocks *out_t) {
-    const int vec = uintptr_t(x) % 16 == 0 && size_t(ldx) * sizeof(T) % 16 == 0;
     const dim3 grid(uint32_t((cols + 127) / 128), uint32_t((rows + 127) / 128));
-    k_quant_blocks<T><<<grid, 256, 0, ctx->stream>>>(static_cast<const T *>(x), rows, cols, ldx, vec, flags & CP_QUANT_POW2,
+    k_quant_blocks<T><<<grid, 256, 0, ctx->stream>>>(static_cast<const T *>(x), rows, cols, ldx, flags & CP_QUANT_POW2,
                                                      held(out), held(out_t));
 }
 
@@ -205,7 +215,7 @@ struct Product {
     uint32_t lda, ldb;
     int M, N, steps, tiles_m, tiles_n, pieces;
     int a_shift, b_shift;            // row -> scale: 0 (one per row) or 7
-    int c_dtype, c_vec;
+    int c_dtype;
     float *parts;
     int *counts;
 };
@@ -213,12 +223,11 @@ struct Product {
 __device__ __forceinline__ void store4(const Product &p, int64_t i, int j, f4 v) {
     const int64_t at = i * p.ldc + j;
     if (p.c_dtype == CP_F32) {
-        *reinterpret_cast<f4 *>(static_cast<float *>(p.c) + at) = v;
+        *reinterpret_cast<nt::f4u *>(static_cast<float *>(p.c) + at) = v;
     } else if (p.c_dtype == CP_BF16) {
-        typedef __bf16 b4 __attribute__((ext_vector_type(4)));
-        *reinterpret_cast<b4 *>(static_cast<__bf16 *>(p.c) + at) = __builtin_convertvector(v, b4);
+        *reinterpret_cast<nt::b4u *>(static_cast<__bf16 *>(p.c) + at) = __builtin_convertvector(v, nt::b4);
     } else {
-        *reinterpret_cast<nt::h4 *>(static_cast<_Float16 *>(p.c) + at) = __builtin_convertvector(v, nt::h4);
+        *reinterpret_cast<nt::h4u *>(static_cast<_Float16 *>(p.c) + at) = __builtin_convertvector(v, nt::h4);
     }
 }
 __device__ __forceinline__ void store1(const Product &p, int64_t i, int j, float v) {
@@ -228,48 +237,28 @@ __device__ __forceinline__ void store1(const Product &p, int64_t i, int j, float
     else static_cast<_Float16 *>(p.c)[at] = _Float16(v);
 }
 
-// A wave's part of C [16 WI rows from i0, 16 WJ columns from j0].  Where four neighbours cannot be stored at once, sixteen rows
-// at a time go through LDS (`own`: the wave's), so that lanes hold neighbours: single stores of 16 lanes' different rows took
-// 126 us more on a 20000 x 4005 product in bfloat16.
+// A wave's part of C [16 WI rows from i0, 16 WJ columns from j0]
 template <int WI, int WJ>
-__device__ __forceinline__ void write_c(const Product &p, const f4 (&acc)[WI][WJ], float *own, int i0, int j0, int lane) {
-    if (p.c_vec) {
-        f4 bias[WJ];
+__device__ __forceinline__ void write_c(const Product &p, const f4 (&acc)[WI][WJ], int i0, int j0, int lane) {
+    f4 bias[WJ];
+#pragma unroll
+    for (int wj = 0; wj < WJ; ++wj) {
+        const int j = j0 + wj * 16 + (lane >> 4) * 4;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) bias[wj][r] = p.bias && j + r < p.N ? p.bias[j + r] : 0.f;
+    }
+#pragma unroll
+    for (int wi = 0; wi < WI; ++wi) {
+        const int i = i0 + wi * 16 + (lane & 15);
+        if (i >= p.M) continue;
 #pragma unroll
         for (int wj = 0; wj < WJ; ++wj) {
             const int j = j0 + wj * 16 + (lane >> 4) * 4;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) bias[wj][r] = p.bias && j + r < p.N ? p.bias[j + r] : 0.f;
-        }
-#pragma unroll
-        for (int wi = 0; wi < WI; ++wi) {
-            const int i = i0 + wi * 16 + (lane & 15);
-            if (i >= p.M) continue;
-#pragma unroll
-            for (int wj = 0; wj < WJ; ++wj) {
-                const int j = j0 + wj * 16 + (lane >> 4) * 4;
-                const f4 v = acc[wi][wj] + bias[wj];
-                if (j + 4 <= p.N) store4(p, i, j, v);
-                else
-                    for (int r = 0; r < 3; ++r)
-                        if (j + r < p.N) store1(p, i, j + r, v[r]);
-            }
-        }
-        return;
-    }
-    constexpr int W = WJ * 16, LD = W + 4, AT_ONCE = 64 / W, N = 16 / AT_ONCE;
-    const int j = j0 + lane % W;
-    const float bias = p.bias && j < p.N ? p.bias[j] : 0.f;
-#pragma unroll
-    for (int wi = 0; wi < WI; ++wi) {
-        const int i = i0 + wi * 16 + lane / W;
-        if (i0 + wi * 16 >= p.M) break;
-#pragma unroll
-        for (int wj = 0; wj < WJ; ++wj) *reinterpret_cast<f4 *>(own + (lane & 15) * LD + wj * 16 + (lane >> 4) * 4) = acc[wi][wj];
-#pragma unroll
-        for (int r = 0; r < N; ++r) {
-            const float v = own[(r * AT_ONCE + lane / W) * LD + lane % W] + bias;
-            if (i + r * AT_ONCE < p.M && j < p.N) store1(p, i + r * AT_ONCE, j, v);
+            const f4 v = acc[wi][wj] + bias[wj];
+            if (j + 4 <= p.N) store4(p, i, j, v);
+            else
+                for (int r = 0; r < 3; ++r)
+                    if (j + r < p.N) store1(p, i, j + r, v[r]);
         }
     }
 }
@@ -279,7 +268,6 @@ __global__ void __launch_bounds__(CFG::T) k_matmul_blocks(Product p) {
     constexpr int BM = CFG::BM, BN = CFG::BN, T = CFG::T, WI = CFG::WI, WJ = CFG::WJ;
     static_assert((BM + BN) / 64 <= CFG::NWM * CFG::NWN, "one wave per 64 scales");
     static_assert(!COMMON || 128 % (16 * WJ) == 0, "a wave's columns share their scale");
-    static_assert(CFG::NWM * CFG::NWN * 16 * (WJ * 16 + 4) * 4 <= CFG::STAGE, "LDS");
     NT_STAGES(st, CFG::STAGES, CFG::STAGE + (BM + BN) * 4);
     __shared__ int flag;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -326,7 +314,7 @@ __global__ void __launch_bounds__(CFG::T) k_matmul_blocks(Product p) {
             nt::products8<WI, WJ, FA, FB, COMMON, WIDE>(s + ra * 128, s + (BM + rb) * 128, sc + ra, sc + BM + rb, lane, acc, between);
         });
     if (p.pieces > 1 && !nt::join<T>(acc, piece, p.pieces, p.parts + int64_t(tile) * (BM * BN), tiles, p.counts + tile, &flag, tid)) return;
-    write_c<WI, WJ>(p, acc, reinterpret_cast<float *>(st[0]) + wave * 16 * (WJ * 16 + 4), i0 + ra, j0 + rb, lane);
+    write_c<WI, WJ>(p, acc, i0 + ra, j0 + rb, lane);
 }
 
 // Few rows of A: bound by reading B once.  A workgroup takes sixteen rows of B and its eight waves an eighth of k each, straight
@@ -398,7 +386,7 @@ __global__ void __launch_bounds__(512) k_matmul_blocks_rows(Product p) {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
             if (p.bias && j + r < p.N) v[r] += p.bias[j + r];
-        if (p.c_vec && j + 4 <= p.N) store4(p, i, j, v);
+        if (j + 4 <= p.N) store4(p, i, j, v);
         else
             for (int r = 0; r < 4; ++r)
                 if (j + r < p.N) store1(p, i, j + r, v[r]);
@@ -569,7 +557,6 @@ extern "C" int cp_matmul_blocks(cp_ctx *ctx, const cp_blocks *A, const cp_blocks
     p.a_shift = A->tile == 1 ? 0 : 7;
     p.b_shift = B->tile == 1 ? 0 : 7;
     p.c_dtype = c_dtype;
-    p.c_vec = ldc % 4 == 0 && uintptr_t(C) % (4 * size) == 0;
     const bool a5 = A->fmt == CP_E5M2, b5 = B->fmt == CP_E5M2;
     if (a5 && b5) launch_product<1, 1>(ctx, p, f);
     else if (a5) launch_product<1, 0>(ctx, p, f);

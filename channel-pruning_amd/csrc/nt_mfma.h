@@ -33,6 +33,15 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef int i8v __attribute__((ext_vector_type(8)));
 typedef int i4v __attribute__((ext_vector_type(4)));
 
+// the same, at any element's address: the vector loads and stores of this chip take any alignment
+typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef f4 f4u __attribute__((aligned(4)));
+typedef h4 h4u __attribute__((aligned(2)));
+typedef h8 h8u __attribute__((aligned(2)));
+typedef b4 b4u __attribute__((aligned(2)));
+typedef b8 b8u __attribute__((aligned(2)));
+
 __device__ __forceinline__ void load_lds16(const char *g, char *l) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)g,
                                      (__attribute__((address_space(3))) void *)l, 16, 0, 0);
@@ -237,12 +246,10 @@ __device__ __forceinline__ void products8(const char *a, const char *b, const fl
     f4 sj[WJ], t[2][WJ];
     float si[2];
     const float common = COMMON ? sb[0] : 1.f;
-    auto join = [&](int i) {   // a row group's products join the accumulators while the next one's are formed
+    auto join = [&](int i, int j) {   // a row group's products join the accumulators while the next one's are formed
 #pragma unroll
-        for (int j = 0; j < WJ; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                acc[i][j][r] = fmaf(t[i & 1][j][r], COMMON ? si[i & 1] : si[i & 1] * sj[j][r], acc[i][j][r]);
+        for (int r = 0; r < 4; ++r)
+            acc[i][j][r] = fmaf(t[i & 1][j][r], COMMON ? si[i & 1] : si[i & 1] * sj[j][r], acc[i][j][r]);
     };
     af[0].load(a, o0, o1);
     si[0] = sa[lane & 15] * common;
@@ -255,16 +262,28 @@ __device__ __forceinline__ void products8(const char *a, const char *b, const fl
 #pragma unroll
     for (int i = 0; i < WI; ++i) {
         const int u = i & 1;
-        if (i + 1 < WI) af[u ^ 1].load(a + (i + 1) * 2048, o0, o1);
+        float next = 0.f;
+        if (i + 1 < WI) {
+            af[u ^ 1].load(a + (i + 1) * 2048, o0, o1);
+            if (COMMON) next = sa[(i + 1) * 16 + (lane & 15)];   // (registers are short where every column has its scale)
+        }
         between(i);
         NT_STAY();
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int j = 0; j < WJ; ++j) t[u][j] = block_product<FA, FB, WIDE>(af[u], bf[j]);
-        if (i > 0) join(i - 1);
-        if (i + 1 < WI) si[u ^ 1] = sa[(i + 1) * 16 + (lane & 15)] * common;
+        for (int j = 0; j < WJ; ++j) {
+            t[u][j] = block_product<FA, FB, WIDE>(af[u], bf[j]);
+            if (i > 0) join(i - 1, j);
+            // a matrix instruction, then the vector instructions that fit beside it
+            __builtin_amdgcn_sched_group_barrier(0x008, WIDE ? 4 : 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, COMMON ? 4 : 8, 0);
+        }
+        __builtin_amdgcn_s_setprio(0);
+        if (i + 1 < WI) si[u ^ 1] = COMMON ? next * common : sa[(i + 1) * 16 + (lane & 15)];
         NT_STAY();
     }
-    join(WI - 1);
+#pragma unroll
+    for (int j = 0; j < WJ; ++j) join(WI - 1, j);
 }
 
 // ---- tiles that several workgroups share ---------------------------------------------------------------------------------

@@ -40,7 +40,6 @@ struct Job {
     int rows, cols, mp, np;
     int sum_rows, rows_per, width, chunks;   // |U|: rows, and rows, columns that a workgroup sums, chunks of columns
     int16_t g_dtype, o_dtype;
-    int16_t vec_in, vec_sum, vec_out;   // whether eight numbers of G and M / four of the output can be moved at once
     float lr;                    // lr * gamma
 };
 
@@ -84,33 +83,31 @@ __device__ __forceinline__ void store_as(void *p, int dtype, int64_t at, float v
     else if (dtype == CP_BF16) static_cast<__bf16 *>(p)[at] = __bf16(v);
     else static_cast<_Float16 *>(p)[at] = _Float16(v);
 }
-typedef __bf16 b4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ f4 load4_as_float(const void *p, int dtype, int64_t at) {
-    if (dtype == CP_F32) return *reinterpret_cast<const f4 *>(static_cast<const float *>(p) + at);
-    if (dtype == CP_BF16) return __builtin_convertvector(*reinterpret_cast<const b4 *>(static_cast<const __bf16 *>(p) + at), f4);
-    return __builtin_convertvector(*reinterpret_cast<const h4 *>(static_cast<const _Float16 *>(p) + at), f4);
+    if (dtype == CP_F32) return *reinterpret_cast<const nt::f4u *>(static_cast<const float *>(p) + at);
+    if (dtype == CP_BF16) return __builtin_convertvector(*reinterpret_cast<const nt::b4u *>(static_cast<const __bf16 *>(p) + at), f4);
+    return __builtin_convertvector(*reinterpret_cast<const nt::h4u *>(static_cast<const _Float16 *>(p) + at), f4);
 }
 __device__ __forceinline__ void store4_as(void *p, int dtype, int64_t at, f4 v) {
-    if (dtype == CP_F32) *reinterpret_cast<f4 *>(static_cast<float *>(p) + at) = v;
-    else if (dtype == CP_BF16) *reinterpret_cast<b4 *>(static_cast<__bf16 *>(p) + at) = __builtin_convertvector(v, b4);
-    else *reinterpret_cast<h4 *>(static_cast<_Float16 *>(p) + at) = __builtin_convertvector(v, h4);
+    if (dtype == CP_F32) *reinterpret_cast<nt::f4u *>(static_cast<float *>(p) + at) = v;
+    else if (dtype == CP_BF16) *reinterpret_cast<nt::b4u *>(static_cast<__bf16 *>(p) + at) = __builtin_convertvector(v, nt::b4);
+    else *reinterpret_cast<nt::h4u *>(static_cast<_Float16 *>(p) + at) = __builtin_convertvector(v, h4);
 }
 
 // eight numbers of a row from column c, zero from `cols` on
-__device__ __forceinline__ void load8(const void *row, int dtype, int c, int cols, bool vec, float (&v)[8]) {
-    if (vec && c + 8 <= cols) {
+__device__ __forceinline__ void load8(const void *row, int dtype, int c, int cols, float (&v)[8]) {
+    if (c + 8 <= cols) {
         if (dtype == CP_F32) {
-            const f4 *p = reinterpret_cast<const f4 *>(static_cast<const float *>(row) + c);
+            const nt::f4u *p = reinterpret_cast<const nt::f4u *>(static_cast<const float *>(row) + c);
             const f4 a = p[0], b = p[1];
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = a[e], v[e + 4] = b[e];
         } else if (dtype == CP_BF16) {
-            typedef __bf16 b8 __attribute__((ext_vector_type(8)));
-            const b8 a = *reinterpret_cast<const b8 *>(static_cast<const __bf16 *>(row) + c);
+            const nt::b8 a = *reinterpret_cast<const nt::b8u *>(static_cast<const __bf16 *>(row) + c);
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = float(a[e]);
         } else {
-            const h8 a = *reinterpret_cast<const h8 *>(static_cast<const _Float16 *>(row) + c);
+            const h8 a = *reinterpret_cast<const nt::h8u *>(static_cast<const _Float16 *>(row) + c);
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = float(a[e]);
         }
@@ -155,18 +152,18 @@ __global__ void __launch_bounds__(256) k_ortho_norm(Jobs js, Table t, float mome
     for (int u = threadIdx.x; u < (r1 - r0) * eights; u += 256) {
         const int k = r1 - r0 > 1 ? u / eights : 0, r = r0 + k, c = (u - k * eights) * 8;
         float v[8];
-        load8(row_of(j.G, j.g_dtype, r * j.ldg + c0), j.g_dtype, c, wide, j.vec_sum, v);
+        load8(row_of(j.G, j.g_dtype, r * j.ldg + c0), j.g_dtype, c, wide, v);
         if (j.M) {
             float *row = j.M + r * j.ldm + c0, m[8];
-            load8(row, CP_F32, c, wide, j.vec_sum, m);
+            load8(row, CP_F32, c, wide, m);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 m[e] = fmaf(momentum, m[e], v[e]);
                 v[e] = nesterov ? fmaf(momentum, m[e], v[e]) : m[e];
             }
-            if (j.vec_sum && c + 8 <= wide) {
-                *reinterpret_cast<f4 *>(row + c) = f4{m[0], m[1], m[2], m[3]};
-                *reinterpret_cast<f4 *>(row + c + 4) = f4{m[4], m[5], m[6], m[7]};
+            if (c + 8 <= wide) {
+                *reinterpret_cast<nt::f4u *>(row + c) = f4{m[0], m[1], m[2], m[3]};
+                *reinterpret_cast<nt::f4u *>(row + c + 4) = f4{m[4], m[5], m[6], m[7]};
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
@@ -233,32 +230,15 @@ __device__ __forceinline__ f4 transpose4(f4 v, int lane) {
 }
 
 // ---- X = U / (|U|_F + eps) in both orientations, zero in the padding: one 64 x 64 tile of G to a workgroup --------------------
-// sixteen of a tile's numbers as a thread reads them: of one row where rows are aligned, else of one column's 64 lanes
-__device__ __forceinline__ void load_tile(const void *p, int dtype, int64_t ld, const Job &j, int r0, int c0, int tid, float (&v)[16]) {
-    if (j.vec_in) {
-        const int r = r0 + (tid >> 2), c = c0 + (tid & 3) * 16;
-        float a[8] = {}, b[8] = {};
-        if (r < j.rows) {
-            load8(row_of(p, dtype, r * ld), dtype, c, j.cols, true, a);
-            load8(row_of(p, dtype, r * ld), dtype, c + 8, j.cols, true, b);
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = a[e], v[e + 8] = b[e];
-        return;
+// sixteen numbers of a tile's row
+__device__ __forceinline__ void load_tile(const void *p, int dtype, int64_t ld, const Job &j, int r, int c, float (&v)[16]) {
+    float a[8] = {}, b[8] = {};
+    if (r < j.rows) {
+        load8(row_of(p, dtype, r * ld), dtype, c, j.cols, a);
+        load8(row_of(p, dtype, r * ld), dtype, c + 8, j.cols, b);
     }
-    const int c = c0 + (tid & 63), r = r0 + (tid >> 6);
-    const int64_t at = int64_t(r) * ld + c;
-    const bool in = c < j.cols;
-    if (dtype == CP_F32) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = in && r + 4 * e < j.rows ? static_cast<const float *>(p)[at + 4 * e * ld] : 0.f;
-    } else if (dtype == CP_BF16) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = in && r + 4 * e < j.rows ? float(static_cast<const __bf16 *>(p)[at + 4 * e * ld]) : 0.f;
-    } else {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = in && r + 4 * e < j.rows ? float(static_cast<const _Float16 *>(p)[at + 4 * e * ld]) : 0.f;
-    }
+    for (int e = 0; e < 8; ++e) v[e] = a[e], v[e + 8] = b[e];
 }
 
 template <bool SPLIT>
@@ -273,15 +253,15 @@ __global__ void __launch_bounds__(256) k_ortho_load(Table tab, float momentum, i
     const int tid = threadIdx.x, line = tid >> 2, k = (tid & 3) * 16;
     float v[16];
     if (j.M) {
-        load_tile(j.M, CP_F32, j.ldm, j, r0, c0, tid, v);
+        load_tile(j.M, CP_F32, j.ldm, j, r0 + line, c0 + k, v);
         if (nesterov) {
             float u[16];
-            load_tile(j.G, j.g_dtype, j.ldg, j, r0, c0, tid, u);
+            load_tile(j.G, j.g_dtype, j.ldg, j, r0 + line, c0 + k, u);
 #pragma unroll
             for (int e = 0; e < 16; ++e) v[e] = fmaf(momentum, v[e], u[e]);
         }
     } else {
-        load_tile(j.G, j.g_dtype, j.ldg, j, r0, c0, tid, v);
+        load_tile(j.G, j.g_dtype, j.ldg, j, r0 + line, c0 + k, v);
     }
     const int n_part = (j.sum_rows + j.rows_per - 1) / j.rows_per * j.chunks;
     double part = 0.0;
@@ -293,16 +273,13 @@ __global__ void __launch_bounds__(256) k_ortho_load(Table tab, float momentum, i
     const double inv = norm > 0.0 || norm != norm ? double(x_scale) / norm : 0.0;
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-        const float x = float(double(v[e]) * inv);
-        if (j.vec_in) t[line][k + e] = x;
-        else t[(tid >> 6) + 4 * e][tid & 63] = x;
+        v[e] = float(double(v[e]) * inv);
+        t[line][k + e] = v[e];
     }
-    __syncthreads();
     char *n = tall ? j.xt0 : j.x, *o = tall ? j.x : j.xt0;
     const uint32_t ldn = tall ? j.lds : j.ldn, ldo = tall ? j.ldn : j.lds;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) v[e] = t[line][k + e];
     store16<SPLIT>(n + int64_t(r0 + line) * ldn, c0 + k, v);
+    __syncthreads();
 #pragma unroll
     for (int e = 0; e < 16; ++e) v[e] = t[k + e][line];
     store16<SPLIT>(o + int64_t(c0 + line) * ldo, r0 + k, v);
@@ -316,33 +293,6 @@ struct Factors {
     float keep;           // LAST: 1 - lr * weight_decay (cp_ortho_step)
     int xt;               // which X^T is read
 };
-
-// A wave's part of O or W where rows are not aligned: sixteen rows at a time go through LDS (its own), so that lanes hold
-// neighbours of a row.  W is read where it is there, without a branch, and all of a group before the first is written.
-template <typename T, int WI, int WJ>
-__device__ __forceinline__ void write_rows(const Job &j, const Factors &f, const f4 (&acc)[WI][WJ], float *own, int i0, int j0, int lane) {
-    constexpr int W = WJ * 16, LD = W + 4, AT_ONCE = 64 / W, N = 16 / AT_ONCE;
-    T *out = static_cast<T *>(j.out);
-    const int c = j0 + lane % W;
-#pragma unroll
-    for (int wi = 0; wi < WI; ++wi) {
-        const int i = i0 + wi * 16 + lane / W;
-        if (i0 + wi * 16 >= j.rows) break;
-        float w[N];
-        if (j.M) {
-#pragma unroll
-            for (int r = 0; r < N; ++r) w[r] = float(out[int64_t(min(i + r * AT_ONCE, j.rows - 1)) * j.ldo + min(c, j.cols - 1)]);
-        }
-#pragma unroll
-        for (int wj = 0; wj < WJ; ++wj) *reinterpret_cast<f4 *>(own + (lane & 15) * LD + wj * 16 + (lane >> 4) * 4) = acc[wi][wj] * f.acc;
-#pragma unroll
-        for (int r = 0; r < N; ++r) {
-            float o = own[(r * AT_ONCE + lane / W) * LD + lane % W];
-            if (j.M) o = f.keep * w[r] - j.lr * o;
-            if (i + r * AT_ONCE < j.rows && c < j.cols) out[int64_t(i + r * AT_ONCE) * j.ldo + c] = T(o);
-        }
-    }
-}
 
 template <int PHASE, bool SPLIT, class CFG>
 __global__ void __launch_bounds__(CFG::T) k_ortho_product(Table tab, Factors f, float *parts, int *counts) {
@@ -392,14 +342,6 @@ __global__ void __launch_bounds__(CFG::T) k_ortho_product(Table tab, Factors f, 
         });
     if (pieces > 1 && !nt::join<T>(acc, piece, pieces, parts + int64_t(first + tile) * (BM * BN), tiles, counts + first + tile, &flag, tid))
         return;
-    if (PHASE == LAST && !j.vec_out) {
-        float *own = reinterpret_cast<float *>(st[0]) + wave * 16 * (WJ * 16 + 4);
-        static_assert(CFG::NWM * CFG::NWN * 16 * (WJ * 16 + 4) * 4 <= CFG::STAGE, "LDS");
-        if (j.o_dtype == CP_F32) write_rows<float>(j, f, acc, own, i0 + ra, j0 + rb, lane);
-        else if (j.o_dtype == CP_BF16) write_rows<__bf16>(j, f, acc, own, i0 + ra, j0 + rb, lane);
-        else write_rows<_Float16>(j, f, acc, own, i0 + ra, j0 + rb, lane);
-        return;
-    }
 #pragma unroll
     for (int wi = 0; wi < WI; ++wi) {
         const int i = i0 + ra + wi * 16 + (lane & 15);
@@ -691,14 +633,10 @@ int lay_out(cp_ctx *ctx, const std::vector<Request> &rq, double lr, Layout &lay)
         j.lds = uint32_t(mp * e);
         j.g_dtype = int16_t(r.g_dtype);
         j.o_dtype = int16_t(r.o_dtype);
-        const bool aligned = uintptr_t(r.G) % 16 == 0 && uintptr_t(r.M) % 16 == 0;
-        j.vec_in = aligned && r.ldg * type_size(r.g_dtype) % 16 == 0 && r.ldm % 4 == 0;
-        j.vec_out = uintptr_t(r.out) % (4 * type_size(r.o_dtype)) == 0 && r.ldo % 4 == 0;
         j.lr = float(lr * r.gamma);
         const bool flat = r.ldg == r.cols && (!r.M || r.ldm == r.cols);
         j.sum_rows = flat ? 1 : r.rows;
         j.sum_cols = flat ? int64_t(r.rows) * r.cols : r.cols;
-        j.vec_sum = flat ? aligned : j.vec_in;
         j.width = flat ? int(std::max<int64_t>(4096, (j.sum_cols / kPartials + 2048) / 2048 * 2048)) : 4096;
         j.chunks = int((j.sum_cols + j.width - 1) / j.width);
         j.rows_per = int(std::max<int64_t>(1, 4096 / std::min<int64_t>(j.sum_cols, 4096)));
