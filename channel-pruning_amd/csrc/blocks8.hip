@@ -30,11 +30,14 @@ int check_blocks(cp_ctx *ctx, const cp_blocks *m, const char *name) {
 // ---- the cast ------------------------------------------------------------------------------------------------------------
 // One workgroup takes a 128 x 128 tile: exactly one block column of the matrix and, transposed, one of out_t.  A thread keeps
 // an 8 x 8 patch in registers, so x is read once for both orientations; a wave's patches form 64 x 64, which makes the
-// segments that it writes 64 bytes long in either.  Bound by HBM.
+// segments that it writes 64 bytes long in either.  Bound by HBM, as long as the arithmetic stays short: the largest magnitudes
+// are found on the bit patterns; a thread makes the factors of one row or column, not of its patch's sixteen; and what only
+// infinities and NaN need is done in tiles that hold one.  (No cut to +-fmax is needed: a finite x times the inverse exceeds
+// fmax by two roundings at most, and rounds to it.)
 struct Held {
     uint8_t *q;
     float *scale;
-    int64_t ld, lds;
+    int64_t rows, ld, lds;
     int fmt, tile;
 };
 
@@ -59,15 +62,52 @@ __device__ __forceinline__ void load8(const _Float16 *p, float (&v)[8]) {
     for (int e = 0; e < 8; ++e) v[e] = float(a[e]);
 }
 
-__device__ __forceinline__ float finite_abs(float v) {
-    const float a = fabsf(v);
-    return a <= FLT_MAX ? a : 0.f;
+constexpr uint32_t kInf = 0x7f800000u;
+// |v| as an integer of the same order; FINITE: zero for what is not
+template <bool FINITE>
+__device__ __forceinline__ uint32_t magnitude(float v) {
+    const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
+    return FINITE && b >= kInf ? 0u : b;
+}
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t max_with(uint32_t v) {
+    return max(v, uint32_t(__builtin_amdgcn_update_dpp(0, int(v), CTRL, 0xf, 0xf, true)));
+}
+
+// The largest magnitudes into LDS: of the rows over this wave's 64 columns, of the columns over this thread's eight rows
+// (group: which eight of the tile).  Returns the thread's largest.
+template <bool FINITE>
+__device__ __forceinline__ uint32_t maxima(const float (&v)[8][8], uint32_t *rmax, uint32_t *cmax, bool columns, int lr, int lane) {
+    uint32_t all = 0, rm[8], cm[8] = {};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        rm[i] = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t m = magnitude<FINITE>(v[i][j]);
+            rm[i] = max(rm[i], m);
+            cm[j] = max(cm[j], m);
+        }
+        all = max(all, rm[i]);
+        NT_STAY();   // one row after the other: all magnitudes at once would take as many registers again
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) rm[i] = max_with<0x141>(max_with<0x4E>(max_with<0xB1>(rm[i])));   // over eight neighbouring lanes
+    if ((lane & 7) == 0) {
+        *reinterpret_cast<uint4 *>(rmax + lr) = make_uint4(rm[0], rm[1], rm[2], rm[3]);
+        *reinterpret_cast<uint4 *>(rmax + lr + 4) = make_uint4(rm[4], rm[5], rm[6], rm[7]);
+    }
+    if (columns) {
+        *reinterpret_cast<uint4 *>(cmax) = make_uint4(cm[0], cm[1], cm[2], cm[3]);
+        *reinterpret_cast<uint4 *>(cmax + 4) = make_uint4(cm[4], cm[5], cm[6], cm[7]);
+    }
+    return all;
 }
 
 // a block's scale and the factor that its elements are cast with
-__device__ __forceinline__ void scale_of(float amax, int fmt, bool pow2, float &scale, float &inv) {
-    const float top = fmt == CP_E4M3 ? 448.f : 57344.f;
-    amax = fmaxf(amax, kTiny);
+__device__ __forceinline__ void scale_of(uint32_t largest, int fmt, bool pow2, float &scale, float &inv) {
+    const float top = fmt == CP_E4M3 ? 448.f : 57344.f, amax = fmaxf(__uint_as_float(largest), kTiny);
     scale = amax / top;
     if (pow2) {
         const uint32_t b = __float_as_uint(scale), e = (b >> 23) + ((b & 0x7fffffu) != 0);   // scale is a normal number
@@ -78,14 +118,18 @@ __device__ __forceinline__ void scale_of(float amax, int fmt, bool pow2, float &
     }
 }
 
-__device__ __forceinline__ float cut(float x, float inv, float top) {
-    const float y = __builtin_amdgcn_fmed3f(x * inv, -top, top);
-    return fabsf(x) <= FLT_MAX ? y : __uint_as_float(0x7fc00000u);
-}
-
-__device__ __forceinline__ uint32_t pack4(const float (&y)[4], int fmt) {
+// four numbers times their factor, in 8 bits; SPECIAL: what is not finite becomes NaN
+template <int FMT, bool SPECIAL>
+__device__ __forceinline__ uint32_t pack4(float x0, float x1, float x2, float x3, float inv) {
+    const float x[4] = {x0, x1, x2, x3};
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        y[e] = x[e] * inv;
+        if (SPECIAL && magnitude<false>(x[e]) >= kInf) y[e] = __uint_as_float(0x7fc00000u);
+    }
     int w = 0;
-    if (fmt == CP_E4M3) {
+    if (FMT == CP_E4M3) {
         w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], w, false);
         w = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
     } else {
@@ -95,106 +139,104 @@ __device__ __forceinline__ uint32_t pack4(const float (&y)[4], int fmt) {
     return uint32_t(w);
 }
 
+// a thread's patch into its eight rows of a matrix (TURN: of the transpose), `at`: the first's place, n: how many there are
+template <int FMT, bool SPECIAL, bool TURN>
+__device__ __forceinline__ void write_patch(const float (&v)[8][8], const float *inverse, uint8_t *at, int64_t ld, int64_t n) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (i >= n) break;
+        const float f = inverse[i];
+        uint2 w;
+        w.x = TURN ? pack4<FMT, SPECIAL>(v[0][i], v[1][i], v[2][i], v[3][i], f) : pack4<FMT, SPECIAL>(v[i][0], v[i][1], v[i][2], v[i][3], f);
+        w.y = TURN ? pack4<FMT, SPECIAL>(v[4][i], v[5][i], v[6][i], v[7][i], f) : pack4<FMT, SPECIAL>(v[i][4], v[i][5], v[i][6], v[i][7], f);
+        *reinterpret_cast<uint2 *>(at) = w;
+        at += ld;
+        NT_STAY();   // row after row, in few registers
+    }
+}
+template <bool TURN>
+__device__ __forceinline__ void write_patch(const float (&v)[8][8], const float *inverse, const Held &h, int64_t row, int64_t col, bool special) {
+    uint8_t *at = h.q + row * h.ld + col;
+    const int64_t n = h.rows - row;
+    if (h.fmt == CP_E4M3) special ? write_patch<CP_E4M3, true, TURN>(v, inverse, at, h.ld, n) : write_patch<CP_E4M3, false, TURN>(v, inverse, at, h.ld, n);
+    else special ? write_patch<CP_E5M2, true, TURN>(v, inverse, at, h.ld, n) : write_patch<CP_E5M2, false, TURN>(v, inverse, at, h.ld, n);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(256) k_quant_blocks(const T *__restrict__ x, int64_t rows, int64_t cols, int64_t ldx, int pow2,
                                                       Held o, Held t) {
-    __shared__ float rmax[2][128], cmax[2][128];
+    __shared__ alignas(16) uint32_t rmax[2][128], cmax[16][128];
+    __shared__ float inverse[2][128];   // of the tile's rows and columns
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int lr = (wave >> 1) * 64 + (lane >> 3) * 8, lc = (wave & 1) * 64 + (lane & 7) * 8;
     const int64_t r0 = int64_t(blockIdx.y) * 128, c0 = int64_t(blockIdx.x) * 128;
     const int64_t row = r0 + lr, col = c0 + lc;
 
     float v[8][8];
+    const T *p = x + row * ldx + col;
+    if (r0 + 128 <= rows && c0 + 128 <= cols) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const T *p = x + (row + i) * ldx + col;
-        if (row + i < rows && col + 8 <= cols) {
-            load8(p, v[i]);
-        } else {
+        for (int i = 0; i < 8; ++i) load8(p + i * ldx, v[i]);
+    } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = row + i < rows && col + j < cols ? float(p[j]) : 0.f;
+        for (int i = 0; i < 8; ++i, p += ldx) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+            if (row + i < rows) {
+                if (col + 8 <= cols) {
+                    load8(p, v[i]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (col + j < cols) v[i][j] = float(p[j]);
+                }
+            }
+            NT_STAY();   // the edge's rows one after the other, in few registers
         }
     }
+    const uint32_t mine = maxima<false>(v, rmax[wave & 1], cmax[lr >> 3] + lc, t.q, lr, lane);
+    const bool special = __syncthreads_or(mine >= kInf);
+    if (special) {
+        // (to the compiler these are new numbers: it would keep 64 magnitudes in registers for this rare path)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        float m = 0.f;
+        for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_abs(v[i][j]));
-        for (int s = 1; s < 8; s <<= 1) m = fmaxf(m, __shfl_xor(m, s));
-        if ((lane & 7) == 0) rmax[wave & 1][lr + i] = m;
+            for (int j = 0; j < 8; ++j) asm volatile("" : "+v"(v[i][j]));
+        maxima<true>(v, rmax[wave & 1], cmax[lr >> 3] + lc, t.q, lr, lane);
+        __syncthreads();
     }
-    if (t.q) {
+    // thread k < 128: row k of the tile; 128 + k: column k
+    {
+        const bool is_col = tid >= 128;
+        const int k = tid & 127;
+        const Held &h = is_col ? t : o;
+        if (h.q) {
+            uint32_t m = max(rmax[0][k], rmax[1][k]);
+            if (is_col) {
+                m = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            float m = 0.f;
+                for (int g = 0; g < 16; ++g) m = max(m, cmax[g][k]);
+            }
+            if (h.tile != 1) {
+                m = max(max(rmax[0][lane], rmax[1][lane]), max(rmax[0][lane + 64], rmax[1][lane + 64]));
 #pragma unroll
-            for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_abs(v[i][j]));
-            for (int s = 8; s < 64; s <<= 1) m = fmaxf(m, __shfl_xor(m, s));
-            if (lane < 8) cmax[wave >> 1][lc + j] = m;
+                for (int s = 1; s < 64; s <<= 1) m = max(m, uint32_t(__shfl_xor(int(m), s)));
+            }
+            float scale;
+            scale_of(m, h.fmt, pow2, scale, inverse[is_col][k]);
+            float *sp = is_col ? t.scale + blockIdx.y * t.lds : o.scale + blockIdx.x * o.lds;
+            const int64_t at = (is_col ? c0 : r0) + k, n = is_col ? cols : rows;
+            if (h.tile == 1 ? at < n : k == 0) sp[h.tile == 1 ? at : at / 128] = scale;
         }
     }
     __syncthreads();
-    float whole = 0.f;
-    if ((o.q && o.tile != 1) || (t.q && t.tile != 1)) {
-        whole = fmaxf(fmaxf(rmax[0][lane], rmax[1][lane]), fmaxf(rmax[0][lane + 64], rmax[1][lane + 64]));
-        for (int s = 1; s < 64; s <<= 1) whole = fmaxf(whole, __shfl_xor(whole, s));
-    }
-    float scale, inv;
-    if (o.q) {
-        const float top = o.fmt == CP_E4M3 ? 448.f : 57344.f;
-        float *sp = o.scale + blockIdx.x * o.lds;
-        if (o.tile != 1) {
-            scale_of(whole, o.fmt, pow2, scale, inv);
-            if (tid == 0) sp[blockIdx.y] = scale;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (row + i >= rows) break;
-            if (o.tile == 1) {
-                scale_of(fmaxf(rmax[0][lr + i], rmax[1][lr + i]), o.fmt, pow2, scale, inv);
-                if (lc == 0) sp[row + i] = scale;
-            }
-            uint32_t w[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float y[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] = cut(v[i][4 * h + e], inv, top);
-                w[h] = pack4(y, o.fmt);
-            }
-            *reinterpret_cast<uint2 *>(o.q + (row + i) * o.ld + col) = make_uint2(w[0], w[1]);
-        }
-    }
-    if (t.q) {
-        const float top = t.fmt == CP_E4M3 ? 448.f : 57344.f;
-        float *sp = t.scale + blockIdx.y * t.lds;
-        if (t.tile != 1) {
-            scale_of(whole, t.fmt, pow2, scale, inv);
-            if (tid == 0) sp[blockIdx.x] = scale;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            if (col + j >= cols) break;
-            if (t.tile == 1) {
-                scale_of(fmaxf(cmax[0][lc + j], cmax[1][lc + j]), t.fmt, pow2, scale, inv);
-                if (lr == 0) sp[col + j] = scale;
-            }
-            uint32_t w[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float y[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] = cut(v[4 * h + e][j], inv, top);
-                w[h] = pack4(y, t.fmt);
-            }
-            *reinterpret_cast<uint2 *>(t.q + (col + j) * t.ld + row) = make_uint2(w[0], w[1]);
-        }
-    }
+    if (o.q) write_patch<false>(v, inverse[0] + lr, o, row, col, special);
+    if (t.q) write_patch<true>(v, inverse[1] + lc, t, col, row, special);
 }
 
 Held held(const cp_blocks *m) {
     Held h = {};
-    if (m) h = {static_cast<uint8_t *>(m->q), m->scale, m->ld, m->lds, m->fmt, m->tile};
+    if (m) h = {static_cast<uint8_t *>(m->q), m->scale, m->rows, m->ld, m->lds, m->fmt, m->tile};
     return h;
 }
 
