@@ -209,24 +209,33 @@ def _ptr(x):
     return int(x)
 
 
-_TORCH_NAMES = {CP_F32: "torch.float32", CP_F64: "torch.float64", CP_BF16: "torch.bfloat16", CP_F16: "torch.float16"}
+_TORCH_CODES = {}      # torch dtype -> dtype code, filled when torch is first seen
+
+
+def _torch_codes():
+    import torch
+    _TORCH_CODES.update({torch.float32: CP_F32, torch.float64: CP_F64, torch.bfloat16: CP_BF16, torch.float16: CP_F16})
+    return _TORCH_CODES
 
 
 def _matrix(x, dtype, rows, cols, ld, name):
     """(pointer, row stride in elements, device index or None) of a device matrix.  A torch tensor is held to the dtype code,
     the shape and unit column stride, and gives its own row stride; a DevBuf to its size; an int is taken as it is."""
-    if hasattr(x, "data_ptr"):
-        if tuple(x.shape) != (rows, cols) or (cols > 1 and rows and x.stride(1) != 1):
-            raise ValueError("%s: a [%d, %d] tensor with unit column stride is needed, got %s, strides %s"
-                             % (name, rows, cols, tuple(x.shape), tuple(x.stride())))
-        if str(x.dtype) != _TORCH_NAMES.get(dtype):
+    if hasattr(x, "stride"):
+        codes = _TORCH_CODES or _torch_codes()
+        if codes.get(x.dtype) != dtype:
             raise ValueError("%s: dtype code %r does not fit a tensor of %s" % (name, dtype, x.dtype))
-        if not x.is_cuda:
+        strides = x.stride()
+        if x.shape != (rows, cols) or (strides[1] != 1 and cols > 1 and rows):
+            raise ValueError("%s: a [%d, %d] tensor with unit column stride is needed, got %s, strides %s"
+                             % (name, rows, cols, tuple(x.shape), strides))
+        device = x.get_device()
+        if device < 0:
             raise ValueError("%s: a tensor on the device is needed" % name)
-        own = x.stride(0) if rows > 1 else max(cols, 1)
+        own = strides[0] if rows > 1 else max(cols, 1)
         if ld is not None and rows > 1 and ld != own:
             raise ValueError("%s: row stride %d does not fit the tensor's %d" % (name, ld, own))
-        return x.data_ptr(), own if ld is None else ld, x.device.index
+        return x.data_ptr(), own if ld is None else ld, device
     ld = max(cols, 1) if ld is None else int(ld)
     if isinstance(x, DevBuf):
         if rows and cols and ((rows - 1) * ld + cols) * (8 if dtype == CP_F64 else 4 if dtype == CP_F32 else 2) > x.nbytes:
@@ -269,7 +278,8 @@ class Blocks:
         self.q, self.scale, self.rows, self.cols, self.fmt, self.tile = q, scale, rows, cols, fmt, tile
         self.ld, self.lds = int(ld), int(lds)
         self.c = BlocksStruct(_ptr(q), _ptr(scale), rows, cols, self.ld, self.lds, fmt, tile)
-        rc = load().cp_blocks_check(ctypes.byref(self.c))
+        self.ref = ctypes.byref(self.c)
+        rc = load().cp_blocks_check(self.ref)
         if rc != 0:
             raise CpError(rc, "cp_blocks_check", "rows %d, cols %d, ld %d, lds %d, fmt %d, tile %d"
                           % (rows, cols, self.ld, self.lds, fmt, tile))
@@ -592,15 +602,12 @@ class Context:
                 bfr.free()
 
     # -- 8-bit matrices ----------------------------------------------------------------------
-    def _here(self, device, name):
-        if device is not None and device != self.device:
-            raise ValueError("%s is on device %d, the context on %d" % (name, device, self.device))
+    def _elsewhere(self, device, name):
+        raise ValueError("%s is on device %d, the context on %d" % (name, device, self.device))
 
     @staticmethod
     def _ws(ws):
-        if ws is None:
-            return None, 0
-        return _ptr(ws), int(ws.nbytes)
+        return (None, 0) if ws is None else (_ptr(ws), int(ws.nbytes))
 
     def quant_blocks(self, x, x_dtype, out=None, out_t=None, ldx=None, flags=0):
         """x [rows, cols] -> the 8-bit matrices out [rows, cols] and / or out_t [cols, rows] (Blocks), in one read of x
@@ -609,31 +616,34 @@ class Context:
             raise ValueError("no output")
         rows, cols = (out.rows, out.cols) if out is not None else (out_t.cols, out_t.rows)
         p, ldx, dev = _matrix(x, x_dtype, rows, cols, ldx, "x")
-        self._here(dev, "x")
-        for m in (out, out_t):
-            if m is not None:
-                self._here(m.device, "an output")
-        self._check(self.lib.cp_quant_blocks(self.h, p, x_dtype, rows, cols, ldx, flags,
-                                             ctypes.byref(out.c) if out is not None else None,
-                                             ctypes.byref(out_t.c) if out_t is not None else None), "cp_quant_blocks")
+        for d, name in ((dev, "x"), (out and out.device, "out"), (out_t and out_t.device, "out_t")):
+            if d is not None and d != self.device:
+                self._elsewhere(d, name)
+        rc = self.lib.cp_quant_blocks(self.h, p, x_dtype, rows, cols, ldx, flags, out and out.ref, out_t and out_t.ref)
+        if rc:
+            self._check(rc, "cp_quant_blocks")
 
     def matmul_blocks(self, A, B, C, c_dtype, bias=None, ldc=None, ws=None):
         """C [M, N] = A [M, K] B [N, K]^T (+ bias float32 [N]) of two Blocks (cp_matmul_blocks).  ws: None or a device buffer
         of matmul_blocks_workspace() bytes (needed under stream capture)."""
         p, ldc, dev = _matrix(C, c_dtype, A.rows, B.rows, ldc, "C")
         for d, name in ((dev, "C"), (A.device, "A"), (B.device, "B")):
-            self._here(d, name)
-        if hasattr(bias, "data_ptr"):
-            if tuple(bias.shape) != (B.rows,) or str(bias.dtype) != "torch.float32" or not bias.is_contiguous() or not bias.is_cuda:
-                raise ValueError("bias: a contiguous float32 tensor [%d] on the device is needed" % B.rows)
-            self._here(bias.device.index, "bias")
-        w, wb = self._ws(ws)
-        self._check(self.lib.cp_matmul_blocks(self.h, ctypes.byref(A.c), ctypes.byref(B.c), _ptr(bias), p, c_dtype, ldc, w, wb),
-                    "cp_matmul_blocks")
+            if d is not None and d != self.device:
+                self._elsewhere(d, name)
+        if bias is not None:
+            if hasattr(bias, "stride"):
+                if bias.shape != (B.rows,) or _TORCH_CODES.get(bias.dtype) != CP_F32 or not bias.is_contiguous() \
+                        or bias.get_device() != self.device:
+                    raise ValueError("bias: a contiguous float32 tensor [%d] on device %d is needed" % (B.rows, self.device))
+            bias = _ptr(bias)
+        w, wb = (None, 0) if ws is None else self._ws(ws)
+        rc = self.lib.cp_matmul_blocks(self.h, A.ref, B.ref, bias, p, c_dtype, ldc, w, wb)
+        if rc:
+            self._check(rc, "cp_matmul_blocks")
 
     def matmul_blocks_workspace(self, A, B, c_dtype, ldc=None):
         n = ctypes.c_size_t()
-        self._check(self.lib.cp_matmul_blocks_workspace(ctypes.byref(A.c), ctypes.byref(B.c), c_dtype,
+        self._check(self.lib.cp_matmul_blocks_workspace(A.ref, B.ref, c_dtype,
                                                         max(B.rows, 1) if ldc is None else ldc, ctypes.byref(n)),
                     "cp_matmul_blocks_workspace")
         return n.value
@@ -649,7 +659,8 @@ class Context:
     def orthogonalise(self, jobs, steps=5, coef=None, eps=1e-7, ws=None):
         """O = the Newton-Schulz approximation of G's orthogonal polar factor, for every matrix of an OrthoJobs list in common
         launches (cp_orthogonalise).  coef: (a, b, c) or one row per step; None = (3.4445, -4.7750, 2.0315)."""
-        self._here(jobs.device, "a job")
+        if jobs.device not in (None, self.device):
+            self._elsewhere(jobs.device, "a job")
         q = self._coef(coef, steps)
         w, wb = self._ws(ws)
         self._check(self.lib.cp_orthogonalise(self.h, jobs.n, jobs.c, steps, None if q is None else q.ctypes.data, eps, w, wb),
@@ -658,7 +669,8 @@ class Context:
     def ortho_step(self, jobs, lr, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coef=None, eps=1e-7, ws=None):
         """One optimiser step on every layer of an OrthoStepJobs list: momentum, orthogonalisation, decay, weights
         (cp_ortho_step).  G is read, M and W are updated."""
-        self._here(jobs.device, "a job")
+        if jobs.device not in (None, self.device):
+            self._elsewhere(jobs.device, "a job")
         q = self._coef(coef, steps)
         w, wb = self._ws(ws)
         self._check(self.lib.cp_ortho_step(self.h, jobs.n, jobs.c, lr, momentum, int(nesterov), weight_decay, steps,
