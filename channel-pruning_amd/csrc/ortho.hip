@@ -121,10 +121,32 @@ __device__ __forceinline__ const void *row_of(const void *p, int dtype, int64_t 
     return static_cast<const char *>(p) + at * (dtype == CP_F32 ? 4 : 2);
 }
 
+// One number for all of its uses.  The compiler may fuse a product with its rounding to fp16, but not with the difference from
+// that rounding: the halves of a pair would belong to different numbers.
+__device__ __forceinline__ float settled(float v) {
+    asm("" : "+v"(v));
+    return v;
+}
+__device__ __forceinline__ f4 settled(f4 v) { return f4{settled(v[0]), settled(v[1]), settled(v[2]), settled(v[3])}; }
+
 __device__ __forceinline__ double wave_sum(double v) {
     for (int s = 32; s; s >>= 1) v += __shfl_xor(v, s);
     return v;
 }
+
+// scale / (|U|_F + eps), which may lie outside float32 where its products with U do not: as a mantissa and an exponent
+struct Inverse {
+    float mantissa;
+    int exponent;
+    __device__ __forceinline__ Inverse(double sum, double eps, double scale) {
+        const double norm = sqrt(sum) + eps, inv = norm > 0.0 || norm != norm ? scale / norm : 0.0;
+        mantissa = float(__builtin_amdgcn_frexp_mant(inv));
+        exponent = __builtin_amdgcn_frexp_exp(inv);
+    }
+    __device__ __forceinline__ float times(float v) const {
+        return settled(ldexpf(v, exponent) * mantissa);
+    }
+};
 
 // ---- |U|_F, and the momentum: one pass over G (and M), bound by HBM -----------------------------------------------------------
 // A workgroup sums rows_per rows of a chunk of `width` columns; the partial sums are added in one order by whoever needs the
@@ -201,6 +223,7 @@ __device__ __forceinline__ void store16(char *row, int k, const float (&v)[16]) 
 template <bool SPLIT>
 __device__ __forceinline__ void store4(char *row, int k, f4 v) {
     char *p = row + (SPLIT ? (k >> 5) * 128 + (k & 31) * 2 : k * 2);
+    if (SPLIT) v = settled(v);
     const h4 hi = __builtin_convertvector(v, h4);
     *reinterpret_cast<h4 *>(p) = hi;
     if (SPLIT) *reinterpret_cast<h4 *>(p + 64) = __builtin_convertvector(v - __builtin_convertvector(hi, f4), h4);
@@ -269,11 +292,10 @@ __global__ void __launch_bounds__(256) k_ortho_load(Table tab, float momentum, i
     part = wave_sum(part);
     if ((tid & 63) == 0) s[tid >> 6] = part;
     __syncthreads();
-    const double norm = sqrt((s[0] + s[1]) + (s[2] + s[3])) + eps;
-    const double inv = norm > 0.0 || norm != norm ? double(x_scale) / norm : 0.0;
+    const Inverse inv((s[0] + s[1]) + (s[2] + s[3]), eps, x_scale);
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-        v[e] = float(double(v[e]) * inv);
+        v[e] = inv.times(v[e]);
         t[line][k + e] = v[e];
     }
     char *n = tall ? j.xt0 : j.x, *o = tall ? j.x : j.xt0;
@@ -378,6 +400,336 @@ __global__ void __launch_bounds__(CFG::T) k_ortho_product(Table tab, Factors f, 
                 }
             }
         }
+    }
+}
+
+// ---- small matrices: the whole step in one workgroup ---------------------------------------------------------------------------
+// Where the short side fits 64 rows and the long side the registers of eight waves, seventeen launches of 4.3 us each do 1 us
+// of arithmetic.  Here a workgroup keeps X in registers from the first product to the last.
+// A wave owns CT tiles of 16 columns, in the two forms that the matrix instruction's operands need: by columns (lane: column
+// j, eight rows; K = rows, for B X) and by rows (lane: row i, eight columns; K = columns, for X X^T).  The result of a product
+// IS such an operand (lane: column, four consecutive rows; or, with the operands exchanged, row and four columns) once K's
+// order within a block of 32 is taken as (4 g .. 4 g + 3, 16 + 4 g .. 16 + 4 g + 3) for lane group g: B X comes out in one form, a
+// product with the unit matrix turns it, exactly, into the other, and nothing of X passes through LDS.  Only A and B do.
+constexpr int kSmallWaves = 8;
+constexpr int kSmallJobs = 24;
+constexpr int kSmallTiles[2] = {8, 4};   // column tiles of a wave at most: one fp16 a number, pairs
+
+struct SmallJob {
+    const void *G;
+    float *M;
+    void *out;
+    int64_t ldg, ldm, ldo;
+    int rows, cols;
+    int g_dtype, o_dtype;
+    float lr;
+};
+struct StepFactors {
+    float gram, poly, a, diag, apply;   // what a step's accumulators, A's entry and the diagonal count for
+};
+struct SmallJobs {
+    SmallJob job[kSmallJobs];
+    StepFactors step[kMaxSteps];
+    double eps, x_scale;
+    float momentum, keep;
+    int nesterov, steps;
+};
+static_assert(sizeof(SmallJobs) <= 3900, "kernel arguments");
+
+template <bool SPLIT>
+struct Op {   // an operand: eight numbers of a lane, as fp16 or as pairs
+    h8 v[SPLIT ? 2 : 1];
+    __device__ __forceinline__ void set(int half, f4 x) {
+        if (SPLIT) x = settled(x);
+        const h4 hi = __builtin_convertvector(x, h4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[0][4 * half + e] = hi[e];
+        if constexpr (SPLIT) {
+            const h4 lo = __builtin_convertvector(x - __builtin_convertvector(hi, f4), h4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[1][4 * half + e] = lo[e];
+        }
+    }
+};
+template <bool SPLIT>
+__device__ __forceinline__ f4 multiply(const Op<SPLIT> &a, const Op<SPLIT> &b, f4 acc) {
+    if constexpr (SPLIT) {
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.v[1], b.v[0], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.v[0], b.v[1], acc, 0, 0, 0);
+    }
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a.v[0], b.v[0], acc, 0, 0, 0);
+}
+
+template <bool SPLIT, int CT, bool TALL>
+__global__ void __launch_bounds__(64 * kSmallWaves) k_ortho_small(SmallJobs js) {
+    constexpr int N = SPLIT ? 2 : 1, T = 64 * kSmallWaves, LONG = CT * kSmallWaves * 16;
+    constexpr int LD = 72;   // a row of A or B: 64 numbers, and eight that keep rows off one bank
+    // LDS: first X as it comes (G's rows); then the waves' shares of A, and A and B; last O's rows, half of the column tiles at a time
+    constexpr int R = TALL ? LONG : 64, C = TALL ? 64 : LONG, LDX = C + 8;   // G's padded shape
+    constexpr int RO = TALL ? LONG / 2 : 64, CO = TALL ? 64 : LONG / 2, LDO = CO + 4;
+    constexpr int PARTS = kSmallWaves * 10 * 64 * 16, MATS = N * 64 * LD * 2, XS = N * R * LDX * 2, OS = RO * LDO * 4;
+    constexpr int BYTES = (PARTS + 2 * MATS > XS ? PARTS + 2 * MATS : XS) > OS ? (PARTS + 2 * MATS > XS ? PARTS + 2 * MATS : XS) : OS;
+    __shared__ alignas(16) char lds[BYTES];
+    __shared__ double sums[kSmallWaves];
+    auto part = reinterpret_cast<float(*)[10][64][4]>(lds);
+    auto as = reinterpret_cast<_Float16(*)[64][LD]>(lds + PARTS), bs = reinterpret_cast<_Float16(*)[64][LD]>(lds + PARTS + MATS);
+    auto xs = reinterpret_cast<_Float16(*)[R][LDX]>(lds);
+    auto os = reinterpret_cast<float(*)[LDO]>(lds);
+    const SmallJob &j = js.job[blockIdx.x];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 15, g = lane >> 4;
+
+    // |U|, and the momentum
+    double sum = 0.0;
+    const int eights = (j.cols + 7) / 8;
+    for (int i = tid; i < j.rows * eights; i += T) {
+        const int r = i / eights, c = i % eights * 8;
+        float v[8];
+        load8(row_of(j.G, j.g_dtype, r * j.ldg), j.g_dtype, c, j.cols, v);
+        if (j.M) {
+            float *row = j.M + r * j.ldm, m[8];
+            load8(row, CP_F32, c, j.cols, m);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                m[e] = fmaf(js.momentum, m[e], v[e]);
+                v[e] = js.nesterov ? fmaf(js.momentum, m[e], v[e]) : m[e];
+                if (c + e < j.cols) row[c + e] = m[e];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = fma(double(v[e]), double(v[e]), sum);
+    }
+    sum = wave_sum(sum);
+    if (lane == 0) sums[wave] = sum;
+    __syncthreads();
+    sum = 0.0;
+#pragma unroll
+    for (int w = 0; w < kSmallWaves; ++w) sum += sums[w];
+    const Inverse inv(sum, js.eps, js.x_scale);
+    // X into LDS, zero in the padding.  (A thread reads the M that it wrote.)
+    for (int i = tid; i < j.rows * eights; i += T) {
+        const int r = i / eights, c = i % eights * 8;
+        float v[8];
+        load8(row_of(j.G, j.g_dtype, r * j.ldg), j.g_dtype, c, j.cols, v);
+        if (j.M) {
+            float m[8];
+            load8(j.M + r * j.ldm, CP_F32, c, j.cols, m);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = js.nesterov ? fmaf(js.momentum, m[e], v[e]) : m[e];
+        }
+        h8 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float x = inv.times(v[e]);
+            hi[e] = _Float16(x);
+            lo[e] = _Float16(x - float(hi[e]));
+        }
+        *reinterpret_cast<h8 *>(&xs[0][r][c]) = hi;
+        if constexpr (SPLIT) *reinterpret_cast<h8 *>(&xs[N - 1][r][c]) = lo;
+    }
+    for (int i = tid; i < R * (C / 8); i += T) {
+        const int r = i / (C / 8), c = i % (C / 8) * 8;
+        if (r < j.rows && c < j.cols) continue;
+        const h8 z = {};
+#pragma unroll
+        for (int s = 0; s < N; ++s) *reinterpret_cast<h8 *>(&xs[s][r][c]) = z;
+    }
+    __syncthreads();
+
+    // X by columns, xc[c][h] (rows 32 h ..), and by rows, xr[t][p] (tiles 2 p, 2 p + 1).  G's rows give one form; a product with
+    // the unit matrix gives the other, exactly
+    Op<SPLIT> xc[CT][2], xr[4][CT / 2];
+    h8 unit[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) unit[s][e] = _Float16((e >> 2) == s && 4 * g + (e & 3) == n ? 1.f : 0.f);
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int s = 0; s < N; ++s) {
+                const int tile = (wave * CT + c) * 16, row = TALL ? tile + n : t * 16 + n, col = (TALL ? t * 16 : tile) + g * 4;
+                const h4 x = *reinterpret_cast<const h4 *>(&xs[s][row][col]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (TALL) xc[c][t >> 1].v[s][4 * (t & 1) + e] = x[e];
+                    else xr[t][c >> 1].v[s][4 * (c & 1) + e] = x[e];
+                }
+            }
+    auto turn = [&](int c) {   // the other form of a column tile
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int s = 0; s < N; ++s) {
+                const f4 z = {0.f, 0.f, 0.f, 0.f};
+                const f4 y = TALL ? __builtin_amdgcn_mfma_f32_16x16x32_f16(xc[c][t >> 1].v[s], unit[t & 1], z, 0, 0, 0)
+                                  : __builtin_amdgcn_mfma_f32_16x16x32_f16(xr[t][c >> 1].v[s], unit[c & 1], z, 0, 0, 0);
+                const h4 q = __builtin_convertvector(y, h4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (TALL) xr[t][c >> 1].v[s][4 * (c & 1) + e] = q[e];
+                    else xc[c][t >> 1].v[s][4 * (t & 1) + e] = q[e];
+                }
+            }
+    };
+#pragma unroll
+    for (int c = 0; c < CT; ++c) turn(c);
+    __syncthreads();   // X has left LDS
+
+    const int long_side = TALL ? j.rows : j.cols, shares = min(kSmallWaves, (long_side + CT * 16 - 1) / (CT * 16));   // waves with columns
+    // a step's B, in fragments
+    Op<SPLIT> bf[4][2];
+    auto make_b = [&](const StepFactors &f) {
+        if (wave < shares) {   // this wave's share of A = X X^T: tile (a, b) as (lane: row of a, four rows of b)
+            int k = 0;
+#pragma unroll
+            for (int a = 0; a < 4; ++a)
+#pragma unroll
+                for (int b = 0; b <= a; ++b, ++k) {
+                    f4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int p = 0; p < CT / 2; ++p) acc = multiply<SPLIT>(xr[b][p], xr[a][p], acc);
+                    *reinterpret_cast<f4 *>(part[wave][k][lane]) = acc;
+                }
+        }
+        __syncthreads();
+        for (int i = tid; i < 640; i += T) {
+            const int k = i >> 6, l = i & 63;
+            const int a = k >= 6 ? 3 : k >= 3 ? 2 : k >= 1 ? 1 : 0, b = k - a * (a + 1) / 2;
+            f4 v = *reinterpret_cast<const f4 *>(part[0][k][l]);
+            for (int w = 1; w < shares; ++w) v += *reinterpret_cast<const f4 *>(part[w][k][l]);
+            v = settled(v * f.gram);
+            const int row = a * 16 + (l & 15), col = b * 16 + (l >> 4) * 4;
+            const h4 hi = __builtin_convertvector(v, h4);
+            *reinterpret_cast<h4 *>(&as[0][row][col]) = hi;
+            h4 lo;
+            if constexpr (SPLIT) {
+                lo = __builtin_convertvector(v - __builtin_convertvector(hi, f4), h4);
+                *reinterpret_cast<h4 *>(&as[N - 1][row][col]) = lo;
+            }
+            if (a != b) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    as[0][col + r][row] = hi[r];
+                    if constexpr (SPLIT) as[N - 1][col + r][row] = lo[r];
+                }
+            }
+        }
+        __syncthreads();
+        auto fragment = [&](const _Float16(*m)[64][LD], int t, int h) {   // rows 16 t .. of A or B, K = 32 h ..
+            Op<SPLIT> q;
+#pragma unroll
+            for (int s = 0; s < N; ++s) {
+                const h4 x = *reinterpret_cast<const h4 *>(&m[s][t * 16 + n][h * 32 + g * 4]);
+                const h4 y = *reinterpret_cast<const h4 *>(&m[s][t * 16 + n][h * 32 + 16 + g * 4]);
+                q.v[s] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+            }
+            return q;
+        };
+        // B = a I + b A + c A A, two tiles to a wave
+#pragma unroll
+        for (int q = 0; q < 16 / kSmallWaves; ++q) {
+            const int a = (wave * (16 / kSmallWaves) + q) >> 2, b = (wave * (16 / kSmallWaves) + q) & 3;
+            f4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int h = 0; h < 2; ++h) v = multiply<SPLIT>(fragment(as, b, h), fragment(as, a, h), v);
+            const int row = a * 16 + n, col = b * 16 + g * 4;
+            f4 at = __builtin_convertvector(*reinterpret_cast<const h4 *>(&as[0][row][col]), f4);
+            if constexpr (SPLIT) at += __builtin_convertvector(*reinterpret_cast<const h4 *>(&as[N - 1][row][col]), f4);
+            v = v * f.poly + at * f.a;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (col + r == row) v[r] += f.diag;
+            v = settled(v);
+            const h4 hi = __builtin_convertvector(v, h4);
+            *reinterpret_cast<h4 *>(&bs[0][row][col]) = hi;
+            if constexpr (SPLIT) *reinterpret_cast<h4 *>(&bs[N - 1][row][col]) = __builtin_convertvector(v - __builtin_convertvector(hi, f4), h4);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) bf[t][h] = fragment(bs, t, h);
+    };
+    for (int step = 0; step + 1 < js.steps; ++step) {
+        const StepFactors f = js.step[step];
+        make_b(f);
+        // X <- B X in G's form, and turned.  (B carries the factor: the accumulators are X's next numbers as they are.)
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+            f4 y[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                y[t] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int h = 0; h < 2; ++h) y[t] = TALL ? multiply<SPLIT>(bf[t][h], xc[c][h], y[t]) : multiply<SPLIT>(xc[c][h], bf[t][h], y[t]);
+            }
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                if (TALL) xc[c][t >> 1].set(t & 1, y[t]);
+                else xr[t][c >> 1].set(c & 1, y[t]);
+            }
+            turn(c);
+            NT_STAY();
+        }
+    }
+    const StepFactors last = js.step[js.steps - 1];
+    make_b(last);
+    // O in the form whose four numbers lie in a row of G, through LDS, so that one short loop writes it
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < CT / 2; ++c)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int tile = (wave * (CT / 2) + c) * 16, row = TALL ? tile + n : t * 16 + n, col = (TALL ? t * 16 : tile) + g * 4;
+                f4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const Op<SPLIT> &x = xc[half * (CT / 2) + c][h];
+                    y = TALL ? multiply<SPLIT>(bf[t][h], x, y) : multiply<SPLIT>(x, bf[t][h], y);
+                }
+                *reinterpret_cast<f4 *>(&os[row][col]) = y * last.apply;
+            }
+        __syncthreads();
+        for (int i = tid; i < RO * (CO / 4); i += T) {
+            const int r = i / (CO / 4), c = i % (CO / 4) * 4;
+            // place in the long side: wave's tiles of this half
+            const int l = TALL ? r : c, at = (l / (CT * 8) * CT + half * (CT / 2)) * 16 + l % (CT * 8);
+            const int row = TALL ? at : r, col = TALL ? c : at;
+            if (row >= j.rows || col >= j.cols) continue;
+            f4 v = *reinterpret_cast<const f4 *>(&os[r][c]);
+            const int64_t to = row * j.ldo + col;
+            if (col + 4 <= j.cols) {
+                if (j.M) v = load4_as_float(j.out, j.o_dtype, to) * js.keep - v * j.lr;
+                store4_as(j.out, j.o_dtype, to, v);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 3; ++e) {
+                    if (col + e >= j.cols) break;
+                    store_as(j.out, j.o_dtype, to + e, j.M ? js.keep * load_as_float(j.out, j.o_dtype, to + e) - j.lr * v[e] : v[e]);
+                }
+            }
+        }
+    }
+}
+
+// a copy of G's rows (of `size` bytes a number), without gaps
+struct CopyJob {
+    const char *from;
+    char *to;
+    int64_t ld;
+    int rows, cols, size;
+};
+__global__ void __launch_bounds__(256) k_ortho_copy(CopyJob j) {
+    const int64_t n = int64_t(j.rows) * j.cols;
+    for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) {
+        const int64_t at = i / j.cols * j.ld + i % j.cols;
+        if (j.size == 4) reinterpret_cast<uint32_t *>(j.to)[i] = reinterpret_cast<const uint32_t *>(j.from)[at];
+        else reinterpret_cast<uint16_t *>(j.to)[i] = reinterpret_cast<const uint16_t *>(j.from)[at];
     }
 }
 
@@ -603,18 +955,79 @@ bool choose(Class &cl, int phase, Choice &best) {
 
 // The layout of a call in its workspace: | arrival counters | pieces of tiles | tables | the jobs' matrices |
 struct Layout {
-    size_t counts = 0, parts = 0, tables = 0, jobs = 0;   // bytes
+    size_t counts = 0, parts = 0, tables = 0, jobs = 0, copies = 0;   // bytes
     Class cls[2];
-    size_t all() const { return jobs ? counts + parts + tables + jobs : 0; }
+    std::vector<SmallJob> small[2][2][5];   // [class][tall][column tiles of a wave / 2]
+    std::vector<CopyJob> copied;
+    size_t all() const { return (jobs ? counts + parts + tables + jobs : 0) + copies; }
 };
+
+// column tiles that each of eight waves takes of a small matrix (an even number), or 0 where the matrix is not small
+int small_tiles(const Request &r) {
+    const bool split = is_split(r);
+    const int tiles = (std::max(r.rows, r.cols) + 15) / 16, each = (tiles + kSmallWaves - 1) / kSmallWaves;
+    return std::min(r.rows, r.cols) <= 64 && each <= kSmallTiles[split] ? (each + 1) / 2 * 2 : 0;
+}
+
+// Whether an output of the call shares memory with another job's G.  The products' path reads every G before it writes, but
+// a small matrix is read and written by one kernel: those G are copied first.
+bool crossed(const std::vector<Request> &rq) {
+    struct Span {
+        uintptr_t from, to;
+        size_t job;
+        bool out;
+    };
+    std::vector<Span> sp;
+    auto add = [&](const void *p, int64_t ld, const Request &r, size_t size, size_t job, bool out) {
+        if (p) sp.push_back({uintptr_t(p), uintptr_t(p) + (size_t(r.rows - 1) * ld + r.cols) * size, job, out});
+    };
+    for (size_t k = 0; k < rq.size(); ++k) {
+        const Request &r = rq[k];
+        if (!r.rows || !r.cols) continue;
+        add(r.G, r.ldg, r, type_size(r.g_dtype), k, false);
+        add(r.out, r.ldo, r, type_size(r.o_dtype), k, true);
+        add(r.M, r.ldm, r, 4, k, true);
+    }
+    std::sort(sp.begin(), sp.end(), [](const Span &a, const Span &b) { return a.from < b.from; });
+    // the furthest ends so far of either kind: the two furthest of different jobs
+    Span far[2][2] = {};
+    for (const Span &s : sp) {
+        for (const Span &f : far[!s.out])
+            if (f.to > s.from && f.job != s.job) return true;
+        Span *f = far[s.out];
+        if (s.to > f[0].to) {
+            if (f[0].job != s.job) f[1] = f[0];
+            f[0] = s;
+        } else if (s.to > f[1].to && f[0].job != s.job) {
+            f[1] = s;
+        }
+    }
+    return false;
+}
 
 size_t table_bytes(size_t n) { return cp_align_up(n * (sizeof(Job) + 2 * PHASES * sizeof(int)), 256); }
 
 int lay_out(cp_ctx *ctx, const std::vector<Request> &rq, double lr, Layout &lay) {
     lay.cls[0].split = false;
     lay.cls[1].split = true;
+    bool small = !cp_knob(CP_KNOB_NT_TILE);   // beside larger matrices, small ones cost next to nothing in the products' launches
+    for (const Request &r : rq) small &= !r.rows || !r.cols || small_tiles(r) > 0;
+    const bool copy = small && crossed(rq);
     for (const Request &r : rq) {
         if (!r.rows || !r.cols) continue;
+        if (small) {
+            const int ct = small_tiles(r);
+            SmallJob j = {r.G, r.M, r.out, r.ldg, r.ldm, r.ldo, r.rows, r.cols, r.g_dtype, r.o_dtype, float(lr * r.gamma)};
+            if (copy) {
+                const size_t size = type_size(r.g_dtype);
+                lay.copied.push_back({static_cast<const char *>(r.G), reinterpret_cast<char *>(lay.copies), r.ldg, r.rows, r.cols, int(size)});
+                j.G = reinterpret_cast<const void *>(lay.copies);   // offsets so far
+                j.ldg = r.cols;
+                lay.copies += cp_align_up(size_t(r.rows) * r.cols * size, 256);
+            }
+            lay.small[is_split(r)][r.rows > r.cols][ct / 2].push_back(j);
+            continue;
+        }
         Class &cl = lay.cls[is_split(r)];
         const size_t e = cl.split ? 4 : 2;
         const size_t mp = padded(std::min(r.rows, r.cols)), np = padded(std::max(r.rows, r.cols));
@@ -668,6 +1081,14 @@ int lay_out(cp_ctx *ctx, const std::vector<Request> &rq, double lr, Layout &lay)
 // the offsets become pointers into the workspace
 void place(Layout &lay, char *ws) {
     char *tables = ws + lay.counts + lay.parts, *jobs = tables + lay.tables;
+    if (!lay.copied.empty()) {
+        char *copies = jobs + lay.jobs;
+        for (CopyJob &c : lay.copied) c.to = copies + reinterpret_cast<size_t>(c.to);
+        for (auto &of : lay.small)
+            for (auto &way : of)
+                for (auto &list : way)
+                    for (SmallJob &j : list) j.G = copies + reinterpret_cast<size_t>(j.G);
+    }
     for (Class &cl : lay.cls) {
         const size_t n = cl.jobs.size();
         if (!n) continue;
@@ -692,6 +1113,12 @@ void place(Layout &lay, char *ws) {
     }
 }
 
+StepFactors step_factors(const Plan &pl, int k) {
+    const double sx = pl.sx[k], sa = pl.sa[k], sb = pl.sb[k];
+    return {float(sa / (sx * sx)), float(pl.coef[k][2] * sb / (sa * sa)), float(pl.coef[k][1] * sb / sa), float(pl.coef[k][0] * sb),
+            float((k + 1 < pl.steps ? pl.sx[k + 1] : 1.0) / (sb * sx))};
+}
+
 struct Call {
     hipStream_t st;
     const Layout &lay;
@@ -710,23 +1137,33 @@ void launch_product(const Call &call, const Table &t, const Choice &c, const Fac
 template <bool SPLIT>
 void launch_steps(const Call &call, const Class &cl, const Plan &pl, float keep) {
     for (int k = 0; k < pl.steps; ++k) {
-        const double a = pl.coef[k][0], b = pl.coef[k][1], c = pl.coef[k][2];
-        const double sx = pl.sx[k], sa = pl.sa[k], sb = pl.sb[k];
+        const StepFactors q = step_factors(pl, k);
         Factors f = {};
         f.xt = k & 1;
-        f.acc = float(sa / (sx * sx));
+        f.acc = q.gram;
         launch_product<GRAM, SPLIT>(call, cl.table, cl.gram, f);
-        f.acc = float(c * sb / (sa * sa));
-        f.a = float(b * sb / sa);
-        f.diag = float(a * sb);
+        f.acc = q.poly;
+        f.a = q.a;
+        f.diag = q.diag;
         launch_product<POLY, SPLIT>(call, cl.table, cl.poly, f);
-        if (k + 1 < pl.steps) {
-            f.acc = float(pl.sx[k + 1] / (sb * sx));
-            launch_product<APPLY, SPLIT>(call, cl.table, cl.apply, f);
-        } else {
-            f.acc = float(1.0 / (sb * sx));
-            f.keep = keep;
-            launch_product<LAST, SPLIT>(call, cl.table, cl.apply, f);
+        f.acc = q.apply;
+        f.keep = keep;
+        if (k + 1 < pl.steps) launch_product<APPLY, SPLIT>(call, cl.table, cl.apply, f);
+        else launch_product<LAST, SPLIT>(call, cl.table, cl.apply, f);
+    }
+}
+
+template <bool SPLIT, bool TALL>
+void launch_small(hipStream_t st, const std::vector<SmallJob> &jobs, SmallJobs &js, int ct) {
+    const int T = 64 * kSmallWaves;
+    for (size_t base = 0; base < jobs.size(); base += kSmallJobs) {
+        const int n = int(std::min<size_t>(kSmallJobs, jobs.size() - base));
+        std::copy(jobs.begin() + base, jobs.begin() + base + n, js.job);
+        if (ct == 1) k_ortho_small<SPLIT, 2, TALL><<<n, T, 0, st>>>(js);
+        else if (ct == 2) k_ortho_small<SPLIT, 4, TALL><<<n, T, 0, st>>>(js);
+        if constexpr (!SPLIT) {
+            if (ct == 3) k_ortho_small<SPLIT, 6, TALL><<<n, T, 0, st>>>(js);
+            else if (ct == 4) k_ortho_small<SPLIT, 8, TALL><<<n, T, 0, st>>>(js);
         }
     }
 }
@@ -735,14 +1172,17 @@ int run(cp_ctx *ctx, const std::vector<Request> &rq, const Plan &pl, double lr, 
         double eps, void *given, size_t given_bytes) {
     Layout lay;
     CP_TRY(lay_out(ctx, rq, lr, lay));
-    if (!lay.all()) return CP_OK;
     CP_HIP(ctx, hipSetDevice(ctx->device));
     char *ws = nullptr;
-    CP_TRY(cp_scratch(ctx, given, given_bytes, lay.all(), &ws));
-    place(lay, ws);
+    if (lay.all()) {
+        CP_TRY(cp_scratch(ctx, given, given_bytes, lay.all(), &ws));
+        place(lay, ws);
+    }
     const Call call = {ctx->stream, lay, ws};
     const float mu = float(momentum), keep = float(1.0 - lr * decay), sx = float(pl.sx[0]);
-    // every job's G is read before any output is written: an output may be another job's G
+    // every job's G is read (or copied) before any output is written: an output may be another job's G
+    for (const CopyJob &c : lay.copied)
+        k_ortho_copy<<<int(std::min<int64_t>(256, (int64_t(c.rows) * c.cols + 255) / 256)), 256, 0, call.st>>>(c);
     for (const Class &cl : lay.cls)
         for (size_t base = 0; base < cl.jobs.size(); base += kJobs) {
             Jobs js = {};
@@ -760,6 +1200,30 @@ int run(cp_ctx *ctx, const std::vector<Request> &rq, const Plan &pl, double lr, 
         if (cl.jobs.empty()) continue;
         if (cl.split) k_ortho_load<true><<<cl.loads, 256, 0, call.st>>>(cl.table, mu, nesterov, eps, sx);
         else k_ortho_load<false><<<cl.loads, 256, 0, call.st>>>(cl.table, mu, nesterov, eps, sx);
+    }
+    SmallJobs js = {};
+    js.eps = eps;
+    js.x_scale = pl.sx[0];
+    js.momentum = mu;
+    js.keep = keep;
+    js.nesterov = nesterov;
+    js.steps = pl.steps;
+    for (int k = 0; k < pl.steps; ++k) {
+        StepFactors q = step_factors(pl, k);
+        if (k + 1 < pl.steps) {   // B takes X from its scale to the next step's
+            q.poly *= q.apply;
+            q.a *= q.apply;
+            q.diag *= q.apply;
+            q.apply = 1.f;
+        }
+        js.step[k] = q;
+    }
+    for (int ct = 1; ct <= 4; ++ct) {
+        launch_small<false, false>(call.st, lay.small[0][0][ct], js, ct);
+        launch_small<false, true>(call.st, lay.small[0][1][ct], js, ct);
+        if (ct > 2) continue;
+        launch_small<true, false>(call.st, lay.small[1][0][ct], js, ct);
+        launch_small<true, true>(call.st, lay.small[1][1][ct], js, ct);
     }
     for (const Class &cl : lay.cls) {
         if (cl.jobs.empty()) continue;

@@ -165,7 +165,8 @@ def test_long_matrices(ctx, tile_shape, rows, cols, kind):
 @gpu
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
 def test_many_matrices_in_one_call(ctx, kind):
-    """More than one launch's table, of mixed sizes and types, against each on its own: equal bits."""
+    """More than one launch's table, of mixed sizes and types, against each on its own: equal bits, but where the short side is
+    at most 64: a call of such matrices alone forms them in one kernel, with other sums."""
     rs = np.random.RandomState(3)
     shapes = [(int(rs.randint(1, 150)), int(rs.randint(1, 200))) for _ in range(30)] + [(140, 400), (0, 5), (5, 0), (300, 150)]
     kinds = [kind if i % 5 else "f16" for i in range(len(shapes))]
@@ -178,7 +179,27 @@ def test_many_matrices_in_one_call(ctx, kind):
         one = Mat(ctx, np.zeros(s), k)
         ctx.orthogonalise(capi.OrthoJobs([(G.ptr, TYPES[k], s[0], s[1], one.ptr, TYPES[k])]))
         within(O.get(), *distance(G.get(), k), k)
-        assert np.array_equal(one.raw(), O.raw())
+        within(one.get(), *distance(G.get(), k), k)
+        assert min(s) <= 64 or np.array_equal(one.raw(), O.raw())
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_small_matrices_in_one_call(ctx, kind):
+    """More than one launch's records, both ways round, of every length that one kernel takes, against each on its own."""
+    rs = np.random.RandomState(13)
+    top = 512 if kind == "f32" else 1024
+    shapes = [(int(rs.randint(1, 65)), int(rs.randint(1, top + 1))) for _ in range(40)] + [(64, top), (1, 1), (64, 64), (33, 129)]
+    shapes += [(b, a) for a, b in shapes]
+    Gs = [Mat(ctx, gradient(rs, *s), kind) for s in shapes]
+    Os = [Mat(ctx, np.zeros(s), kind) for s in shapes]
+    T = TYPES[kind]
+    ctx.orthogonalise(capi.OrthoJobs([(G.ptr, T, s[0], s[1], O.ptr, T) for G, O, s in zip(Gs, Os, shapes)]))
+    for G, O, s in zip(Gs, Os, shapes):
+        within(O.get(), *distance(G.get(), kind), kind)
+        one = Mat(ctx, np.zeros(s), kind)
+        ctx.orthogonalise(capi.OrthoJobs([(G.ptr, T, s[0], s[1], one.ptr, T)]))
+        assert O.untouched() and np.array_equal(one.raw(), O.raw())
 
 
 @gpu
