@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(CFG::T) k_ortho_product(Table tab, Factors f, 
 // product with the unit matrix turns it, exactly, into the other, and nothing of X passes through LDS.  Only A and B do.
 constexpr int kSmallWaves = 8;
 constexpr int kSmallJobs = 24;
-constexpr int kSmallTiles[2] = {8, 4};   // column tiles of a wave at most: one fp16 a number, pairs
+constexpr int kSmallTiles[2] = {6, 4};   // column tiles of a wave at most: one fp16 a number, pairs
 
 struct SmallJob {
     const void *G;
@@ -479,26 +479,76 @@ __global__ void __launch_bounds__(64 * kSmallWaves) k_ortho_small(SmallJobs js) 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, g = lane >> 4;
 
-    // |U|, and the momentum
+    // U, eight neighbours to a unit, all of a thread's loads under way at once: whole units, then the rows' ends
+    constexpr int UNITS = R * (C / 8) / T, ENDS = (R + T - 1) / T;
+    static_assert(R * (C / 8) % T == 0, "");
+    float u[UNITS + ENDS][8];
+    auto place = [&](int k, int &r, int &c) {   // a unit's row and column; false: there is none
+        const int i = k * T + tid;
+        if (k < UNITS) {
+            r = i / (C / 8);
+            c = i % (C / 8) * 8;
+            return r < j.rows && c + 8 <= j.cols;
+        }
+        r = (k - UNITS) * T + tid;
+        c = j.cols & ~7;
+        return r < j.rows && c < j.cols;
+    };
+    auto load = [&](const void *p, int dtype, int64_t ld, float(&v)[UNITS + ENDS][8]) {
+        auto whole = [&](auto type) {
+            typedef decltype(type) V;   // eight numbers
+#pragma unroll
+            for (int k = 0; k < UNITS; ++k) {
+                int r, c;
+                const bool in = place(k, r, c);
+                V q = {};
+                if (in) __builtin_memcpy(&q, static_cast<const char *>(p) + (r * ld + c) * int(sizeof(V) / 8), sizeof(V));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[k][e] = float(q[e]);
+            }
+        };
+        typedef float f8 __attribute__((ext_vector_type(8)));
+        if (dtype == CP_F32) whole(f8());
+        else if (dtype == CP_BF16) whole(nt::b8());
+        else whole(h8());
+#pragma unroll
+        for (int k = UNITS; k < UNITS + ENDS; ++k) {
+            int r, c;
+            const bool in = place(k, r, c);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[k][e] = in && c + e < j.cols ? load_as_float(p, dtype, r * ld + c + e) : 0.f;
+        }
+    };
+    load(j.G, j.g_dtype, j.ldg, u);
     double sum = 0.0;
-    const int eights = (j.cols + 7) / 8;
-    for (int i = tid; i < j.rows * eights; i += T) {
-        const int r = i / eights, c = i % eights * 8;
-        float v[8];
-        load8(row_of(j.G, j.g_dtype, r * j.ldg), j.g_dtype, c, j.cols, v);
-        if (j.M) {
-            float *row = j.M + r * j.ldm, m[8];
-            load8(row, CP_F32, c, j.cols, m);
+    if (j.M) {
+        float m[UNITS + ENDS][8];
+        load(j.M, CP_F32, j.ldm, m);
+#pragma unroll
+        for (int k = 0; k < UNITS + ENDS; ++k) {
+            int r, c;
+            const bool in = place(k, r, c);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                m[e] = fmaf(js.momentum, m[e], v[e]);
-                v[e] = js.nesterov ? fmaf(js.momentum, m[e], v[e]) : m[e];
-                if (c + e < j.cols) row[c + e] = m[e];
+                m[k][e] = fmaf(js.momentum, m[k][e], u[k][e]);
+                u[k][e] = js.nesterov ? fmaf(js.momentum, m[k][e], u[k][e]) : m[k][e];
+            }
+            if (!in) continue;
+            float *row = j.M + r * j.ldm + c;
+            if (k < UNITS) {
+                *reinterpret_cast<nt::f4u *>(row) = f4{m[k][0], m[k][1], m[k][2], m[k][3]};
+                *reinterpret_cast<nt::f4u *>(row + 4) = f4{m[k][4], m[k][5], m[k][6], m[k][7]};
+            } else {
+#pragma unroll
+                for (int e = 0; e < 7; ++e)
+                    if (c + e < j.cols) row[e] = m[k][e];
             }
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum = fma(double(v[e]), double(v[e]), sum);
     }
+#pragma unroll
+    for (int k = 0; k < UNITS + ENDS; ++k)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = fma(double(u[k][e]), double(u[k][e]), sum);
     sum = wave_sum(sum);
     if (lane == 0) sums[wave] = sum;
     __syncthreads();
@@ -506,33 +556,25 @@ __global__ void __launch_bounds__(64 * kSmallWaves) k_ortho_small(SmallJobs js) 
 #pragma unroll
     for (int w = 0; w < kSmallWaves; ++w) sum += sums[w];
     const Inverse inv(sum, js.eps, js.x_scale);
-    // X into LDS, zero in the padding.  (A thread reads the M that it wrote.)
-    for (int i = tid; i < j.rows * eights; i += T) {
-        const int r = i / eights, c = i % eights * 8;
-        float v[8];
-        load8(row_of(j.G, j.g_dtype, r * j.ldg), j.g_dtype, c, j.cols, v);
-        if (j.M) {
-            float m[8];
-            load8(j.M + r * j.ldm, CP_F32, c, j.cols, m);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = js.nesterov ? fmaf(js.momentum, m[e], v[e]) : m[e];
-        }
+    // X into LDS, zero in the padding; then the rows' ends
+    auto put = [&](int k, int r, int c) {
         h8 hi, lo;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float x = inv.times(v[e]);
+            const float x = inv.times(u[k][e]);
             hi[e] = _Float16(x);
             lo[e] = _Float16(x - float(hi[e]));
         }
         *reinterpret_cast<h8 *>(&xs[0][r][c]) = hi;
         if constexpr (SPLIT) *reinterpret_cast<h8 *>(&xs[N - 1][r][c]) = lo;
-    }
-    for (int i = tid; i < R * (C / 8); i += T) {
-        const int r = i / (C / 8), c = i % (C / 8) * 8;
-        if (r < j.rows && c < j.cols) continue;
-        const h8 z = {};
+    };
 #pragma unroll
-        for (int s = 0; s < N; ++s) *reinterpret_cast<h8 *>(&xs[s][r][c]) = z;
+    for (int k = 0; k < UNITS; ++k) put(k, (k * T + tid) / (C / 8), (k * T + tid) % (C / 8) * 8);
+    __syncthreads();
+#pragma unroll
+    for (int k = UNITS; k < UNITS + ENDS; ++k) {
+        int r, c;
+        if (place(k, r, c)) put(k, r, c);
     }
     __syncthreads();
 
@@ -695,22 +737,32 @@ __global__ void __launch_bounds__(64 * kSmallWaves) k_ortho_small(SmallJobs js) 
                 *reinterpret_cast<f4 *>(&os[row][col]) = y * last.apply;
             }
         __syncthreads();
-        for (int i = tid; i < RO * (CO / 4); i += T) {
-            const int r = i / (CO / 4), c = i % (CO / 4) * 4;
-            // place in the long side: wave's tiles of this half
-            const int l = TALL ? r : c, at = (l / (CT * 8) * CT + half * (CT / 2)) * 16 + l % (CT * 8);
-            const int row = TALL ? at : r, col = TALL ? c : at;
-            if (row >= j.rows || col >= j.cols) continue;
-            f4 v = *reinterpret_cast<const f4 *>(&os[r][c]);
-            const int64_t to = row * j.ldo + col;
-            if (col + 4 <= j.cols) {
-                if (j.M) v = load4_as_float(j.out, j.o_dtype, to) * js.keep - v * j.lr;
-                store4_as(j.out, j.o_dtype, to, v);
-            } else {
+        constexpr int FOURS = RO * (CO / 4) / T, AT_ONCE = FOURS % 4 ? 2 : 4;   // of a thread; W's loads that are under way at once
+        static_assert(RO * (CO / 4) % T == 0 && FOURS % AT_ONCE == 0, "");
+        for (int i0 = 0; i0 < FOURS; i0 += AT_ONCE) {
+            f4 v[AT_ONCE], w[AT_ONCE];
+            int row[AT_ONCE], col[AT_ONCE];
 #pragma unroll
-                for (int e = 0; e < 3; ++e) {
-                    if (col + e >= j.cols) break;
-                    store_as(j.out, j.o_dtype, to + e, j.M ? js.keep * load_as_float(j.out, j.o_dtype, to + e) - j.lr * v[e] : v[e]);
+            for (int q = 0; q < AT_ONCE; ++q) {
+                const int i = (i0 + q) * T + tid, r = i / (CO / 4), c = i % (CO / 4) * 4;
+                // place in the long side: wave's tiles of this half
+                const int l = TALL ? r : c, at = (l / (CT * 8) * CT + half * (CT / 2)) * 16 + l % (CT * 8);
+                row[q] = TALL ? at : r;
+                col[q] = TALL ? c : at;
+                v[q] = *reinterpret_cast<const f4 *>(&os[r][c]);
+                if (j.M && row[q] < j.rows && col[q] + 4 <= j.cols) w[q] = load4_as_float(j.out, j.o_dtype, row[q] * j.ldo + col[q]);
+            }
+#pragma unroll
+            for (int q = 0; q < AT_ONCE; ++q) {
+                if (row[q] >= j.rows || col[q] >= j.cols) continue;
+                const int64_t to = row[q] * j.ldo + col[q];
+                if (col[q] + 4 <= j.cols) {
+                    store4_as(j.out, j.o_dtype, to, j.M ? w[q] * js.keep - v[q] * j.lr : v[q]);
+                } else {
+                    for (int e = 0; col[q] + e < j.cols; ++e) {
+                        const float o = e == 0 ? v[q][0] : e == 1 ? v[q][1] : v[q][2];
+                        store_as(j.out, j.o_dtype, to + e, j.M ? js.keep * load_as_float(j.out, j.o_dtype, to + e) - j.lr * o : o);
+                    }
                 }
             }
         }
@@ -957,7 +1009,7 @@ bool choose(Class &cl, int phase, Choice &best) {
 struct Layout {
     size_t counts = 0, parts = 0, tables = 0, jobs = 0, copies = 0;   // bytes
     Class cls[2];
-    std::vector<SmallJob> small[2][2][5];   // [class][tall][column tiles of a wave / 2]
+    std::vector<SmallJob> small[2][2][4];   // [class][tall][column tiles of a wave / 2]
     std::vector<CopyJob> copied;
     size_t all() const { return (jobs ? counts + parts + tables + jobs : 0) + copies; }
 };
@@ -1163,7 +1215,6 @@ void launch_small(hipStream_t st, const std::vector<SmallJob> &jobs, SmallJobs &
         else if (ct == 2) k_ortho_small<SPLIT, 4, TALL><<<n, T, 0, st>>>(js);
         if constexpr (!SPLIT) {
             if (ct == 3) k_ortho_small<SPLIT, 6, TALL><<<n, T, 0, st>>>(js);
-            else if (ct == 4) k_ortho_small<SPLIT, 8, TALL><<<n, T, 0, st>>>(js);
         }
     }
 }
@@ -1218,7 +1269,7 @@ int run(cp_ctx *ctx, const std::vector<Request> &rq, const Plan &pl, double lr, 
         }
         js.step[k] = q;
     }
-    for (int ct = 1; ct <= 4; ++ct) {
+    for (int ct = 1; ct <= 3; ++ct) {
         launch_small<false, false>(call.st, lay.small[0][0][ct], js, ct);
         launch_small<false, true>(call.st, lay.small[0][1][ct], js, ct);
         if (ct > 2) continue;
