@@ -632,7 +632,7 @@ class Context:
                 self._elsewhere(d, name)
         if bias is not None:
             if hasattr(bias, "stride"):
-                if bias.shape != (B.rows,) or _TORCH_CODES.get(bias.dtype) != CP_F32 or not bias.is_contiguous() \
+                if bias.shape != (B.rows,) or (_TORCH_CODES or _torch_codes()).get(bias.dtype) != CP_F32 or not bias.is_contiguous() \
                         or bias.get_device() != self.device:
                     raise ValueError("bias: a contiguous float32 tensor [%d] on device %d is needed" % (B.rows, self.device))
             bias = _ptr(bias)

@@ -435,6 +435,9 @@ __global__ void __launch_bounds__(512) k_matmul_blocks_rows(Product p) {
     }
 }
 
+bool wide_form(int c_dtype) { return c_dtype != CP_BF16; }   // what the 8-bit matrix instructions drop is below bfloat16's rounding only
+constexpr int64_t kMaxThreads = (int64_t(1) << 32) - 1;       // of a launch
+
 int check_product(cp_ctx *ctx, const cp_blocks *A, const cp_blocks *B, int c_dtype, int64_t ldc) {
     CP_TRY(check_blocks(ctx, A, "A"));
     CP_TRY(check_blocks(ctx, B, "B"));
@@ -442,7 +445,10 @@ int check_product(cp_ctx *ctx, const cp_blocks *A, const cp_blocks *B, int c_dty
         return cp_set_error(ctx, CP_ERR_ARG, "A has %lld columns, B %lld", (long long)A->cols, (long long)B->cols);
     if (c_dtype != CP_F32 && c_dtype != CP_BF16 && c_dtype != CP_F16) return cp_set_error(ctx, CP_ERR_ARG, "c_dtype %d", c_dtype);
     if (ldc < B->rows) return cp_set_error(ctx, CP_ERR_ARG, "ldc %lld < %lld", (long long)ldc, (long long)B->rows);
-    if (((A->rows + 63) / 64) * ((B->rows + 63) / 64) >= (int64_t(1) << 31)) return cp_set_error(ctx, CP_ERR_UNSUPPORTED, "C is too large");
+    const bool wide = wide_form(c_dtype);
+    const int64_t edge = wide ? nt::Medium::BM : nt::Large::BM;
+    if (((A->rows + edge - 1) / edge) * ((B->rows + edge - 1) / edge) * (wide ? nt::Medium::T : nt::Large::T) > kMaxThreads)
+        return cp_set_error(ctx, CP_ERR_UNSUPPORTED, "C is too large");
     return CP_OK;
 }
 
@@ -455,8 +461,6 @@ struct Form {
 constexpr int kMaxJoined = 16384;   // workgroups of a launch that joins pieces
 constexpr int kChip = 256;          // CUs that a split is planned for
 
-bool wide_form(int c_dtype) { return c_dtype != CP_BF16; }   // what the 8-bit matrix instructions drop is below bfloat16's rounding only
-
 Form form_of(const cp_blocks *A, const cp_blocks *B, int c_dtype) {
     // us per step and workgroup on a full chip / with at most one to a CU, beside the steps, and for a join; [wide][cfg]
     static const double full[2][3] = {{2.2, 1.1, 0.36}, {1e3, 1.75, 0.6}}, alone[2][3] = {{1.9, 0.85, 0.26}, {1e3, 1.4, 0.45}};
@@ -465,11 +469,12 @@ Form form_of(const cp_blocks *A, const cp_blocks *B, int c_dtype) {
     const bool wide = wide_form(c_dtype);
     Form best = {};
     const int forced = cp_knob(CP_KNOB_NT_TILE);
-    if (A->rows <= 32 && !forced) return {3, 0, 0, 1, 0, 0};
+    if (A->rows <= 32 && B->rows <= kMaxThreads / 512 * 16 && !forced) return {3, 0, 0, 1, 0, 0};
     double least = 1e300;
     for (int cfg = wide ? 1 : 0; cfg < 3; ++cfg) {
         if (forced && forced - 1 != cfg && !(wide && forced == 1 && cfg == 1)) continue;
         const int64_t edge = 256 >> cfg, tm = (A->rows + edge - 1) / edge, tn = (B->rows + edge - 1) / edge;
+        if (tm * tn * (cfg == 0 ? nt::Large::T : nt::Medium::T) > kMaxThreads) continue;   // (the largest tile's count is checked)
         for (int p = 1; p <= 32 && (p == 1 || (steps / p >= 4 && tm * tn * p <= kMaxJoined)); ++p) {
             const double groups = double(tm) * tn * p, rounds = std::ceil(groups / (cfg == 0 ? kChip : 2 * kChip));
             const double step = groups > kChip ? full[wide][cfg] : alone[wide][cfg];
@@ -532,7 +537,7 @@ extern "C" int cp_quant_blocks(cp_ctx *ctx, const void *x, int x_dtype, int64_t 
         CP_TRY(check_blocks(ctx, out_t, "out_t"));
         if (out_t->rows != cols || out_t->cols != rows) return cp_set_error(ctx, CP_ERR_ARG, "out_t is not [cols, rows]");
     }
-    if (out && out_t && out->q == out_t->q && out->q) return cp_set_error(ctx, CP_ERR_ARG, "out and out_t are the same memory");
+    if (out && out_t && out->q == out_t->q && out->q && rows && cols) return cp_set_error(ctx, CP_ERR_ARG, "out and out_t are the same memory");
     if (!rows || !cols) return CP_OK;
     const size_t size = x_dtype == CP_F64 ? 8 : x_dtype == CP_F32 ? 4 : 2;
     if (!x || uintptr_t(x) % size) return cp_set_error(ctx, CP_ERR_ARG, "x is null or misaligned");

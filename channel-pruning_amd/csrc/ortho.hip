@@ -845,19 +845,21 @@ int make_plan(cp_ctx *ctx, int steps, const double *coef, double eps, Plan &pl) 
 bool ortho_type(int d) { return d == CP_F32 || d == CP_BF16 || d == CP_F16; }
 size_t type_size(int d) { return d == CP_F32 ? 4 : 2; }
 
-// one matrix that is written, for the overlap check
-struct Written {
+// one matrix of the call, for the overlap check
+struct Region {
     uintptr_t at;
     int64_t ld, rows, cols;
     size_t size;
+    size_t job;
+    bool read;   // G
     uintptr_t end() const { return at + (size_t(rows - 1) * ld + cols) * size; }
 };
 
 // whether two matrices share an element: rows of one stride interleave as column ranges of one wider matrix do
-bool overlap(const Written &p, const Written &q) {
+bool overlap(const Region &p, const Region &q) {
     if (p.at >= q.end() || q.at >= p.end()) return false;
     if (p.ld != q.ld || p.size != q.size) return true;
-    const Written &lo = p.at <= q.at ? p : q, &hi = p.at <= q.at ? q : p;
+    const Region &lo = p.at <= q.at ? p : q, &hi = p.at <= q.at ? q : p;
     if ((hi.at - lo.at) % lo.size) return true;
     const int64_t d = int64_t((hi.at - lo.at) / lo.size) % lo.ld;   // hi's first column, counted from lo's
     return d < lo.cols || d + hi.cols > lo.ld;
@@ -872,8 +874,10 @@ struct Request {
     double gamma;
 };
 
-int check_requests(cp_ctx *ctx, const std::vector<Request> &rq, bool step) {
-    std::vector<Written> w;
+// `crossed`: whether an output shares memory with another job's G.  The products' path reads every G before it writes, but a
+// small matrix is read and written by one kernel: such a call's G are copied first.
+int check_requests(cp_ctx *ctx, const std::vector<Request> &rq, bool step, bool &crossed) {
+    std::vector<Region> w;
     for (size_t k = 0; k < rq.size(); ++k) {
         const Request &r = rq[k];
         if (r.rows < 0 || r.cols < 0 || r.rows > (1 << 20) || r.cols > (1 << 20))
@@ -888,18 +892,21 @@ int check_requests(cp_ctx *ctx, const std::vector<Request> &rq, bool step) {
             return cp_set_error(ctx, CP_ERR_ARG, "job %d: alignment", int(k));
         if (std::min(r.rows, r.cols) > 65536)
             return cp_set_error(ctx, CP_ERR_UNSUPPORTED, "job %d: shorter side above 65536", int(k));
-        w.push_back({uintptr_t(r.out), r.ldo, r.rows, r.cols, type_size(r.o_dtype)});
-        const Written g = {uintptr_t(r.G), r.ldg, r.rows, r.cols, type_size(r.g_dtype)};
-        if (step) {
-            w.push_back({uintptr_t(r.M), r.ldm, r.rows, r.cols, 4});
-            if (overlap(g, w.back()) || overlap(g, w[w.size() - 2]))
-                return cp_set_error(ctx, CP_ERR_ARG, "job %d: G overlaps M or W", int(k));
-        }
+        w.push_back({uintptr_t(r.G), r.ldg, r.rows, r.cols, type_size(r.g_dtype), k, true});
+        w.push_back({uintptr_t(r.out), r.ldo, r.rows, r.cols, type_size(r.o_dtype), k, false});
+        if (step) w.push_back({uintptr_t(r.M), r.ldm, r.rows, r.cols, 4, k, false});
     }
-    std::sort(w.begin(), w.end(), [](const Written &p, const Written &q) { return p.at < q.at; });
+    std::sort(w.begin(), w.end(), [](const Region &p, const Region &q) { return p.at < q.at; });
+    crossed = false;
     for (size_t i = 0; i < w.size(); ++i)
-        for (size_t k = i + 1; k < w.size() && w[k].at < w[i].end(); ++k)
-            if (overlap(w[i], w[k])) return cp_set_error(ctx, CP_ERR_ARG, "two outputs of the call overlap");
+        for (size_t k = i + 1; k < w.size() && w[k].at < w[i].end(); ++k) {
+            const Region &p = w[i], &q = w[k];
+            if ((p.read && q.read) || !overlap(p, q)) continue;
+            if (!p.read && !q.read) return cp_set_error(ctx, CP_ERR_ARG, "two outputs of the call overlap");
+            if (step)   // the momentum is written while other jobs' gradients are still to be read
+                return cp_set_error(ctx, CP_ERR_ARG, "job %d's G overlaps job %d's M or W", int((p.read ? p : q).job), int((p.read ? q : p).job));
+            crossed |= p.job != q.job;
+        }
     return CP_OK;
 }
 
@@ -928,11 +935,12 @@ struct Class {
     std::vector<Place> places;
     std::vector<int> sum_groups;   // workgroups of k_ortho_norm
     Table table;
-    int loads = 0;
+    int64_t loads = 0;
     Choice gram, poly, apply;
 };
 
 constexpr int kEdge[3] = {256, 128, 64};
+constexpr int64_t kMaxThreads = (int64_t(1) << 32) - 1;   // of a launch
 
 int64_t tiles_of(const Job &j, int phase, int edge) {
     const int64_t m = (j.mp + edge - 1) / edge, n = (j.np + edge - 1) / edge;
@@ -988,7 +996,7 @@ bool choose(Class &cl, int phase, Choice &best) {
             total += tiles * steps;
             longest = std::max(longest, (steps + p - 1) / p);
         }
-        if (groups >= (int64_t(1) << 31)) continue;
+        if (groups * (cfg == 0 ? nt::Large::T : nt::Medium::T) > kMaxThreads) continue;
         c.grid = int(groups);
         const double cost = cost_of(cfg, cl.split, groups, total, longest, c.joins);
         if (cost < least) {
@@ -1021,50 +1029,14 @@ int small_tiles(const Request &r) {
     return std::min(r.rows, r.cols) <= 64 && each <= kSmallTiles[split] ? (each + 1) / 2 * 2 : 0;
 }
 
-// Whether an output of the call shares memory with another job's G.  The products' path reads every G before it writes, but
-// a small matrix is read and written by one kernel: those G are copied first.
-bool crossed(const std::vector<Request> &rq) {
-    struct Span {
-        uintptr_t from, to;
-        size_t job;
-        bool out;
-    };
-    std::vector<Span> sp;
-    auto add = [&](const void *p, int64_t ld, const Request &r, size_t size, size_t job, bool out) {
-        if (p) sp.push_back({uintptr_t(p), uintptr_t(p) + (size_t(r.rows - 1) * ld + r.cols) * size, job, out});
-    };
-    for (size_t k = 0; k < rq.size(); ++k) {
-        const Request &r = rq[k];
-        if (!r.rows || !r.cols) continue;
-        add(r.G, r.ldg, r, type_size(r.g_dtype), k, false);
-        add(r.out, r.ldo, r, type_size(r.o_dtype), k, true);
-        add(r.M, r.ldm, r, 4, k, true);
-    }
-    std::sort(sp.begin(), sp.end(), [](const Span &a, const Span &b) { return a.from < b.from; });
-    // the furthest ends so far of either kind: the two furthest of different jobs
-    Span far[2][2] = {};
-    for (const Span &s : sp) {
-        for (const Span &f : far[!s.out])
-            if (f.to > s.from && f.job != s.job) return true;
-        Span *f = far[s.out];
-        if (s.to > f[0].to) {
-            if (f[0].job != s.job) f[1] = f[0];
-            f[0] = s;
-        } else if (s.to > f[1].to && f[0].job != s.job) {
-            f[1] = s;
-        }
-    }
-    return false;
-}
-
 size_t table_bytes(size_t n) { return cp_align_up(n * (sizeof(Job) + 2 * PHASES * sizeof(int)), 256); }
 
-int lay_out(cp_ctx *ctx, const std::vector<Request> &rq, double lr, Layout &lay) {
+int lay_out(cp_ctx *ctx, const std::vector<Request> &rq, bool crossed, double lr, Layout &lay) {
     lay.cls[0].split = false;
     lay.cls[1].split = true;
     bool small = !cp_knob(CP_KNOB_NT_TILE);   // beside larger matrices, small ones cost next to nothing in the products' launches
     for (const Request &r : rq) small &= !r.rows || !r.cols || small_tiles(r) > 0;
-    const bool copy = small && crossed(rq);
+    const bool copy = small && crossed;
     for (const Request &r : rq) {
         if (!r.rows || !r.cols) continue;
         if (small) {
@@ -1109,8 +1081,8 @@ int lay_out(cp_ctx *ctx, const std::vector<Request> &rq, double lr, Layout &lay)
         j.part = reinterpret_cast<double *>(lay.jobs);   // an offset so far
         lay.jobs += job_bytes(r);
         Place p = {};
-        p.first[LOAD] = cl.loads;
-        cl.loads += int((mp / 64) * (np / 64));
+        p.first[LOAD] = int(cl.loads);
+        cl.loads += int64_t(mp / 64) * int64_t(np / 64);
         for (int phase = GRAM; phase < PHASES; ++phase) p.pieces[phase] = int16_t(pieces_of(j, phase, cl.split));
         cl.sum_groups.push_back((j.sum_rows + j.rows_per - 1) / j.rows_per * j.chunks);
         cl.jobs.push_back(j);
@@ -1118,8 +1090,8 @@ int lay_out(cp_ctx *ctx, const std::vector<Request> &rq, double lr, Layout &lay)
     }
     for (Class &cl : lay.cls) {
         if (cl.jobs.empty()) continue;
-        if (!choose(cl, GRAM, cl.gram) || !choose(cl, POLY, cl.poly) || !choose(cl, APPLY, cl.apply))
-            return cp_set_error(ctx, CP_ERR_UNSUPPORTED, "a product of more than 2^31 tiles");
+        if (cl.loads * 256 > kMaxThreads || !choose(cl, GRAM, cl.gram) || !choose(cl, POLY, cl.poly) || !choose(cl, APPLY, cl.apply))
+            return cp_set_error(ctx, CP_ERR_UNSUPPORTED, "matrices of a call too large for one launch");
         for (const Choice *c : {&cl.gram, &cl.poly, &cl.apply})
             if (c->joins) {
                 lay.counts = std::max(lay.counts, cp_align_up(size_t(c->grid) * sizeof(int), 256));
@@ -1219,10 +1191,10 @@ void launch_small(hipStream_t st, const std::vector<SmallJob> &jobs, SmallJobs &
     }
 }
 
-int run(cp_ctx *ctx, const std::vector<Request> &rq, const Plan &pl, double lr, double momentum, int nesterov, double decay,
+int run(cp_ctx *ctx, const std::vector<Request> &rq, bool crossed, const Plan &pl, double lr, double momentum, int nesterov, double decay,
         double eps, void *given, size_t given_bytes) {
     Layout lay;
-    CP_TRY(lay_out(ctx, rq, lr, lay));
+    CP_TRY(lay_out(ctx, rq, crossed, lr, lay));
     CP_HIP(ctx, hipSetDevice(ctx->device));
     char *ws = nullptr;
     if (lay.all()) {
@@ -1249,8 +1221,8 @@ int run(cp_ctx *ctx, const std::vector<Request> &rq, const Plan &pl, double lr, 
         }
     for (const Class &cl : lay.cls) {
         if (cl.jobs.empty()) continue;
-        if (cl.split) k_ortho_load<true><<<cl.loads, 256, 0, call.st>>>(cl.table, mu, nesterov, eps, sx);
-        else k_ortho_load<false><<<cl.loads, 256, 0, call.st>>>(cl.table, mu, nesterov, eps, sx);
+        if (cl.split) k_ortho_load<true><<<uint32_t(cl.loads), 256, 0, call.st>>>(cl.table, mu, nesterov, eps, sx);
+        else k_ortho_load<false><<<uint32_t(cl.loads), 256, 0, call.st>>>(cl.table, mu, nesterov, eps, sx);
     }
     SmallJobs js = {};
     js.eps = eps;
@@ -1285,22 +1257,22 @@ int run(cp_ctx *ctx, const std::vector<Request> &rq, const Plan &pl, double lr, 
     return CP_OK;
 }
 
-int take_jobs(cp_ctx *ctx, int n, const cp_ortho_job *jobs, std::vector<Request> &rq) {
+int take_jobs(cp_ctx *ctx, int n, const cp_ortho_job *jobs, std::vector<Request> &rq, bool &crossed) {
     if (n < 0 || (n && !jobs)) return cp_set_error(ctx, CP_ERR_ARG, "jobs");
     for (int i = 0; i < n; ++i) {
         const cp_ortho_job &q = jobs[i];
         rq.push_back({q.G, nullptr, q.O, q.ldg, 0, q.ldo, q.rows, q.cols, q.g_dtype, q.o_dtype, 1.0});
     }
-    return check_requests(ctx, rq, false);
+    return check_requests(ctx, rq, false, crossed);
 }
 
-int take_jobs(cp_ctx *ctx, int n, const cp_ortho_step_job *jobs, std::vector<Request> &rq) {
+int take_jobs(cp_ctx *ctx, int n, const cp_ortho_step_job *jobs, std::vector<Request> &rq, bool &crossed) {
     if (n < 0 || (n && !jobs)) return cp_set_error(ctx, CP_ERR_ARG, "jobs");
     for (int i = 0; i < n; ++i) {
         const cp_ortho_step_job &q = jobs[i];
         rq.push_back({q.G, q.M, q.W, q.ldg, q.ldm, q.ldw, q.rows, q.cols, q.g_dtype, q.w_dtype, q.gamma});
     }
-    return check_requests(ctx, rq, true);
+    return check_requests(ctx, rq, true, crossed);
 }
 
 template <typename J>
@@ -1309,10 +1281,11 @@ int workspace(int n, const J *jobs, int steps, const double *coef, double eps, s
     try {
         Plan pl;
         std::vector<Request> rq;
+        bool crossed = false;
         CP_TRY(make_plan(nullptr, steps, coef, eps, pl));
-        CP_TRY(take_jobs(nullptr, n, jobs, rq));
+        CP_TRY(take_jobs(nullptr, n, jobs, rq, crossed));
         Layout lay;
-        CP_TRY(lay_out(nullptr, rq, 0.0, lay));
+        CP_TRY(lay_out(nullptr, rq, crossed, 0.0, lay));
         *bytes = lay.all();
         return CP_OK;
     } catch (...) {
@@ -1338,9 +1311,10 @@ extern "C" int cp_orthogonalise(cp_ctx *ctx, int n_jobs, const cp_ortho_job *job
     try {
         Plan pl;
         std::vector<Request> rq;
+        bool crossed = false;
         CP_TRY(make_plan(ctx, steps, coef, eps, pl));
-        CP_TRY(take_jobs(ctx, n_jobs, jobs, rq));
-        return run(ctx, rq, pl, 0.0, 0.0, 0, 0.0, eps, ws, ws_bytes);
+        CP_TRY(take_jobs(ctx, n_jobs, jobs, rq, crossed));
+        return run(ctx, rq, crossed, pl, 0.0, 0.0, 0, 0.0, eps, ws, ws_bytes);
     } catch (...) {
         return cp_set_error(ctx, CP_ERR_NOMEM, "host memory");
     }
@@ -1354,9 +1328,10 @@ extern "C" int cp_ortho_step(cp_ctx *ctx, int n_jobs, const cp_ortho_step_job *j
     try {
         Plan pl;
         std::vector<Request> rq;
+        bool crossed = false;
         CP_TRY(make_plan(ctx, steps, coef, eps, pl));
-        CP_TRY(take_jobs(ctx, n_jobs, jobs, rq));
-        return run(ctx, rq, pl, lr, momentum, nesterov != 0, weight_decay, eps, ws, ws_bytes);
+        CP_TRY(take_jobs(ctx, n_jobs, jobs, rq, crossed));
+        return run(ctx, rq, crossed, pl, lr, momentum, nesterov != 0, weight_decay, eps, ws, ws_bytes);
     } catch (...) {
         return cp_set_error(ctx, CP_ERR_NOMEM, "host memory");
     }

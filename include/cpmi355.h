@@ -269,17 +269,19 @@ int cp_blocks_check(const cp_blocks *m);
  *   amax  = the largest |x| of its finite values, at least 2^-100;   scale = amax / fmax,  inverse = fmax / amax
  *   (CP_QUANT_POW2: scale = the smallest power of two >= amax / fmax, inverse = 1 / scale);
  *   q = x * inverse cut to +-fmax, rounded to nearest even.  A NaN or an infinity becomes NaN.
- * F64 is rounded to float32 first.  Asynchronous on the context's stream, no workspace; can be captured. */
+ * F64 is rounded to float32 first.  x and the outputs must not overlap; rows up to 65535 * 128.  Asynchronous on the context's
+ * stream, no workspace; can be captured. */
 int cp_quant_blocks(cp_ctx *ctx, const void *x, int x_dtype, int64_t rows, int64_t cols, int64_t ldx, int flags,
                     const cp_blocks *out, const cp_blocks *out_t);
 /* C[i, j] = sum_k A[i, k] B[j, k] (+ bias[j]): A [M, K], B [N, K], C DEVICE [M, N] (c_dtype F32, BF16 or F16, row stride
  * ldc elements), bias DEVICE f32 [N] or NULL.  With x [M, c k^2], w [n, c k^2], dy [M, n]: y = x w^T, dx = dy (w^T)^T,
  * dw = dy^T (x^T)^T, the operands in the orientation that cp_quant_blocks' out / out_t give.  The products of a block are
  * summed in float32 and joined in float32 times both scales; one rounding to c_dtype at the end.  (For BF16 the matrix unit
- * adds products eight at a time, each cut below 2^-13 of the largest; F32 and F16 results keep all of float32.)  The order of the sums
- * depends on the shape alone.  C must not overlap the operands.  K = 0: C = bias (or 0).  Asynchronous.
+ * adds products eight at a time, each cut below 2^-13 of the largest; F32 and F16 results keep all of float32.)  The order of
+ * the sums depends on the shape alone.  C must not overlap the operands.  K = 0: C = bias (or 0).  Asynchronous.
  * ws: DEVICE scratch of cp_matmul_blocks_workspace() bytes, 256-byte aligned, or NULL: the context's own, which a call under
- * stream capture refuses (a graph outlives it) -- give every captured call a workspace that no concurrent replay uses. */
+ * stream capture refuses (a graph outlives it) -- give every captured call a workspace that no concurrent replay uses.
+ * Calls with the context's own scratch have to be ordered among each other, also after cp_ctx_set_stream. */
 int cp_matmul_blocks(cp_ctx *ctx, const cp_blocks *A, const cp_blocks *B, const float *bias, void *C, int c_dtype,
                      int64_t ldc, void *ws, size_t ws_bytes);
 /* The scratch that this product needs (0: none).  Checks the arguments like the call itself; needs no device. */
@@ -292,8 +294,11 @@ int cp_matmul_blocks_workspace(const cp_blocks *A, const cp_blocks *B, int c_dty
  * [0.7, 1.2].  G DEVICE [rows, cols] (g_dtype F32, BF16 or F16, row stride ldg), O DEVICE [rows, cols] (o_dtype likewise; may
  * be G itself).  All jobs of a call run in common launches.  Products are carried with 22 bits of mantissa where the result
  * is F32 or F16 and with 11 where it is BF16 (8), sums in float32, the norm in float64.  G = 0 gives O = 0; a NaN or an
- * infinity in G makes that job's O NaN.  coef must keep |x| <= 1 below 16 in every step (checked), steps 1..32.  Outputs of
- * a call must not overlap each other.  Asynchronous on the context's stream; ws as in cp_matmul_blocks. */
+ * infinity in G makes that job's O NaN.  coef must keep |x| <= 1 below 16 in every step (checked), steps 1..32.  The shorter
+ * side is at most 65536, the longer 2^20.  Outputs of a call must not overlap each other; an output may be another job's G (all
+ * are read first).  The order of a job's sums depends on its shape and types, and, where its short side is at most 64, on
+ * whether all of the call's matrices are small (such a call is one kernel, and needs no workspace unless an output is another
+ * job's G).  Asynchronous on the context's stream; ws as in cp_matmul_blocks. */
 typedef struct cp_ortho_job {
     const void *G;
     void *O;
@@ -306,8 +311,8 @@ int cp_orthogonalise_workspace(int n_jobs, const cp_ortho_job *jobs, int steps, 
 /* One optimiser step on a set of layers' weights:
  *   M <- momentum M + G;   U = nesterov ? G + momentum M : M;   W <- (1 - lr weight_decay) W - lr gamma O(U)
  * G DEVICE (g_dtype F32, BF16 or F16), M DEVICE f32 in/out, W DEVICE (w_dtype F32, BF16 or F16) in/out, all [rows, cols];
- * gamma: the job's factor on lr (sqrt(max(1, rows / cols)) is usual).  O(U) as above, carried for W's type.  G, M and W must
- * not overlap, nor the jobs' M and W each other.  Nothing is kept between calls but M. */
+ * gamma: the job's factor on lr (sqrt(max(1, rows / cols)) is usual).  O(U) as above, carried for W's type.  no M or W
+ * of a call may overlap another matrix of it (a G may serve several jobs).  Nothing is kept between calls but M. */
 typedef struct cp_ortho_step_job {
     const void *G;
     float *M;

@@ -1,5 +1,8 @@
 """Plain NumPy forms of the low-precision types (bfloat16, float16, the two 8-bit types), and device matrices in them.
 Test infrastructure: written from the formats' definitions, shares nothing with the library."""
+import contextlib
+import ctypes
+
 import numpy as np
 
 from cpmi355 import capi
@@ -169,3 +172,72 @@ class Held:
         ctx.sync()
         h.real = q * s.astype(np.float64).T.repeat(tile, 0)[:h.rows].repeat(128, 1)[:, :h.cols]
         return h
+
+
+def _hip(ctx, name, *args):
+    """A call of the HIP runtime that the library itself is linked to."""
+    fn = getattr(ctx.lib, name)
+    fn.restype = ctypes.c_int
+    rc = fn(*args)
+    if rc:
+        raise RuntimeError("%s: %d" % (name, rc))
+
+
+@contextlib.contextmanager
+def other_stream(ctx):
+    """ctx runs on a stream of the caller's."""
+    st = ctypes.c_void_p()
+    ctx.sync()
+    _hip(ctx, "hipStreamCreateWithFlags", ctypes.byref(st), ctypes.c_uint(1))
+    ctx.set_stream(st)
+    try:
+        yield st
+    finally:
+        ctx.sync()
+        ctx.set_stream(None)
+        _hip(ctx, "hipStreamDestroy", st)
+
+
+class Graph:
+    """What `calls` enqueues on ctx's stream (a caller's one), as a graph."""
+
+    def __init__(self, ctx, stream, calls):
+        self.ctx, self.stream, self.graph, self.run = ctx, stream, ctypes.c_void_p(), ctypes.c_void_p()
+        _hip(ctx, "hipStreamBeginCapture", stream, ctypes.c_int(2))          # relaxed
+        try:
+            calls()
+        finally:
+            _hip(ctx, "hipStreamEndCapture", stream, ctypes.byref(self.graph))
+        _hip(ctx, "hipGraphInstantiate", ctypes.byref(self.run), self.graph, None, None, ctypes.c_size_t(0))
+
+    def replay(self):
+        _hip(self.ctx, "hipGraphLaunch", self.run, self.stream)
+
+    def close(self):
+        self.ctx.sync()
+        _hip(self.ctx, "hipGraphExecDestroy", self.run)
+        _hip(self.ctx, "hipGraphDestroy", self.graph)
+
+
+class Far:
+    """A [rows, cols] matrix of a type whose rows lie `gap` elements apart: bytes past 2^32 from its start.  Only the rows and
+    the element before and behind each are filled."""
+
+    def __init__(self, ctx, a, kind, gap):
+        self.ctx, self.kind, self.ld, (self.rows, self.cols) = ctx, kind, gap, a.shape
+        assert (self.rows - 1) * gap * size(kind) > 1 << 32
+        self.buf = ctx.empty(((self.rows - 1) * gap + self.cols + 2) * size(kind))
+        self.ptr = self.buf.ptr + size(kind)
+        self.edge = np.full(1, 0x5a, dtype=np.uint8).repeat(size(kind)).view(np_type(kind))
+        for r in range(self.rows):
+            line = np.ascontiguousarray(np.concatenate([self.edge, to_bits(a[r], kind), self.edge]))
+            ctx._check(ctx.lib.cp_memcpy_h2d(ctx.h, self.buf.ptr + r * gap * size(kind), line.ctypes.data, line.nbytes), "cp_memcpy_h2d")
+
+    def get(self):
+        """The matrix; None if anything beside it was written."""
+        out = np.empty((self.rows, self.cols + 2), dtype=np_type(self.kind))
+        for r in range(self.rows):
+            self.ctx._check(self.ctx.lib.cp_memcpy_d2h(self.ctx.h, out[r].ctypes.data, self.buf.ptr + r * self.ld * size(self.kind),
+                                                       out[r].nbytes), "cp_memcpy_d2h")
+        ends = np.ascontiguousarray(out[:, [0, -1]]).view(np.uint8)
+        return from_bits(np.ascontiguousarray(out[:, 1:-1]), self.kind) if (ends == 0x5a).all() else None

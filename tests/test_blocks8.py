@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 from cpmi355 import capi
-from lowbits import FMT, HALF, TYPES, Held, Mat, from_bits, quant, table8, to_bits
+from lowbits import FMT, HALF, TYPES, Far, Graph, Held, Mat, from_bits, other_stream, quant, table8, to_bits
 
 gpu = pytest.mark.gpu
 
@@ -51,6 +51,9 @@ def test_products_are_checked():
     assert ask(m(5, 130), m(7, 130), ldc=6) == -1
     assert lib.cp_matmul_blocks_workspace(ctypes.byref(m(5, 130).c), None, 0, 7, ctypes.byref(n)) == -1
     assert lib.cp_matmul_blocks_workspace(ctypes.byref(m(5, 130).c), ctypes.byref(m(7, 130).c), 0, 7, None) == -1
+    far = capi.Blocks(256, 256, 1 << 30, 130, capi.CP_E4M3, 1)
+    assert ask(far, far, ldc=1 << 30) == -4                               # more tiles than a launch takes
+    assert ask(m(1, 130), far, ldc=1 << 30) == 0 and ask(far, m(1, 130)) == 0
     assert lib.cp_quant_blocks(None, None, 0, 1, 1, 1, 0, None, None) == -1
     assert lib.cp_matmul_blocks(None, None, None, None, None, 0, 0, None, 0) == -1
 
@@ -75,6 +78,12 @@ def test_calls_refuse(ctx):
     assert lib.cp_matmul_blocks(ctx.h, byref(o.b.c), byref(w.b.c), None, C.ptr, 0, 200, None, 0) == -1
     assert ctx.lib.cp_last_error(ctx.h)
     assert (o.codes() == 0x33).all() and C.untouched()
+    o.b.device = 1                                                        # a matrix on another device than the context's
+    with pytest.raises(ValueError):
+        ctx.quant_blocks(x.ptr, capi.CP_F32, o.b)
+    with pytest.raises(ValueError):
+        ctx.matmul_blocks(o.b, b.b, C.ptr, capi.CP_F32)
+    o.b.device = 0
     with pytest.raises(ValueError):
         ctx.quant_blocks(x.buf, capi.CP_F32)
     with pytest.raises(ValueError):
@@ -285,6 +294,120 @@ def test_scales_far_apart(ctx):
     assert (np.abs(C.get() - want) <= tol).all() and (C.get()[3] == 0).all()
 
 
+# ---- workspaces, streams, graphs -----------------------------------------------------------------------------------------
+
+
+@gpu
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+def test_product_in_a_workspace_of_any_contents(ctx, out):
+    rs = np.random.RandomState(4)
+    A, B = Held.of(ctx, values(rs, 129, 6000), "e4m3", 1), Held.of(ctx, rs.randn(65, 6000), "e4m3", 128)
+    C, D = Mat(ctx, np.zeros((129, 65)), out), Mat(ctx, np.zeros((129, 65)), out)
+    need = ctx.matmul_blocks_workspace(A.b, B.b, TYPES[out])
+    assert need > 0 and need % 256 == 0
+    ws = ctx.to_device(np.full(need + 256, 0xff, dtype=np.uint8))
+    ctx.matmul_blocks(A.b, B.b, C.ptr, TYPES[out])
+    args = (ctx.h, A.b.ref, B.b.ref, None, D.ptr, TYPES[out], 65)
+    assert ctx.lib.cp_matmul_blocks(*args, ws.ptr, need - 1) == -1 and ctx.lib.cp_matmul_blocks(*args, ws.ptr + 128, need) == -1
+    assert not D.get().any()
+    for _ in range(3):
+        assert ctx.lib.cp_matmul_blocks(*args, ws.ptr, need) == 0
+        assert np.array_equal(C.raw(), D.raw())
+        assert (ctx.to_host(ws, (need + 256,), np.uint8)[need:] == 0xff).all()
+
+
+@gpu
+def test_product_on_other_streams_and_contexts(ctx):
+    """Calls of two contexts under way at once, and calls on a caller's stream: the same bits."""
+    import cpmi355
+    rs = np.random.RandomState(5)
+    x, w = values(rs, 200, 5000), rs.randn(70, 5000)
+    A, B, C = Held.of(ctx, x, "e4m3", 1), Held.of(ctx, w, "e4m3", 128), Mat(ctx, np.zeros((200, 70)), "f32")
+    ctx.matmul_blocks(A.b, B.b, C.ptr, 0)
+    want = C.raw()
+    two = cpmi355.Context(0)
+    A2, B2 = Held.of(two, x, "e4m3", 1), Held.of(two, w, "e4m3", 128)
+    outs, outs2 = [Mat(ctx, np.zeros((200, 70)), "f32") for _ in range(8)], [Mat(two, np.zeros((200, 70)), "f32") for _ in range(8)]
+    for c, d in zip(outs, outs2):
+        ctx.matmul_blocks(A.b, B.b, c.ptr, 0)
+        two.matmul_blocks(A2.b, B2.b, d.ptr, 0)
+    for c in outs + outs2:
+        assert np.array_equal(c.raw(), want)
+    with other_stream(ctx):
+        for c in outs:
+            ctx.matmul_blocks(A.b, B.b, c.ptr, 0)
+        for c in outs:
+            assert np.array_equal(c.raw(), want)
+    del A2, B2, outs2, c, d
+    two.close()
+
+
+@gpu
+def test_products_in_graphs(ctx):
+    """Cast and products captured, two graphs with one workspace replayed in turn among eager calls, on new contents each time."""
+    rs = np.random.RandomState(6)
+    m, n, k = 129, 65, 6000
+    X, W = Mat(ctx, values(rs, m, k), "f32"), Mat(ctx, rs.randn(n, k), "f32")
+    A, B = Held(ctx, m, k, "e4m3", 1), Held(ctx, n, k, "e4m3", 128)
+    a, b = Held(ctx, m, k, "e4m3", 1), Held(ctx, n, k, "e4m3", 128)
+    C, D, E, F = (Mat(ctx, np.zeros((m, n)), t) for t in ("f32", "bf16", "f32", "bf16"))
+    ws = ctx.empty(max(ctx.matmul_blocks_workspace(A.b, B.b, t) for t in (capi.CP_F32, capi.CP_BF16)))
+
+    def calls(A, B, C, t, ws):
+        ctx.quant_blocks(X.ptr, capi.CP_F32, A.b)
+        ctx.quant_blocks(W.ptr, capi.CP_F32, B.b)
+        ctx.matmul_blocks(A.b, B.b, C.ptr, t, ws=ws)
+
+    with other_stream(ctx) as st:
+        def refused():
+            with pytest.raises(capi.CpError):
+                ctx.matmul_blocks(A.b, B.b, C.ptr, capi.CP_F32)
+            ctx.quant_blocks(X.ptr, capi.CP_F32, A.b)
+
+        graphs = [Graph(ctx, st, refused), Graph(ctx, st, lambda: calls(A, B, C, capi.CP_F32, ws)),
+                  Graph(ctx, st, lambda: calls(A, B, D, capi.CP_BF16, ws))]
+        for turn in range(4):
+            ctx.to_device(values(rs, X.n // k + 1, k).astype(np.float32).reshape(-1)[:X.n], X.buf)
+            graphs[1].replay()
+            graphs[2].replay()
+            calls(a, b, E, capi.CP_F32, None)
+            calls(a, b, F, capi.CP_BF16, None)
+            ctx.sync()
+            assert C.get().any() and np.array_equal(C.raw(), E.raw()) and np.array_equal(D.raw(), F.raw()), turn
+        for g in graphs:
+            g.close()
+
+
+@gpu
+def test_offsets_past_32_bits(ctx):
+    rs = np.random.RandomState(7)
+    x, w = values(rs, 140, 200), rs.randn(60, 200)
+    X, A, At, B = Far(ctx, x, "f32", 8000000), Held(ctx, 140, 200, "e4m3", 1), Held(ctx, 200, 140, "e4m3", 1), Held.of(ctx, w, "e4m3", 128)
+    ctx.quant_blocks(X.ptr, capi.CP_F32, A.b, At.b, ldx=X.ld)
+    ref = Held.of(ctx, x, "e4m3", 1)
+    assert np.array_equal(A.values(), ref.values()) and np.array_equal(A.scales(), ref.scales()) and A.around() and At.around()
+    assert np.array_equal(At.values(), quant(x.T, "e4m3", 1)[0])
+    for out, gap in (("f32", 8000000), ("bf16", 16000001)):
+        C = Far(ctx, np.zeros((140, 60)), out, gap)
+        ctx.matmul_blocks(A.b, B.b, C.ptr, TYPES[out], ldc=C.ld)
+        want, tol = product_bound(ref.real, B.real, out)
+        assert (np.abs(C.get() - want) <= tol).all()
+    # rows of 4 MB: the cast's output, read by a product
+    Y, C = Mat(ctx, values(rs, 1100, 130), "f32"), Mat(ctx, np.zeros((1100, 60)), "bf16")
+    wide = (1 << 22) - 128
+    q = capi.Blocks(ctx.empty(1100 * wide), ctx.empty(2 * 1100 * 4), 1100, 130, capi.CP_E4M3, 1, ld=wide)
+    ctx.quant_blocks(Y.ptr, capi.CP_F32, q)
+    w = Held.of(ctx, rs.randn(60, 130), "e4m3", 128)
+    near = Held.of(ctx, Y.get(), "e4m3", 1)
+    want, tol = product_bound(near.real, w.real, "bf16")
+    ctx.matmul_blocks(q, w.b, C.ptr, capi.CP_BF16)
+    assert (np.abs(C.get() - want) <= tol).all()
+    C = Mat(ctx, np.zeros((60, 1100)), "f32")
+    want, tol = product_bound(w.real, near.real, "f32")
+    ctx.matmul_blocks(w.b, q, C.ptr, capi.CP_F32)
+    assert (np.abs(C.get() - want) <= tol).all()
+
+
 # ---- a training pass -----------------------------------------------------------------------------------------------------
 
 
@@ -321,3 +444,50 @@ def test_training_pass(ctx, m, n, k):
     for got, a, b in ((dx, dy, w.T), (dw, dy.T, x.T)):
         slack = (2.0 ** -3 + 2.0 ** -4 + 2.0 ** -7) * (np.abs(a) @ np.abs(b).T) + 2.0 ** -7 * np.abs(a).max() * np.abs(b).max() * a.shape[1]
         assert (np.abs(got.get() - a @ b.T) <= slack).all()
+
+
+@gpu
+@pytest.mark.parametrize("m,n,k", [(400, 64, 576), (300, 130, 495)])
+def test_cast_products_and_update_of_a_layer(ctx, m, n, k):
+    """A layer's training step from the activations to its new weights: cast, y, dx, dw and the orthogonalised update of W, two
+    steps of it, eager and as a graph: the same bits, and W within the update's bounds of the formula's."""
+    import test_ortho
+    rs = np.random.RandomState(12)
+    w = from_bits(to_bits(0.05 * rs.randn(n, k), "f32"), "f32")
+    X = Mat(ctx, values(rs, m, k, "bf16"), "bf16")
+    dY = Mat(ctx, 1e-4 * rs.randn(m, n), "bf16")
+
+    class Layer:
+        def __init__(self):
+            self.W, self.M, self.dW = Mat(ctx, w, "f32"), Mat(ctx, np.zeros((n, k)), "f32"), Mat(ctx, np.zeros((n, k)), "f32")
+            self.y, self.dx = Mat(ctx, np.zeros((m, n)), "bf16"), Mat(ctx, np.zeros((m, k)), "bf16")
+            self.x, self.xt = Held(ctx, m, k, "e4m3", 1), Held(ctx, k, m, "e4m3", 1)
+            self.w, self.wt = Held(ctx, n, k, "e4m3", 128), Held(ctx, k, n, "e4m3", 128)
+            self.g, self.gt = Held(ctx, m, n, "e5m2", 1), Held(ctx, n, m, "e5m2", 1)
+            self.jobs = capi.OrthoStepJobs([(self.dW.ptr, 0, n, k, self.M.ptr, self.W.ptr, 0)])
+            self.products = [(self.x, self.w, self.y, capi.CP_BF16), (self.g, self.wt, self.dx, capi.CP_BF16), (self.gt, self.xt, self.dW, capi.CP_F32)]
+            need = [ctx.matmul_blocks_workspace(a.b, b.b, t) for a, b, _, t in self.products] + [ctx.ortho_workspace(self.jobs)]
+            self.ws = ctx.empty(max(need + [256]))
+
+        def step(self, ws=None):
+            ctx.quant_blocks(X.ptr, capi.CP_BF16, self.x.b, self.xt.b)
+            ctx.quant_blocks(self.W.ptr, capi.CP_F32, self.w.b, self.wt.b)
+            ctx.quant_blocks(dY.ptr, capi.CP_BF16, self.g.b, self.gt.b)
+            for a, b, c, t in self.products:
+                ctx.matmul_blocks(a.b, b.b, c.ptr, t, ws=ws)
+            ctx.ortho_step(self.jobs, 0.02, weight_decay=0.1, ws=ws)
+
+    with other_stream(ctx) as st:
+        eager, graphed = Layer(), Layer()
+        g = Graph(ctx, st, lambda: graphed.step(graphed.ws))
+        for _ in range(3):
+            M, W = eager.M.get(), eager.W.get()
+            eager.step()
+            g.replay()
+            ctx.sync()
+            for a, b in ((eager.y, graphed.y), (eager.dx, graphed.dx), (eager.dW, graphed.dW), (eager.M, graphed.M), (eager.W, graphed.W)):
+                assert np.array_equal(a.raw(), b.raw()) and a.untouched()
+            _, want, far = test_ortho.step(eager.dW.get(), M, W, "f32", 0.02, 0.95, True, 0.1, max(1, n / k) ** 0.5)
+            err = np.abs(eager.W.get() - want)
+            assert (err <= 12 * far + 5 * 2.0 ** -24 * (np.abs(W) + np.abs(want)) + 2.0 ** -25).all()
+        g.close()

@@ -14,7 +14,7 @@ import numpy as np
 import pytest
 
 from cpmi355 import capi
-from lowbits import HALF, TYPES, Mat, from_bits, to_bits
+from lowbits import Far, Graph, other_stream, HALF, TYPES, Mat, from_bits, to_bits
 
 gpu = pytest.mark.gpu
 COEF = (3.4445, -4.7750, 2.0315)
@@ -88,7 +88,10 @@ def refuses(make, jobs, **kw):
 
 def test_jobs_are_checked():
     O = capi.OrthoJobs
-    assert capi.ortho_workspace(O([job()])) > 0 and capi.ortho_workspace(O([])) == 0
+    big = dict(rows=100, cols=900, O=1 << 20)
+    assert capi.ortho_workspace(O([job(**big)])) > 0 and capi.ortho_workspace(O([])) == 0
+    assert capi.ortho_workspace(O([job()])) == 0                          # a small matrix stays in registers
+    assert capi.ortho_workspace(O([job(), job(G=16384, O=4096)])) > 0     # one's output is the other's input: copied first
     assert capi.ortho_workspace(O([job(0, 6), job(4, 0)])) == 0
     for bad in (job(rows=-1), job(gd=capi.CP_F64), job(od=capi.CP_E4M3), job(ldg=5), job(ldo=5), job(G=None), job(O=None),
                 job(G=4098), job(O=8193, od=capi.CP_BF16), job(rows=1 << 21), job(rows=70000, cols=70000)):
@@ -103,7 +106,7 @@ def test_jobs_are_checked():
                dict(coef=(3.4445, 4.7750, 2.0315))):
         refuses(O, [job()], **kw)
     for kw in (dict(steps=32), dict(coef=(1.5, -0.5, 0.0)), dict(coef=(1.875, -1.25, 0.375)), dict(coef=[(3, -3, 1)] * 5)):
-        assert capi.ortho_workspace(O([job()]), **kw) > 0
+        assert capi.ortho_workspace(O([job(**big)]), **kw) > 0
     lib = capi.load()
     assert lib.cp_orthogonalise_workspace(1, None, 5, None, 0.0, ctypes.byref(ctypes.c_size_t())) == -1
     assert lib.cp_orthogonalise_workspace(-1, None, 5, None, 0.0, ctypes.byref(ctypes.c_size_t())) == -1
@@ -114,12 +117,16 @@ def test_jobs_are_checked():
 
 def test_step_jobs_are_checked():
     S = capi.OrthoStepJobs
-    assert capi.ortho_workspace(S([step_job()])) > 0
+    assert capi.ortho_workspace(S([step_job()])) == 0 and capi.ortho_workspace(S([step_job(100, 900, M=1 << 20, W=1 << 21)])) > 0
     for bad in (step_job(M=None), step_job(W=None), step_job(M=8194), step_job(wd=capi.CP_F64), step_job(gamma=np.inf), step_job(ldm=5),
                 step_job(M=4096), step_job(W=4096), step_job(W=8192), step_job(G=8192 + 8)):
         refuses(S, [bad])
     refuses(S, [step_job(), step_job(M=32768)])
     refuses(S, [step_job(), step_job(W=32768)])
+    refuses(S, [step_job(), step_job(G=8192, M=32768, W=65536)])          # its gradient is the first job's momentum
+    refuses(S, [step_job(), step_job(G=16384 + 92, M=32768, W=65536)])    # or ends the first job's weights
+    capi.ortho_workspace(S([step_job(), step_job(G=16384 + 96, M=32768, W=65536)]))
+    refuses(S, [step_job(65536, 1 << 20, G=1 << 40, M=1 << 42, W=1 << 44)] * 1 + [step_job(65536, 1 << 20, G=1 << 40, M=1 << 46, W=1 << 48)])
     capi.ortho_workspace(S([step_job(), step_job(M=32768, W=65536)]))     # one gradient, two layers
     assert capi.OrthoStepJobs([(0, 0, 8, 2, 0, 0, 0)]).c[0].gamma == 2.0 and capi.OrthoStepJobs([(0, 0, 2, 8, 0, 0, 0)]).c[0].gamma == 1.0
 
@@ -296,6 +303,121 @@ def test_repeats_its_bits_on_any_workspace(ctx):
     lib = ctx.lib
     assert lib.cp_orthogonalise(ctx.h, 1, jp.c, 5, None, 0.0, ws.ptr, need - 1) == -1
     assert lib.cp_orthogonalise(ctx.h, 1, jp.c, 5, None, 0.0, ws.ptr + 128, need) == -1
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,cols", [(40, 300), (150, 2500)])
+def test_graphs_streams_and_contexts(ctx, kind, rows, cols):
+    """A small matrix and one whose products are cut along k: captured and replayed on new contents, two graphs on one workspace,
+    two contexts at once, a caller's stream; the bits are the eager call's."""
+    import cpmi355
+    rs = np.random.RandomState(14)
+    T = TYPES[kind]
+    G, M, W, O, P, Q = (Mat(ctx, gradient(rs, rows, cols), kind if i % 3 else "f32") for i in (1, 0, 2, 1, 1, 1))
+    M2, W2 = Mat(ctx, M.get(), "f32"), Mat(ctx, W.get(), kind)
+    jo, jp = (capi.OrthoJobs([(G.ptr, T, rows, cols, o.ptr, T)]) for o in (O, P))
+    jw, jw2 = (capi.OrthoStepJobs([(G.ptr, T, rows, cols, m.ptr, w.ptr, T)]) for m, w in ((M, W), (M2, W2)))
+    ws = ctx.empty(max(ctx.ortho_workspace(jp), ctx.ortho_workspace(jw2), 256))
+    ctx.orthogonalise(jo)
+    first = O.raw()
+    with other_stream(ctx) as st:
+        ctx.orthogonalise(jp)
+        assert np.array_equal(P.raw(), first)
+
+        def refused():
+            if ctx.ortho_workspace(jp):
+                with pytest.raises(capi.CpError):
+                    ctx.orthogonalise(jp)
+            ctx.orthogonalise(capi.OrthoJobs([(G.ptr, T, 1, 1, Q.ptr, T)]))
+
+        graphs = [Graph(ctx, st, refused), Graph(ctx, st, lambda: ctx.orthogonalise(jp, ws=ws)),
+                  Graph(ctx, st, lambda: ctx.ortho_step(jw2, 0.05, weight_decay=0.1, ws=ws))]
+        for turn in range(4):
+            other = Mat(ctx, gradient(rs, rows, cols), kind)
+            ctx.to_device(other.before, G.buf)
+            graphs[1].replay()
+            graphs[2].replay()
+            ctx.orthogonalise(jo)
+            ctx.ortho_step(jw, 0.05, weight_decay=0.1)
+            ctx.sync()
+            assert not np.array_equal(O.raw(), first)
+            for a, b in ((O, P), (M, M2), (W, W2)):
+                assert np.array_equal(a.raw(), b.raw()), turn
+        for g in graphs:
+            g.close()
+    two = cpmi355.Context(0)
+    H = Mat(two, G.get(), kind)
+    outs, outs2 = [Mat(ctx, np.zeros((rows, cols)), kind) for _ in range(5)], [Mat(two, np.zeros((rows, cols)), kind) for _ in range(5)]
+    for a, b in zip(outs, outs2):
+        ctx.orthogonalise(capi.OrthoJobs([(G.ptr, T, rows, cols, a.ptr, T)]))
+        two.orthogonalise(capi.OrthoJobs([(H.ptr, T, rows, cols, b.ptr, T)]))
+    for a in outs + outs2:
+        assert np.array_equal(a.get(), O.get())
+    del H, outs2, a, b
+    two.close()
+    jo.device = 1
+    with pytest.raises(ValueError):
+        ctx.orthogonalise(jo)
+
+
+@gpu
+@pytest.mark.parametrize("rows,cols", [(60, 90), (90, 60), (130, 150), (150, 130)])
+def test_rows_far_apart(ctx, rows, cols):
+    rs = np.random.RandomState(15)
+    gap = ((1 << 30) // rows + 1) * 5 // 4
+    G, M, W = (Far(ctx, gradient(rs, rows, cols), t, g) for t, g in (("bf16", 2 * gap), ("f32", gap), ("bf16", 2 * gap + 1)))
+    O = Far(ctx, np.zeros((rows, cols)), "f32", gap)
+    g, m, w = G.get(), M.get(), W.get()
+    ctx.orthogonalise(capi.OrthoJobs([(G.ptr, TYPES["bf16"], rows, cols, O.ptr, 0, G.ld, O.ld)]))
+    within(O.get(), *distance(g, "f32"), "f32")
+    ctx.ortho_step(capi.OrthoStepJobs([(G.ptr, TYPES["bf16"], rows, cols, M.ptr, W.ptr, TYPES["bf16"], 1.0, G.ld, M.ld, W.ld)]), 0.02)
+    m2, w2, far = step(g, m, w, "bf16", 0.02, 0.95, True, 0.0, 1.0)
+    assert (np.abs(M.get() - m2) <= 2.0 ** -24 * (np.abs(m2) + np.abs(m)) + 1e-30).all()
+    slack = 4 * 2.0 ** -24 * (np.abs(w) + np.abs(w2)) + HALF["bf16"] * np.abs(w2) + 2.0 ** -25
+    assert (np.abs(W.get() - w2) <= 12 * far + slack).all()
+    assert np.array_equal(G.get(), g)
+
+
+@gpu
+@pytest.mark.parametrize("tall", [False, True])
+def test_matrix_of_more_than_2_31_numbers(ctx, tall):
+    """G has one 1 in each of 2100 rows (or columns), far apart: X stays of that form, and its one number x follows
+    x <- round(B x), B = round(a + b A + c A^2), A = round(x^2), each rounding off by at most 2^-11 of the value (the kernel's
+    numbers have 11 bits), the float32 arithmetic by far less (2^-22 is taken)."""
+    m, n, at = 2100, 1 << 20, 499
+    G, O = ctx.empty(2 * m * n), ctx.empty(2 * m * n)
+    for b, v in ((G, 0), (O, 0xff)):
+        ctx._check(ctx.lib.cp_memset(ctx.h, b.ptr, v, 2 * m * n), "cp_memset")
+    place = [(i * at, i) if tall else (i, i * at) for i in range(m)]
+    one = to_bits(np.ones(1), "bf16")
+    width = m if tall else n
+    for r, c in place:
+        ctx._check(ctx.lib.cp_memcpy_h2d(ctx.h, G.ptr + 2 * (r * width + c), one.ctypes.data, 2), "cp_memcpy_h2d")
+    shape = (n, m) if tall else (m, n)
+    ctx.orthogonalise(capi.OrthoJobs([(G, capi.CP_BF16, shape[0], shape[1], O, capi.CP_BF16)]))
+    G.free()
+    a, b, c = 3.4445, -4.7750, 2.0315
+    e, small = 2.0 ** -11, 2.0 ** -22
+    x, err = 1 / np.sqrt(m), e                                            # err: of x, relative
+    for _ in range(5):
+        A, ea = x * x, 2 * err + e + small
+        B = a + b * A + c * A * A
+        eb = abs((b * A + 2 * c * A * A) / B) * ea * 1.01 + e + small
+        x, err = B * x, err + eb + e + small
+    for i in (0, 1, 63, 64, 1000, 2047, 2048, 2099):
+        r, col = place[i]
+        row = np.empty(width, dtype=np.uint16)
+        ctx._check(ctx.lib.cp_memcpy_d2h(ctx.h, row.ctypes.data, O.ptr + 2 * r * width, 2 * width), "cp_memcpy_d2h")
+        row = from_bits(row, "bf16")
+        assert abs(row[col] - x) <= x * (err * 1.01 + 2.0 ** -8), (i, row[col], x)
+        row[col] = 0
+        assert not row.any()
+    if tall:   # the last row, without a 1
+        end = np.empty(m, dtype=np.uint16)
+        ctx._check(ctx.lib.cp_memcpy_d2h(ctx.h, end.ctypes.data, O.ptr + 2 * (n - 1) * m, 2 * m), "cp_memcpy_d2h")
+        assert not from_bits(end, "bf16").any()
+    O.free()
 
 
 # ---- the step --------------------------------------------------------------------------------------------------------------
