@@ -279,28 +279,54 @@ __device__ __forceinline__ void store1(const Product &p, int64_t i, int j, float
     else static_cast<_Float16 *>(p.c)[at] = _Float16(v);
 }
 
+__device__ __forceinline__ void store8(const Product &p, int64_t i, int j, const float (&v)[8]) {
+    const int64_t at = i * p.ldc + j;
+    if (p.c_dtype == CP_F32) {
+        nt::f4u *to = reinterpret_cast<nt::f4u *>(static_cast<float *>(p.c) + at);
+        to[0] = f4{v[0], v[1], v[2], v[3]};
+        to[1] = f4{v[4], v[5], v[6], v[7]};
+    } else if (p.c_dtype == CP_BF16) {
+        nt::b8 q;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[e] = __bf16(v[e]);
+        *reinterpret_cast<nt::b8u *>(static_cast<__bf16 *>(p.c) + at) = q;
+    } else {
+        nt::h8 q;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[e] = _Float16(v[e]);
+        *reinterpret_cast<nt::h8u *>(static_cast<_Float16 *>(p.c) + at) = q;
+    }
+}
+
 // A wave's part of C [16 WI rows from i0, 16 WJ columns from j0]
 template <int WI, int WJ>
-__device__ __forceinline__ void write_c(const Product &p, const f4 (&acc)[WI][WJ], int i0, int j0, int lane) {
-    f4 bias[WJ];
+__device__ __forceinline__ void write_c(const Product &p, const f4 (&acc)[WI][WJ], int i0, int j0, const nt::Patch<WI, WJ> &patch) {
+    typedef nt::Patch<WI, WJ> Patch;
+    float bias[8];   // a lane's columns are the same in all of its groups
+    const int mine = j0 + patch.lane % (Patch::COLS / 8) * 8;
 #pragma unroll
-    for (int wj = 0; wj < WJ; ++wj) {
-        const int j = j0 + wj * 16 + (lane >> 4) * 4;
+    for (int e = 0; e < 8; ++e) bias[e] = p.bias && mine + e < p.N ? p.bias[mine + e] : 0.f;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) bias[wj][r] = p.bias && j + r < p.N ? p.bias[j + r] : 0.f;
-    }
+    for (int pass = 0; pass < Patch::PASSES; ++pass) {
+        if (i0 + pass * Patch::ROWS >= p.M) break;
+        patch.put(acc, pass, 1.f);
 #pragma unroll
-    for (int wi = 0; wi < WI; ++wi) {
-        const int i = i0 + wi * 16 + (lane & 15);
-        if (i >= p.M) continue;
+        for (int u = 0; u < Patch::EIGHTS; ++u) {
+            int i, j;
+            float v[8];
+            patch.of_row(u, i, j, v);
+            i += i0 + pass * Patch::ROWS;
+            j += j0;
+            if (i >= p.M) continue;
 #pragma unroll
-        for (int wj = 0; wj < WJ; ++wj) {
-            const int j = j0 + wj * 16 + (lane >> 4) * 4;
-            const f4 v = acc[wi][wj] + bias[wj];
-            if (j + 4 <= p.N) store4(p, i, j, v);
-            else
-                for (int r = 0; r < 3; ++r)
-                    if (j + r < p.N) store1(p, i, j + r, v[r]);
+            for (int e = 0; e < 8; ++e) v[e] += bias[e];
+            if (j + 8 <= p.N) {
+                store8(p, i, j, v);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 7; ++e)
+                    if (j + e < p.N) store1(p, i, j + e, v[e]);
+            }
         }
     }
 }
@@ -356,7 +382,7 @@ __global__ void __launch_bounds__(CFG::T) k_matmul_blocks(Product p) {
             nt::products8<WI, WJ, FA, FB, COMMON, WIDE>(s + ra * 128, s + (BM + rb) * 128, sc + ra, sc + BM + rb, lane, acc, between);
         });
     if (p.pieces > 1 && !nt::join<T>(acc, piece, p.pieces, p.parts + int64_t(tile) * (BM * BN), tiles, p.counts + tile, &flag, tid)) return;
-    write_c<WI, WJ>(p, acc, i0 + ra, j0 + rb, lane);
+    write_c<WI, WJ>(p, acc, i0 + ra, j0 + rb, nt::Patch<WI, WJ>::template of<CFG>(st, wave, lane));
 }
 
 // Few rows of A: bound by reading B once.  A workgroup takes sixteen rows of B and its eight waves an eighth of k each, straight

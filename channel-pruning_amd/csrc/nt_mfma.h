@@ -42,6 +42,17 @@ typedef h8 h8u __attribute__((aligned(2)));
 typedef b4 b4u __attribute__((aligned(2)));
 typedef b8 b8u __attribute__((aligned(2)));
 
+// Access through a pointer that was itself read from memory: for all that the compiler knows it could point into LDS, and such
+// an access would count, and be waited for, as one of LDS too.
+template <class V>
+__device__ __forceinline__ V take_from(const void *p) {
+    return *(const __attribute__((address_space(1))) V *)p;
+}
+template <class V>
+__device__ __forceinline__ void put_to(void *p, V v) {
+    *(__attribute__((address_space(1))) V *)p = v;
+}
+
 __device__ __forceinline__ void load_lds16(const char *g, char *l) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)g,
                                      (__attribute__((address_space(3))) void *)l, 16, 0, 0);
@@ -339,6 +350,63 @@ __device__ __forceinline__ bool join(f4 (&acc)[WI][WJ], int piece, int n, float 
     }
     return true;
 }
+
+// ---- results ---------------------------------------------------------------------------------------------------------------
+// A lane's accumulators are four numbers of one row: written from there, a row gets 32 or 64 bytes at a time, which costs twice
+// what whole lines cost.  So a wave passes its part of the tile through the LDS that the stages have left (16 KB a wave, its
+// own: no barrier), up to 64 x 64 float32 at a time, and reads it back as eight neighbours of a row or of a column.  The
+// 16-byte chunks of row r lie at chunk ^ key(r), so that writes and both kinds of reads hit all banks evenly.
+template <int WI, int WJ>
+struct Patch {
+    static constexpr int COLS = WJ * 16, ROWS = WI < 4 ? WI * 16 : 64, PASSES = WI * 16 / ROWS;
+    static constexpr int EIGHTS = ROWS * COLS / 512;   // groups of eight numbers to a lane
+    static_assert(ROWS * COLS * 4 <= 16384, "");
+    char *lds;
+    int lane;
+    template <class CFG>
+    __device__ __forceinline__ static Patch of(char *const (&st)[8], int wave, int lane) {
+        constexpr int EACH = CFG::NWM * CFG::NWN / CFG::STAGES;
+        static_assert(CFG::STAGE >= EACH * 16384, "");
+        typedef __attribute__((address_space(3))) char *Lds;
+        uint32_t from = 0;
+#pragma unroll
+        for (int k = 0; k < CFG::STAGES; ++k) {
+            uint32_t s = uint32_t(uintptr_t(Lds(st[k])));
+            asm("" : "+s"(s));   // (the compiler would look these up in a table, which it cannot place)
+            from = wave / EACH == k ? s : from;
+        }
+        return {(char *)(Lds(uintptr_t(from + wave % EACH * 16384))), lane};
+    }
+    __device__ __forceinline__ static void order() {   // a wave's LDS accesses run in order: only the compiler has to be told
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+    __device__ __forceinline__ char *at(int r, int chunk) const { return lds + r * COLS * 4 + ((chunk ^ ((r ^ (r >> 3)) & (COLS / 4 - 1))) << 4); }
+    // rows ROWS * pass .. of the wave's part, times a factor
+    __device__ __forceinline__ void put(const f4 (&acc)[WI][WJ], int pass, float factor) const {
+        order();
+#pragma unroll
+        for (int i = 0; i < ROWS / 16; ++i)
+#pragma unroll
+            for (int j = 0; j < WJ; ++j)
+                *reinterpret_cast<f4 *>(at(i * 16 + (lane & 15), j * 4 + (lane >> 4))) = acc[pass * (ROWS / 16) + i][j] * factor;
+        order();
+    }
+    // group u: eight numbers of row r from column c, or of column c from row r
+    __device__ __forceinline__ void of_row(int u, int &r, int &c, float (&v)[8]) const {
+        r = (u * 64 + lane) / (COLS / 8);
+        c = (u * 64 + lane) % (COLS / 8) * 8;
+        const f4 a = *reinterpret_cast<const f4 *>(at(r, c / 4)), b = *reinterpret_cast<const f4 *>(at(r, c / 4 + 1));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = a[e], v[e + 4] = b[e];
+    }
+    __device__ __forceinline__ void of_column(int u, int &r, int &c, float (&v)[8]) const {
+        c = (u * 64 + lane) / (ROWS / 8);
+        r = (u * 64 + lane) % (ROWS / 8) * 8;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = *reinterpret_cast<const float *>(at(r + e, c >> 2) + (c & 3) * 4);
+    }
+};
 
 // ---- the order of tiles --------------------------------------------------------------------------------------------------
 // Neighbours in the order share operand rows in their XCD's L2: bands of eight tile rows, column by column

@@ -20,6 +20,8 @@ namespace {
 using nt::f4;
 using nt::h4;
 using nt::h8;
+using nt::put_to;
+using nt::take_from;
 
 constexpr int kJobs = 20;        // jobs whose records one launch carries in its arguments (4 KB)
 constexpr int kMaxSteps = 32;
@@ -74,40 +76,40 @@ __device__ __forceinline__ int find_job(const int *first, int n, int at) {
 }
 
 __device__ __forceinline__ float load_as_float(const void *p, int dtype, int64_t at) {
-    if (dtype == CP_F32) return static_cast<const float *>(p)[at];
-    if (dtype == CP_BF16) return float(static_cast<const __bf16 *>(p)[at]);
-    return float(static_cast<const _Float16 *>(p)[at]);
+    if (dtype == CP_F32) return take_from<float>(static_cast<const float *>(p) + at);
+    if (dtype == CP_BF16) return float(take_from<__bf16>(static_cast<const __bf16 *>(p) + at));
+    return float(take_from<_Float16>(static_cast<const _Float16 *>(p) + at));
 }
 __device__ __forceinline__ void store_as(void *p, int dtype, int64_t at, float v) {
-    if (dtype == CP_F32) static_cast<float *>(p)[at] = v;
-    else if (dtype == CP_BF16) static_cast<__bf16 *>(p)[at] = __bf16(v);
-    else static_cast<_Float16 *>(p)[at] = _Float16(v);
+    if (dtype == CP_F32) put_to(static_cast<float *>(p) + at, v);
+    else if (dtype == CP_BF16) put_to(static_cast<__bf16 *>(p) + at, __bf16(v));
+    else put_to(static_cast<_Float16 *>(p) + at, _Float16(v));
 }
 __device__ __forceinline__ f4 load4_as_float(const void *p, int dtype, int64_t at) {
-    if (dtype == CP_F32) return *reinterpret_cast<const nt::f4u *>(static_cast<const float *>(p) + at);
-    if (dtype == CP_BF16) return __builtin_convertvector(*reinterpret_cast<const nt::b4u *>(static_cast<const __bf16 *>(p) + at), f4);
-    return __builtin_convertvector(*reinterpret_cast<const nt::h4u *>(static_cast<const _Float16 *>(p) + at), f4);
+    if (dtype == CP_F32) return take_from<nt::f4u>(static_cast<const float *>(p) + at);
+    if (dtype == CP_BF16) return __builtin_convertvector(take_from<nt::b4u>(static_cast<const __bf16 *>(p) + at), f4);
+    return __builtin_convertvector(take_from<nt::h4u>(static_cast<const _Float16 *>(p) + at), f4);
 }
 __device__ __forceinline__ void store4_as(void *p, int dtype, int64_t at, f4 v) {
-    if (dtype == CP_F32) *reinterpret_cast<nt::f4u *>(static_cast<float *>(p) + at) = v;
-    else if (dtype == CP_BF16) *reinterpret_cast<nt::b4u *>(static_cast<__bf16 *>(p) + at) = __builtin_convertvector(v, nt::b4);
-    else *reinterpret_cast<nt::h4u *>(static_cast<_Float16 *>(p) + at) = __builtin_convertvector(v, h4);
+    if (dtype == CP_F32) put_to<nt::f4u>(static_cast<float *>(p) + at, v);
+    else if (dtype == CP_BF16) put_to<nt::b4u>(static_cast<__bf16 *>(p) + at, __builtin_convertvector(v, nt::b4));
+    else put_to<nt::h4u>(static_cast<_Float16 *>(p) + at, __builtin_convertvector(v, h4));
 }
 
 // eight numbers of a row from column c, zero from `cols` on
 __device__ __forceinline__ void load8(const void *row, int dtype, int c, int cols, float (&v)[8]) {
     if (c + 8 <= cols) {
         if (dtype == CP_F32) {
-            const nt::f4u *p = reinterpret_cast<const nt::f4u *>(static_cast<const float *>(row) + c);
-            const f4 a = p[0], b = p[1];
+            const float *p = static_cast<const float *>(row) + c;
+            const f4 a = take_from<nt::f4u>(p), b = take_from<nt::f4u>(p + 4);
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = a[e], v[e + 4] = b[e];
         } else if (dtype == CP_BF16) {
-            const nt::b8 a = *reinterpret_cast<const nt::b8u *>(static_cast<const __bf16 *>(row) + c);
+            const nt::b8 a = take_from<nt::b8u>(static_cast<const __bf16 *>(row) + c);
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = float(a[e]);
         } else {
-            const h8 a = *reinterpret_cast<const nt::h8u *>(static_cast<const _Float16 *>(row) + c);
+            const h8 a = take_from<nt::h8u>(static_cast<const _Float16 *>(row) + c);
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = float(a[e]);
         }
@@ -115,6 +117,18 @@ __device__ __forceinline__ void load8(const void *row, int dtype, int c, int col
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? load_as_float(row, dtype, c + e) : 0.f;
+}
+
+// eight numbers of a row from column c, those before `cols`
+__device__ __forceinline__ void store8(void *row, int dtype, int c, int cols, const float (&v)[8]) {
+    if (c + 8 <= cols) {
+        store4_as(row, dtype, c, f4{v[0], v[1], v[2], v[3]});
+        store4_as(row, dtype, c + 4, f4{v[4], v[5], v[6], v[7]});
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 7; ++e)
+        if (c + e < cols) store_as(row, dtype, c + e, v[e]);
 }
 
 __device__ __forceinline__ const void *row_of(const void *p, int dtype, int64_t at) {
@@ -202,54 +216,28 @@ __global__ void __launch_bounds__(256) k_ortho_norm(Jobs js, Table t, float mome
     if (threadIdx.x == 0) j.part[id] = (s[0] + s[1]) + (s[2] + s[3]);
 }
 
-// sixteen numbers of a row, from column k (a multiple of 16), as fp16 or as pairs
+// eight numbers of a row, from column k (a multiple of 8), as fp16 or as pairs
 template <bool SPLIT>
-__device__ __forceinline__ void store16(char *row, int k, const float (&v)[16]) {
+__device__ __forceinline__ void store8(char *row, int k, const float *v) {
     char *p = row + (SPLIT ? (k >> 5) * 128 + (k & 31) * 2 : k * 2);
+    h8 hi, lo;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        h8 hi, lo;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            hi[e] = _Float16(v[8 * h + e]);
-            lo[e] = _Float16(v[8 * h + e] - float(hi[e]));
-        }
-        *reinterpret_cast<h8 *>(p + 16 * h) = hi;
-        if (SPLIT) *reinterpret_cast<h8 *>(p + 64 + 16 * h) = lo;
+    for (int e = 0; e < 8; ++e) {
+        const float x = SPLIT ? settled(v[e]) : v[e];
+        hi[e] = _Float16(x);
+        lo[e] = _Float16(x - float(hi[e]));
     }
-}
-
-// four numbers of a row, from column k (a multiple of 4)
-template <bool SPLIT>
-__device__ __forceinline__ void store4(char *row, int k, f4 v) {
-    char *p = row + (SPLIT ? (k >> 5) * 128 + (k & 31) * 2 : k * 2);
-    if (SPLIT) v = settled(v);
-    const h4 hi = __builtin_convertvector(v, h4);
-    *reinterpret_cast<h4 *>(p) = hi;
-    if (SPLIT) *reinterpret_cast<h4 *>(p + 64) = __builtin_convertvector(v - __builtin_convertvector(hi, f4), h4);
+    put_to(p, hi);
+    if (SPLIT) put_to(p + 64, lo);
 }
 template <bool SPLIT>
-__device__ __forceinline__ f4 load4(const char *row, int k) {
+__device__ __forceinline__ void load8(const char *row, int k, float (&v)[8]) {
     const char *p = row + (SPLIT ? (k >> 5) * 128 + (k & 31) * 2 : k * 2);
-    f4 v = __builtin_convertvector(*reinterpret_cast<const h4 *>(p), f4);
-    if (SPLIT) v += __builtin_convertvector(*reinterpret_cast<const h4 *>(p + 64), f4);
-    return v;
-}
-
-template <int CTRL>
-__device__ __forceinline__ float from_quad(float v) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
-}
-// the 4 x 4 numbers of four neighbouring lanes, transposed: lane q's v[r] becomes lane r's v[q]
-__device__ __forceinline__ f4 transpose4(f4 v, int lane) {
-    const bool odd = lane & 1, high = lane & 2;
-    const float a = from_quad<0xB1>(odd ? v[0] : v[1]), b = from_quad<0xB1>(odd ? v[2] : v[3]);
-    if (odd) v[0] = a, v[2] = b;
-    else v[1] = a, v[3] = b;
-    const float c = from_quad<0x4E>(high ? v[0] : v[2]), d = from_quad<0x4E>(high ? v[1] : v[3]);
-    if (high) v[0] = c, v[1] = d;
-    else v[2] = c, v[3] = d;
-    return v;
+    const h8 hi = take_from<h8>(p);
+    h8 lo = {};
+    if (SPLIT) lo = take_from<h8>(p + 64);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = SPLIT ? float(hi[e]) + float(lo[e]) : float(hi[e]);
 }
 
 // ---- X = U / (|U|_F + eps) in both orientations, zero in the padding: one 64 x 64 tile of G to a workgroup --------------------
@@ -288,7 +276,7 @@ __global__ void __launch_bounds__(256) k_ortho_load(Table tab, float momentum, i
     }
     const int n_part = (j.sum_rows + j.rows_per - 1) / j.rows_per * j.chunks;
     double part = 0.0;
-    for (int i = tid; i < n_part; i += 256) part += j.part[i];
+    for (int i = tid; i < n_part; i += 256) part += take_from<double>(j.part + i);
     part = wave_sum(part);
     if ((tid & 63) == 0) s[tid >> 6] = part;
     __syncthreads();
@@ -300,11 +288,13 @@ __global__ void __launch_bounds__(256) k_ortho_load(Table tab, float momentum, i
     }
     char *n = tall ? j.xt0 : j.x, *o = tall ? j.x : j.xt0;
     const uint32_t ldn = tall ? j.lds : j.ldn, ldo = tall ? j.ldn : j.lds;
-    store16<SPLIT>(n + int64_t(r0 + line) * ldn, c0 + k, v);
+    store8<SPLIT>(n + int64_t(r0 + line) * ldn, c0 + k, v);
+    store8<SPLIT>(n + int64_t(r0 + line) * ldn, c0 + k + 8, v + 8);
     __syncthreads();
 #pragma unroll
     for (int e = 0; e < 16; ++e) v[e] = t[k + e][line];
-    store16<SPLIT>(o + int64_t(c0 + line) * ldo, r0 + k, v);
+    store8<SPLIT>(o + int64_t(c0 + line) * ldo, r0 + k, v);
+    store8<SPLIT>(o + int64_t(c0 + line) * ldo, r0 + k + 8, v + 8);
 }
 
 // ---- the products ------------------------------------------------------------------------------------------------------------
@@ -364,40 +354,57 @@ __global__ void __launch_bounds__(CFG::T) k_ortho_product(Table tab, Factors f, 
         });
     if (pieces > 1 && !nt::join<T>(acc, piece, pieces, parts + int64_t(first + tile) * (BM * BN), tiles, counts + first + tile, &flag, tid))
         return;
+    typedef nt::Patch<WI, WJ> Patch;
+    const Patch patch = Patch::template of<CFG>(st, wave, lane);
 #pragma unroll
-    for (int wi = 0; wi < WI; ++wi) {
-        const int i = i0 + ra + wi * 16 + (lane & 15);
+    for (int pass = 0; pass < Patch::PASSES; ++pass) {
+        const int ip = i0 + ra + pass * Patch::ROWS, jp = j0 + rb;
+        // what lies beyond the padding is not there (both sides are multiples of 64: a pass is all in or all out)
+        if (ip >= rows_a || jp >= rows_b) break;
+        patch.put(acc, pass, f.acc);
+        auto finish = [&](int i, int c, float (&v)[8]) {   // eight neighbours of row i, or, as B is symmetric, of column i
+            if (PHASE != POLY) return;
+            float a[8];
+            load8<SPLIT>(j.a + int64_t(i) * j.lds, c, a);
 #pragma unroll
-        for (int wj = 0; wj < WJ; ++wj) {
-            const int c = j0 + rb + wj * 16 + (lane >> 4) * 4;
-            // the tile's rows and columns beyond the padding are not there (both are multiples of 64: a group of 16 is all in or out)
-            if (i0 + ra + wi * 16 >= rows_a || j0 + rb + wj * 16 >= rows_b) continue;
-            f4 v = acc[wi][wj] * f.acc;
-            if (PHASE == POLY) {
-                v += load4<SPLIT>(j.a + int64_t(i) * j.lds, c) * f.a;
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (c + r == i) v[r] += f.diag;
+            for (int e = 0; e < 8; ++e) {
+                v[e] = fmaf(a[e], f.a, v[e]);
+                if (c + e == i) v[e] += f.diag;
             }
+        };
+#pragma unroll 4
+        for (int u = 0; u < Patch::EIGHTS; ++u) {
+            int i, c;
+            float v[8];
+            patch.of_row(u, i, c, v);
+            i += ip;
+            c += jp;
+            finish(i, c, v);
             if (PHASE != LAST) {
                 char *out = PHASE == GRAM ? j.a : PHASE == POLY ? j.b : j.x;
-                char *out_t = PHASE == GRAM ? j.a : PHASE == POLY ? j.b : f.xt ? j.xt0 : j.xt1;
-                store4<SPLIT>(out + int64_t(i) * (SYM ? j.lds : j.ldn), c, v);
-                if (!SYM || tm != tn) store4<SPLIT>(out_t + int64_t(c + (lane & 3)) * j.lds, i & ~3, transpose4(v, lane));
+                store8<SPLIT>(out + int64_t(i) * (SYM ? j.lds : j.ldn), c, v);
             } else if (i < j.rows && c < j.cols) {
-                const int64_t o = i * j.ldo + c;
-                if (c + 4 <= j.cols) {
-                    if (j.M) v = load4_as_float(j.out, j.o_dtype, o) * f.keep - v * j.lr;
-                    store4_as(j.out, j.o_dtype, o, v);
-                } else {
+                void *row = const_cast<void *>(row_of(j.out, j.o_dtype, i * j.ldo));
+                if (j.M) {
+                    float w[8];
+                    load8(row, j.o_dtype, c, j.cols, w);
 #pragma unroll
-                    for (int r = 0; r < 3; ++r) {
-                        if (c + r >= j.cols) break;
-                        float y = v[r];
-                        if (j.M) y = f.keep * load_as_float(j.out, j.o_dtype, o + r) - j.lr * y;
-                        store_as(j.out, j.o_dtype, o + r, y);
-                    }
+                    for (int e = 0; e < 8; ++e) v[e] = f.keep * w[e] - j.lr * v[e];
                 }
+                store8(row, j.o_dtype, c, j.cols, v);
+            }
+        }
+        if (PHASE != LAST && (!SYM || tm != tn)) {
+#pragma unroll 4
+            for (int u = 0; u < Patch::EIGHTS; ++u) {
+                int i, c;
+                float v[8];
+                patch.of_column(u, i, c, v);
+                i += ip;
+                c += jp;
+                finish(c, i, v);
+                char *out_t = PHASE == GRAM ? j.a : PHASE == POLY ? j.b : f.xt ? j.xt0 : j.xt1;
+                store8<SPLIT>(out_t + int64_t(c) * j.lds, i, v);
             }
         }
     }
