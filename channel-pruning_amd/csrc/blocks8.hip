@@ -12,6 +12,7 @@ using nt::f4;
 constexpr float kTiny = 7.888609052210118e-31f;   // 2^-100: a block's largest magnitude counts as at least this
 constexpr int64_t kMaxLd = int64_t(1) << 22;
 constexpr int64_t kMaxRows = int64_t(1) << 30;
+constexpr int64_t kMaxThreads = (int64_t(1) << 32) - 1;   // of a launch
 
 int check_blocks(cp_ctx *ctx, const cp_blocks *m, const char *name) {
     if (!m) return cp_set_error(ctx, CP_ERR_ARG, "%s: null description", name);
@@ -163,13 +164,15 @@ __device__ __forceinline__ void write_patch(const float (&v)[8][8], const float 
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) k_quant_blocks(const T *__restrict__ x, int64_t rows, int64_t cols, int64_t ldx, int pow2,
+__global__ void __launch_bounds__(256) k_quant_blocks(const T *__restrict__ x, int64_t rows, int64_t cols, int64_t ldx, int tiles_c, int pow2,
                                                       Held o, Held t) {
     __shared__ alignas(16) uint32_t rmax[2][128], cmax[16][128];
     __shared__ float inverse[2][128];   // of the tile's rows and columns
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int lr = (wave >> 1) * 64 + (lane >> 3) * 8, lc = (wave & 1) * 64 + (lane & 7) * 8;
-    const int64_t r0 = int64_t(blockIdx.y) * 128, c0 = int64_t(blockIdx.x) * 128;
+    // neighbours in a row on one XCD: where rows begin inside a line, they share it in that XCD's L2
+    const int tile = nt::xcd_runs(blockIdx.x, gridDim.x), tr = tile / tiles_c, tc = tile % tiles_c;
+    const int64_t r0 = int64_t(tr) * 128, c0 = int64_t(tc) * 128;
     const int64_t row = r0 + lr, col = c0 + lc;
 
     float v[8][8];
@@ -224,7 +227,7 @@ __global__ void __launch_bounds__(256) k_quant_blocks(const T *__restrict__ x, i
             }
             float scale;
             scale_of(m, h.fmt, pow2, scale, inverse[is_col][k]);
-            float *sp = is_col ? t.scale + blockIdx.y * t.lds : o.scale + blockIdx.x * o.lds;
+            float *sp = is_col ? t.scale + tr * t.lds : o.scale + tc * o.lds;
             const int64_t at = (is_col ? c0 : r0) + k, n = is_col ? cols : rows;
             if (h.tile == 1 ? at < n : k == 0) sp[h.tile == 1 ? at : at / 128] = scale;
         }
@@ -243,9 +246,9 @@ Held held(const cp_blocks *m) {
 template <typename T>
 void launch_quant(cp_ctx *ctx, const void *x, int64_t rows, int64_t cols, int64_t ldx, int flags, const cp_blocks *out,
                   const cp_blocks *out_t) {
-    const dim3 grid(uint32_t((cols + 127) / 128), uint32_t((rows + 127) / 128));
-    k_quant_blocks<T><<<grid, 256, 0, ctx->stream>>>(static_cast<const T *>(x), rows, cols, ldx, flags & CP_QUANT_POW2,
-                                                     held(out), held(out_t));
+    const int64_t tiles_c = (cols + 127) / 128, tiles_r = (rows + 127) / 128;
+    k_quant_blocks<T><<<uint32_t(tiles_c * tiles_r), 256, 0, ctx->stream>>>(static_cast<const T *>(x), rows, cols, ldx, int(tiles_c),
+                                                                            flags & CP_QUANT_POW2, held(out), held(out_t));
 }
 
 // ---- the product ---------------------------------------------------------------------------------------------------------
@@ -281,11 +284,7 @@ __device__ __forceinline__ void store1(const Product &p, int64_t i, int j, float
 
 __device__ __forceinline__ void store8(const Product &p, int64_t i, int j, const float (&v)[8]) {
     const int64_t at = i * p.ldc + j;
-    if (p.c_dtype == CP_F32) {
-        nt::f4u *to = reinterpret_cast<nt::f4u *>(static_cast<float *>(p.c) + at);
-        to[0] = f4{v[0], v[1], v[2], v[3]};
-        to[1] = f4{v[4], v[5], v[6], v[7]};
-    } else if (p.c_dtype == CP_BF16) {
+    if (p.c_dtype == CP_BF16) {
         nt::b8 q;
 #pragma unroll
         for (int e = 0; e < 8; ++e) q[e] = __bf16(v[e]);
@@ -302,20 +301,39 @@ __device__ __forceinline__ void store8(const Product &p, int64_t i, int j, const
 template <int WI, int WJ>
 __device__ __forceinline__ void write_c(const Product &p, const f4 (&acc)[WI][WJ], int i0, int j0, const nt::Patch<WI, WJ> &patch) {
     typedef nt::Patch<WI, WJ> Patch;
+    const int each = p.c_dtype == CP_F32 ? 4 : 8, mine = j0 + patch.lane % (Patch::COLS / each) * each;
     float bias[8];   // a lane's columns are the same in all of its groups
-    const int mine = j0 + patch.lane % (Patch::COLS / 8) * 8;
 #pragma unroll
     for (int e = 0; e < 8; ++e) bias[e] = p.bias && mine + e < p.N ? p.bias[mine + e] : 0.f;
 #pragma unroll
     for (int pass = 0; pass < Patch::PASSES; ++pass) {
-        if (i0 + pass * Patch::ROWS >= p.M) break;
+        const int ip = i0 + pass * Patch::ROWS;
+        if (ip >= p.M) break;
         patch.put(acc, pass, 1.f);
+        if (p.c_dtype == CP_F32) {
+#pragma unroll
+            for (int u = 0; u < 2 * Patch::EIGHTS; ++u) {
+                int i, j;
+                const f4 v = patch.four_of_row(u, i, j) + f4{bias[0], bias[1], bias[2], bias[3]};
+                i += ip;
+                j += j0;
+                if (i >= p.M) continue;
+                if (j + 4 <= p.N) {
+                    store4(p, i, j, v);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 3; ++e)
+                        if (j + e < p.N) store1(p, i, j + e, v[e]);
+                }
+            }
+            continue;
+        }
 #pragma unroll
         for (int u = 0; u < Patch::EIGHTS; ++u) {
             int i, j;
             float v[8];
             patch.of_row(u, i, j, v);
-            i += i0 + pass * Patch::ROWS;
+            i += ip;
             j += j0;
             if (i >= p.M) continue;
 #pragma unroll
@@ -462,7 +480,6 @@ __global__ void __launch_bounds__(512) k_matmul_blocks_rows(Product p) {
 }
 
 bool wide_form(int c_dtype) { return c_dtype != CP_BF16; }   // what the 8-bit matrix instructions drop is below bfloat16's rounding only
-constexpr int64_t kMaxThreads = (int64_t(1) << 32) - 1;       // of a launch
 
 int check_product(cp_ctx *ctx, const cp_blocks *A, const cp_blocks *B, int c_dtype, int64_t ldc) {
     CP_TRY(check_blocks(ctx, A, "A"));
@@ -567,7 +584,7 @@ extern "C" int cp_quant_blocks(cp_ctx *ctx, const void *x, int x_dtype, int64_t 
     if (!rows || !cols) return CP_OK;
     const size_t size = x_dtype == CP_F64 ? 8 : x_dtype == CP_F32 ? 4 : 2;
     if (!x || uintptr_t(x) % size) return cp_set_error(ctx, CP_ERR_ARG, "x is null or misaligned");
-    if ((rows + 127) / 128 > 65535) return cp_set_error(ctx, CP_ERR_UNSUPPORTED, "more than 65535 * 128 rows");
+    if (((rows + 127) / 128) * ((cols + 127) / 128) * 256 > kMaxThreads) return cp_set_error(ctx, CP_ERR_UNSUPPORTED, "x is too large");
     CP_HIP(ctx, hipSetDevice(ctx->device));
     switch (x_dtype) {
         case CP_F32: launch_quant<float>(ctx, x, rows, cols, ldx, flags, out, out_t); break;

@@ -392,6 +392,12 @@ struct Patch {
                 *reinterpret_cast<f4 *>(at(i * 16 + (lane & 15), j * 4 + (lane >> 4))) = acc[pass * (ROWS / 16) + i][j] * factor;
         order();
     }
+    // four numbers of row r from column c (u < 2 EIGHTS): float32 results, 16 bytes a lane
+    __device__ __forceinline__ f4 four_of_row(int u, int &r, int &c) const {
+        r = (u * 64 + lane) / (COLS / 4);
+        c = (u * 64 + lane) % (COLS / 4) * 4;
+        return *reinterpret_cast<const f4 *>(at(r, c / 4));
+    }
     // group u: eight numbers of row r from column c, or of column c from row r
     __device__ __forceinline__ void of_row(int u, int &r, int &c, float (&v)[8]) const {
         r = (u * 64 + lane) / (COLS / 8);
@@ -440,6 +446,13 @@ __device__ __forceinline__ void lower_tile_at(int t, int tiles, int &tm, int &tn
 __device__ __forceinline__ int xcd_order(int id, int n) {
     const int q = n >> 3, r = n & 7, x = id & 7;
     return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (id >> 3);
+}
+
+// The same in runs of eight, for kernels that stream: neighbours share the lines between them in one L2, while all XCDs work on
+// one region of memory.
+__device__ __forceinline__ int xcd_runs(int id, int n) {
+    const int block = id & ~63;
+    return block + 64 <= n ? block | (id & 7) << 3 | (id >> 3 & 7) : id;
 }
 
 }  // namespace nt

@@ -181,33 +181,69 @@ __global__ void __launch_bounds__(256) k_ortho_norm(Jobs js, Table t, float mome
         }
     }
     for (int i = blockIdx.x * 256 + threadIdx.x; i < n_counts; i += gridDim.x * 256) counts[i] = 0;
-    const int r0 = id / j.chunks * j.rows_per, r1 = min(r0 + j.rows_per, j.sum_rows);
+    const int r0 = id / j.chunks * j.rows_per, rows = min(r0 + j.rows_per, j.sum_rows) - r0;
     const int64_t c0 = int64_t(id % j.chunks) * j.width;
-    const int wide = int(min(j.sum_cols - c0, int64_t(j.width))), eights = (wide + 7) / 8;
+    const int wide = int(min(j.sum_cols - c0, int64_t(j.width))), eights = wide / 8, tail = wide & 7, n = rows * eights;
     double sum = 0.0;
-    for (int u = threadIdx.x; u < (r1 - r0) * eights; u += 256) {
-        const int k = r1 - r0 > 1 ? u / eights : 0, r = r0 + k, c = (u - k * eights) * 8;
-        float v[8];
-        load8(row_of(j.G, j.g_dtype, r * j.ldg + c0), j.g_dtype, c, wide, v);
-        if (j.M) {
-            float *row = j.M + r * j.ldm + c0, m[8];
-            load8(row, CP_F32, c, wide, m);
+    auto momentum_of = [&](float &m, float &v) {
+        m = fmaf(momentum, m, v);
+        v = nesterov ? fmaf(momentum, m, v) : m;
+    };
+    // whole groups of eight, AT_ONCE loads of a thread under way together (beyond the end the last group's again, for nothing)
+    auto groups = [&](auto type) {
+        typedef decltype(type) V;   // eight numbers, at any element's address
+        constexpr int AT_ONCE = 4, SIZE = int(sizeof(V) / 8);
+        for (int u0 = threadIdx.x; u0 < n; u0 += 256 * AT_ONCE) {
+            int64_t r[AT_ONCE];
+            int c[AT_ONCE];
+            V v[AT_ONCE];
+            f4 m[AT_ONCE][2];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                m[e] = fmaf(momentum, m[e], v[e]);
-                v[e] = nesterov ? fmaf(momentum, m[e], v[e]) : m[e];
+            for (int q = 0; q < AT_ONCE; ++q) {
+                const int u = min(u0 + q * 256, n - 1), k = rows > 1 ? u / eights : 0;
+                r[q] = r0 + k;
+                c[q] = (u - k * eights) * 8;
+                v[q] = take_from<V>(static_cast<const char *>(j.G) + (r[q] * j.ldg + c0 + c[q]) * SIZE);
             }
-            if (c + 8 <= wide) {
-                *reinterpret_cast<nt::f4u *>(row + c) = f4{m[0], m[1], m[2], m[3]};
-                *reinterpret_cast<nt::f4u *>(row + c + 4) = f4{m[4], m[5], m[6], m[7]};
-            } else {
+            if (j.M) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (c + e < wide) row[c + e] = m[e];
+                for (int q = 0; q < AT_ONCE; ++q)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) m[q][h] = take_from<nt::f4u>(j.M + r[q] * j.ldm + c0 + c[q] + 4 * h);
+            }
+#pragma unroll
+            for (int q = 0; q < AT_ONCE; ++q) {
+                if (u0 + q * 256 >= n) break;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    float x = float(v[q][e]);
+                    if (j.M) {
+                        float y = m[q][e >> 2][e & 3];
+                        momentum_of(y, x);
+                        m[q][e >> 2][e & 3] = y;
+                    }
+                    sum = fma(double(x), double(x), sum);
+                }
+                if (j.M) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) put_to<nt::f4u>(j.M + r[q] * j.ldm + c0 + c[q] + 4 * h, m[q][h]);
+                }
             }
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum = fma(double(v[e]), double(v[e]), sum);
+    };
+    typedef float f8u __attribute__((ext_vector_type(8), aligned(4)));
+    if (j.g_dtype == CP_F32) groups(f8u());
+    else if (j.g_dtype == CP_BF16) groups(nt::b8u());
+    else groups(nt::h8u());
+    for (int u = threadIdx.x; u < rows * tail; u += 256) {   // the rows' ends
+        const int64_t r = r0 + u / tail, c = c0 + eights * 8 + u % tail;
+        float x = load_as_float(j.G, j.g_dtype, r * j.ldg + c);
+        if (j.M) {
+            float y = load_as_float(j.M, CP_F32, r * j.ldm + c);
+            momentum_of(y, x);
+            store_as(j.M, CP_F32, r * j.ldm + c, y);
+        }
+        sum = fma(double(x), double(x), sum);
     }
     __shared__ double s[4];
     sum = wave_sum(sum);
@@ -254,10 +290,10 @@ __device__ __forceinline__ void load_tile(const void *p, int dtype, int64_t ld, 
 
 template <bool SPLIT>
 __global__ void __launch_bounds__(256) k_ortho_load(Table tab, float momentum, int nesterov, double eps, float x_scale) {
-    const int which = find_job(tab.first[LOAD], tab.n, blockIdx.x);
+    const int at = nt::xcd_runs(blockIdx.x, gridDim.x), which = find_job(tab.first[LOAD], tab.n, at);
     const Job j = tab.job[which];
     const bool tall = j.rows > j.cols;
-    const int id = blockIdx.x - tab.first[LOAD][which], tiles_c = (tall ? j.mp : j.np) / 64;
+    const int id = at - tab.first[LOAD][which], tiles_c = (tall ? j.mp : j.np) / 64;
     const int r0 = id / tiles_c * 64, c0 = id % tiles_c * 64;
     __shared__ double s[4];
     __shared__ float t[64][65];
@@ -372,7 +408,32 @@ __global__ void __launch_bounds__(CFG::T) k_ortho_product(Table tab, Factors f, 
                 if (c + e == i) v[e] += f.diag;
             }
         };
-#pragma unroll 4
+        constexpr int AT_ONCE = Patch::PASSES == 1 ? 8 : 4;
+        if (PHASE == LAST && SPLIT && j.o_dtype == CP_F32) {
+#pragma unroll AT_ONCE
+            for (int u = 0; u < 2 * Patch::EIGHTS; ++u) {
+                int i, c;
+                f4 v = patch.four_of_row(u, i, c);
+                i += ip;
+                c += jp;
+                if (i >= j.rows || c >= j.cols) continue;
+                const int64_t o = i * j.ldo + c;
+                if (c + 4 <= j.cols) {
+                    if (j.M) v = load4_as_float(j.out, CP_F32, o) * f.keep - v * j.lr;
+                    store4_as(j.out, CP_F32, o, v);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 3; ++r) {
+                        if (c + r >= j.cols) break;
+                        float y = v[r];
+                        if (j.M) y = f.keep * load_as_float(j.out, CP_F32, o + r) - j.lr * y;
+                        store_as(j.out, CP_F32, o + r, y);
+                    }
+                }
+            }
+            continue;
+        }
+#pragma unroll AT_ONCE
         for (int u = 0; u < Patch::EIGHTS; ++u) {
             int i, c;
             float v[8];

@@ -269,8 +269,8 @@ int cp_blocks_check(const cp_blocks *m);
  *   amax  = the largest |x| of its finite values, at least 2^-100;   scale = amax / fmax,  inverse = fmax / amax
  *   (CP_QUANT_POW2: scale = the smallest power of two >= amax / fmax, inverse = 1 / scale);
  *   q = x * inverse cut to +-fmax, rounded to nearest even.  A NaN or an infinity becomes NaN.
- * F64 is rounded to float32 first.  x and the outputs must not overlap; rows up to 65535 * 128.  Asynchronous on the context's
- * stream, no workspace; can be captured. */
+ * F64 is rounded to float32 first.  x and the outputs must not overlap.  Asynchronous on the context's stream, no workspace;
+ * can be captured. */
 int cp_quant_blocks(cp_ctx *ctx, const void *x, int x_dtype, int64_t rows, int64_t cols, int64_t ldx, int flags,
                     const cp_blocks *out, const cp_blocks *out_t);
 /* C[i, j] = sum_k A[i, k] B[j, k] (+ bias[j]): A [M, K], B [N, K], C DEVICE [M, N] (c_dtype F32, BF16 or F16, row stride
