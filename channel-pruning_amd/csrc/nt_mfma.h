@@ -448,11 +448,11 @@ __device__ __forceinline__ int xcd_order(int id, int n) {
     return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (id >> 3);
 }
 
-// The same in runs of eight, for kernels that stream: neighbours share the lines between them in one L2, while all XCDs work on
+// The same in runs of 32, for kernels that stream: neighbours share the lines between them in one L2, while all XCDs work on
 // one region of memory.
 __device__ __forceinline__ int xcd_runs(int id, int n) {
-    const int block = id & ~63;
-    return block + 64 <= n ? block | (id & 7) << 3 | (id >> 3 & 7) : id;
+    const int block = id & ~255;
+    return block + 256 <= n ? block | (id & 7) << 5 | (id >> 3 & 31) : id;
 }
 
 }  // namespace nt

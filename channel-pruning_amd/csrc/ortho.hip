@@ -46,7 +46,8 @@ struct Job {
 };
 
 // The phases' launches: job k's first workgroup of each, and the pieces of k that its tiles are cut into
-enum { LOAD, GRAM, POLY, APPLY, PHASES };
+// (LAST: the last step's third product, which writes O or W)
+enum { LOAD, GRAM, POLY, APPLY, LAST, PHASES };
 struct Place {
     int first[PHASES];
     int16_t pieces[PHASES];
@@ -334,8 +335,6 @@ __global__ void __launch_bounds__(256) k_ortho_load(Table tab, float momentum, i
 }
 
 // ---- the products ------------------------------------------------------------------------------------------------------------
-constexpr int LAST = PHASES;   // the step's third product where it is the call's last: writes O or W
-
 struct Factors {
     float acc, a, diag;   // what the accumulator, A's entry and the diagonal count for in the result
     float keep;           // LAST: 1 - lr * weight_decay (cp_ortho_step)
@@ -346,15 +345,14 @@ template <int PHASE, bool SPLIT, class CFG>
 __global__ void __launch_bounds__(CFG::T) k_ortho_product(Table tab, Factors f, float *parts, int *counts) {
     constexpr int BM = CFG::BM, BN = CFG::BN, T = CFG::T, WI = CFG::WI, WJ = CFG::WJ;
     constexpr bool SYM = PHASE == GRAM || PHASE == POLY;
-    constexpr int LIST = PHASE == LAST ? APPLY : PHASE;
     NT_STAGES(st, CFG::STAGES, CFG::STAGE);
     __shared__ int flag;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / CFG::NWN, wn = wave % CFG::NWN;
     const int ra = wm * WI * 16, rb = wn * WJ * 16;
-    const int at = nt::xcd_order(blockIdx.x, gridDim.x), which = find_job(tab.first[LIST], tab.n, at);
+    const int at = nt::xcd_order(blockIdx.x, gridDim.x), which = find_job(tab.first[PHASE], tab.n, at);
     const Job j = tab.job[which];
-    const int first = tab.first[LIST][which], pieces = tab.pieces[LIST][which];
+    const int first = tab.first[PHASE][which], pieces = tab.pieces[PHASE][which];
     const bool tall = j.rows > j.cols;
     const bool swap = PHASE == LAST && tall;   // the result's rows are G's rows: four consecutive numbers lie in one of them
     const char *xt = f.xt ? j.xt1 : j.xt0;
@@ -1004,7 +1002,7 @@ struct Class {
     std::vector<int> sum_groups;   // workgroups of k_ortho_norm
     Table table;
     int64_t loads = 0;
-    Choice gram, poly, apply;
+    Choice gram, poly, apply, last;
 };
 
 constexpr int kEdge[3] = {256, 128, 64};
@@ -1012,18 +1010,20 @@ constexpr int64_t kMaxThreads = (int64_t(1) << 32) - 1;   // of a launch
 
 int64_t tiles_of(const Job &j, int phase, int edge) {
     const int64_t m = (j.mp + edge - 1) / edge, n = (j.np + edge - 1) / edge;
-    return phase == APPLY ? m * n : m * (m + 1) / 2;
+    return phase == APPLY || phase == LAST ? m * n : m * (m + 1) / 2;
 }
 int64_t steps_of(const Job &j, int phase) { return (phase == GRAM ? j.ldn : j.lds) / 128; }
 
 // What a launch costs in us, from its number of workgroups, their K steps in all and the longest's.
 // Measured: us per step and workgroup where a CU holds as many as fit (Large one, the others two), and where there is at most
-// one to a CU; what a workgroup costs beside its steps (first loads, stores: twice as many where numbers are pairs); a join.
-double cost_of(int cfg, bool split, int64_t groups, int64_t total, int64_t longest, bool joins) {
+// one to a CU; what a workgroup costs beside its steps (first loads, stores: twice as many where numbers are pairs); a join; and
+// what it costs to read and write W.
+double cost_of(int cfg, bool split, bool weights, int64_t groups, int64_t total, int64_t longest, bool joins) {
     static const double full[2][3] = {{1.55, 1.04, 0.33}, {2.25, 1.35, 0.37}}, alone[2][3] = {{1.35, 0.60, 0.20}, {2.0, 0.75, 0.28}};
-    static const double extra[2][3] = {{14.0, 6.0, 3.5}, {28.0, 11.0, 5.0}}, joined[3] = {14.0, 5.0, 3.0};
+    static const double extra[2][3] = {{14.0, 6.0, 3.0}, {19.0, 11.0, 4.0}}, joined[3] = {14.0, 5.0, 3.0}, update[3] = {20.0, 13.0, 2.2};
     const int slots = cfg == 0 ? kCus : 2 * kCus;
-    const double step = groups > kCus ? full[split][cfg] : alone[split][cfg], more = extra[split][cfg] + (joins ? joined[cfg] : 0.0);
+    const double step = groups > kCus ? full[split][cfg] : alone[split][cfg];
+    const double more = extra[split][cfg] + (joins ? joined[cfg] : 0.0) + (weights ? update[cfg] : 0.0);
     const double mean = double(total) / groups * step + more, most = longest * step + more, rounds = double(groups) / slots;
     // equal workgroups end together; others fill each other's gaps
     return std::max(most, mean * (total == longest * groups ? std::ceil(rounds) : rounds + 0.3));
@@ -1039,7 +1039,7 @@ int pieces_of(const Job &j, int phase, bool split) {
     for (int cfg = 0; cfg < 3; ++cfg) {
         const int64_t tiles = tiles_of(j, phase, kEdge[cfg]);
         for (int p = 1; p <= 16 && (p == 1 || steps / p >= kLeast); ++p) {
-            const double c = cost_of(cfg, split, tiles * p, tiles * steps, (steps + p - 1) / p, p > 1);
+            const double c = cost_of(cfg, split, phase == LAST && j.M, tiles * p, tiles * steps, (steps + p - 1) / p, p > 1);
             if (c < 0.97 * least) {
                 least = c;
                 best = p;
@@ -1066,7 +1066,7 @@ bool choose(Class &cl, int phase, Choice &best) {
         }
         if (groups * (cfg == 0 ? nt::Large::T : nt::Medium::T) > kMaxThreads) continue;
         c.grid = int(groups);
-        const double cost = cost_of(cfg, cl.split, groups, total, longest, c.joins);
+        const double cost = cost_of(cfg, cl.split, phase == LAST && cl.jobs[0].M, groups, total, longest, c.joins);
         if (cost < least) {
             least = cost;
             best = c;
@@ -1158,9 +1158,9 @@ int lay_out(cp_ctx *ctx, const std::vector<Request> &rq, bool crossed, double lr
     }
     for (Class &cl : lay.cls) {
         if (cl.jobs.empty()) continue;
-        if (cl.loads * 256 > kMaxThreads || !choose(cl, GRAM, cl.gram) || !choose(cl, POLY, cl.poly) || !choose(cl, APPLY, cl.apply))
+        if (cl.loads * 256 > kMaxThreads || !choose(cl, GRAM, cl.gram) || !choose(cl, POLY, cl.poly) || !choose(cl, APPLY, cl.apply) || !choose(cl, LAST, cl.last))
             return cp_set_error(ctx, CP_ERR_UNSUPPORTED, "matrices of a call too large for one launch");
-        for (const Choice *c : {&cl.gram, &cl.poly, &cl.apply})
+        for (const Choice *c : {&cl.gram, &cl.poly, &cl.apply, &cl.last})
             if (c->joins) {
                 lay.counts = std::max(lay.counts, cp_align_up(size_t(c->grid) * sizeof(int), 256));
                 lay.parts = std::max(lay.parts, size_t(c->grid) * kEdge[c->cfg] * kEdge[c->cfg] * sizeof(float));
@@ -1241,7 +1241,7 @@ void launch_steps(const Call &call, const Class &cl, const Plan &pl, float keep)
         f.acc = q.apply;
         f.keep = keep;
         if (k + 1 < pl.steps) launch_product<APPLY, SPLIT>(call, cl.table, cl.apply, f);
-        else launch_product<LAST, SPLIT>(call, cl.table, cl.apply, f);
+        else launch_product<LAST, SPLIT>(call, cl.table, cl.last, f);
     }
 }
 
