@@ -33,7 +33,8 @@ int check_blocks(cp_ctx *ctx, const cp_blocks *m, const char *name) {
 // an 8 x 8 patch in registers, so x is read once for both orientations; a wave's patches form 64 x 64, which makes the
 // segments that it writes 64 bytes long in either.  Bound by HBM, as long as the arithmetic stays short: the largest magnitudes
 // are found on the bit patterns; a thread makes the factors of one row or column, not of its patch's sixteen; and what only
-// infinities and NaN need is done in tiles that hold one.  (No cut to +-fmax is needed: a finite x times the inverse exceeds
+// infinities and NaN need is done in tiles that hold one.  f32 [20000, 4608] both ways: 107 us for 559 MB (5.2 TB/s; a large copy
+// reaches 4.9), bf16 [4096, 25088]: 86 us for 411 MB, bf16 [20000, 4005], whose rows begin anywhere: 82 us for 324 MB.  (No cut to +-fmax is needed: a finite x times the inverse exceeds
 // fmax by two roundings at most, and rounds to it.)
 struct Held {
     uint8_t *q;
@@ -349,6 +350,13 @@ __device__ __forceinline__ void write_c(const Product &p, const f4 (&acc)[WI][WJ
     }
 }
 
+// One tile of C, or a piece of k of it, to a workgroup.  COMMON: B's rows share their scales in blocks of 128 (weights), so that a
+// wave multiplies each sum by one factor; else by a row's and a column's.  Beside the matrix instructions a step has that
+// factor and a fused add for every number of the tile: bound by both together.  8192^3, every row with its own scales: 527 us, 2.09
+// PFLOP/s (a library product without any scales 358); common scales, 20000 x 512 x 4005: 67 us, 1.22 (its
+// 80 MB come from HBM one step ahead of their use).  WIDE (float32 and fp16 results):
+// the operands are widened in registers, 128 conversions to 64 matrix instructions of a wave, which cost as much again
+// (512 x 4005 x 20000: 112 us, 0.73 PFLOP/s); 256 x 256 tiles would need more registers than there are.
 template <class CFG, int FA, int FB, bool COMMON, bool WIDE>
 __global__ void __launch_bounds__(CFG::T) k_matmul_blocks(Product p) {
     constexpr int BM = CFG::BM, BN = CFG::BN, T = CFG::T, WI = CFG::WI, WJ = CFG::WJ;
@@ -405,7 +413,8 @@ __global__ void __launch_bounds__(CFG::T) k_matmul_blocks(Product p) {
 
 // Few rows of A: bound by reading B once.  A workgroup takes sixteen rows of B and its eight waves an eighth of k each, straight
 // from memory into the matrix instruction's registers (a lane holds 32 bytes of one row: the K order within a block is the same
-// for A and B, and that is all that a sum needs); their sums are added in the order of k.
+// for A and B, and that is all that a sum needs); their sums are added in the order of k.  Up to 32 rows: one row by 4096 x 4096
+// takes 5 us (17 MB), a call of it 7.3 (17 rows: 7.5; 64 x 64 tiles 12, 128 x 128 18).
 template <int MT, int FA, int FB, bool COMMON, bool WIDE>
 __global__ void __launch_bounds__(512) k_matmul_blocks_rows(Product p) {
     __shared__ alignas(16) float sum[8][MT][64][4];
@@ -497,7 +506,7 @@ int check_product(cp_ctx *ctx, const cp_blocks *A, const cp_blocks *B, int c_dty
 
 // How a product is formed: by its shape, its types and C's type alone
 struct Form {
-    int cfg;             // 0 Large, 1 Medium, 2 Small, 3 few rows
+    int cfg;             // 0 Large, 1 Medium, 2 Small, 3 Flat, 4 few rows
     int tiles_m, tiles_n, pieces;
     size_t counts, parts;   // bytes
 };
@@ -505,29 +514,36 @@ constexpr int kMaxJoined = 16384;   // workgroups of a launch that joins pieces
 constexpr int kChip = 256;          // CUs that a split is planned for
 
 Form form_of(const cp_blocks *A, const cp_blocks *B, int c_dtype) {
-    // us per step and workgroup on a full chip / with at most one to a CU, beside the steps, and for a join; [wide][cfg]
-    static const double full[2][3] = {{2.2, 1.1, 0.36}, {1e3, 1.75, 0.6}}, alone[2][3] = {{1.9, 0.85, 0.26}, {1e3, 1.4, 0.45}};
-    static const double extra[3] = {8.0, 5.0, 3.5}, joined[3] = {12.0, 5.0, 3.0};
+    // us per step and workgroup on a full chip / with at most one to a CU, beside the steps, for a join and for every piece that it
+    // adds; [wide][cfg].  Fitted to 172 shapes (33..20000 x 64..8192 x 128..16384): off by 4 to 9 % (root mean square), and the
+    // rule's choice takes 1.01 of the time of the best shape of tile.
+    static const double full[2][4] = {{1.67, 1.04, 0.38, 1.24}, {0, 1.82, 0.69, 0}}, alone[2][4] = {{1.31, 0.68, 0.265, 1.14}, {0, 1.2, 0.51, 0}};
+    static const double extra[4] = {6.3, 4.5, 2.2, 6.2}, joined[4] = {16.0, 7.0, 1.2, 15.0}, piece[4] = {1.7, 0.5, 0.5, 1.35};
+    static const int rows_of[4] = {nt::Large::BM, nt::Medium::BM, nt::Small::BM, nt::Flat::BM};
+    static const int cols_of[4] = {nt::Large::BN, nt::Medium::BN, nt::Small::BN, nt::Flat::BN};
     const int64_t steps = (A->cols + 127) / 128;
     const bool wide = wide_form(c_dtype);
     Form best = {};
     const int forced = cp_knob(CP_KNOB_NT_TILE);
-    if (A->rows <= 32 && B->rows <= kMaxThreads / 512 * 16 && !forced) return {3, 0, 0, 1, 0, 0};
+    if (A->rows <= 32 && B->rows <= kMaxThreads / 512 * 16 && !forced) return {4, 0, 0, 1, 0, 0};
     double least = 1e300;
-    for (int cfg = wide ? 1 : 0; cfg < 3; ++cfg) {
-        if (forced && forced - 1 != cfg && !(wide && forced == 1 && cfg == 1)) continue;
-        const int64_t edge = 256 >> cfg, tm = (A->rows + edge - 1) / edge, tn = (B->rows + edge - 1) / edge;
-        if (tm * tn * (cfg == 0 ? nt::Large::T : nt::Medium::T) > kMaxThreads) continue;   // (the largest tile's count is checked)
+    for (int cfg = 0; cfg < 4; ++cfg) {
+        const bool alone_on_cu = cfg == 0 || cfg == 3;
+        if (wide && alone_on_cu) continue;
+        if (forced && forced - 1 != cfg && !(wide && cfg == 1 && (forced == 1 || forced == 4))) continue;
+        const int64_t tm = (A->rows + rows_of[cfg] - 1) / rows_of[cfg], tn = (B->rows + cols_of[cfg] - 1) / cols_of[cfg];
+        if (tm * tn * (alone_on_cu ? nt::Large::T : nt::Medium::T) > kMaxThreads) continue;   // (the largest tile's count is checked)
         for (int p = 1; p <= 32 && (p == 1 || (steps / p >= 4 && tm * tn * p <= kMaxJoined)); ++p) {
-            const double groups = double(tm) * tn * p, rounds = std::ceil(groups / (cfg == 0 ? kChip : 2 * kChip));
-            const double step = groups > kChip ? full[wide][cfg] : alone[wide][cfg];
-            const double cost = rounds * ((steps + p - 1) / p * step + extra[cfg] + (p > 1 ? joined[cfg] : 0.0));
+            const int64_t groups = tm * tn * p, slots = alone_on_cu ? kChip : 2 * kChip, rest = groups % slots;
+            const double beside = extra[cfg] + (p > 1 ? joined[cfg] + p * piece[cfg] : 0.0);
+            const double most = (steps + p - 1) / p * full[wide][cfg] + beside, least_of = (steps + p - 1) / p * alone[wide][cfg] + beside;
+            const double cost = double(groups / slots) * most + (rest > slots / 2 ? most : rest ? least_of : 0.0);
             if (cost < 0.97 * least) {
                 least = cost;
                 best = {cfg, int(tm), int(tn), p, 0, 0};
                 if (p > 1) {
                     best.counts = cp_align_up(size_t(tm * tn) * sizeof(int), 256);
-                    best.parts = size_t(tm * tn * p) * edge * edge * sizeof(float);
+                    best.parts = size_t(tm * tn * p) * rows_of[cfg] * cols_of[cfg] * sizeof(float);
                 }
             }
         }
@@ -542,13 +558,15 @@ __global__ void __launch_bounds__(256) k_zero(int *p, int n) {
 template <int FA, int FB, bool COMMON, bool WIDE>
 void launch_product(cp_ctx *ctx, const Product &p, const Form &f) {
     const int n = f.tiles_m * f.tiles_n * f.pieces;
-    if (f.cfg == 3) {
+    if (f.cfg == 4) {
         if (p.M <= 16) k_matmul_blocks_rows<1, FA, FB, COMMON, WIDE><<<(p.N + 15) / 16, 512, 0, ctx->stream>>>(p);
         else k_matmul_blocks_rows<2, FA, FB, COMMON, WIDE><<<(p.N + 15) / 16, 512, 0, ctx->stream>>>(p);
         return;
     }
-    if constexpr (!WIDE)   // the widened fragments of 256 x 256 do not fit into registers
+    if constexpr (!WIDE) {   // the widened fragments of 256 x 256 do not fit into registers
         if (f.cfg == 0) return (void)(k_matmul_blocks<nt::Large, FA, FB, COMMON, WIDE><<<n, nt::Large::T, 0, ctx->stream>>>(p));
+        if (f.cfg == 3) return (void)(k_matmul_blocks<nt::Flat, FA, FB, COMMON, WIDE><<<n, nt::Flat::T, 0, ctx->stream>>>(p));
+    }
     if (f.cfg <= 1) k_matmul_blocks<nt::Medium, FA, FB, COMMON, WIDE><<<n, nt::Medium::T, 0, ctx->stream>>>(p);
     else k_matmul_blocks<nt::Small, FA, FB, COMMON, WIDE><<<n, nt::Small::T, 0, ctx->stream>>>(p);
 }

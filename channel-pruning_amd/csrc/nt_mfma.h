@@ -13,8 +13,13 @@
 //
 // STAGES LDS stages, each in its own __shared__ array so that the compiler can tell a load into one from reads of the others
 // (and inserts no wait between them); one barrier per K step, behind which the loads of a step STAGES - 1 ahead are issued.
-// A tile that fills the chip alone needs two stages (a step of 256 x 256 takes 2000 cycles); few small tiles are bound by the
-// latency of their loads (0.8 us from a cold L2) and take more.
+// A tile that fills the chip alone needs two stages (a step of 256 x 256 takes 3500 cycles, a load from a cold L2 2000); small
+// tiles take four.  128 x 128 with four stages and one workgroup to a CU instead of two with two: no faster where tiles are few
+// (8-bit 5000 x 512 x 4005: 28.1 against 29.4 us), slower where there are many (20000 x 4005 x 512: 152 against 109).
+//
+// What bounds it: the matrix instructions.  A 256 x 256 step of fp16 takes 1.55-1.7 us with its loads, 1.49 without any (1440
+// TFLOP/s of the chip, which lowers its clock under such a load; a large library product reaches 1570-1590), the loads alone
+// 0.96.  128 x 128 takes 0.52 (a third more for its part of 256 x 256: the same LDS reads feed half the products), 64 x 64 0.18.
 //
 // A tile with a long k and few tiles beside it is cut into pieces of k (their number follows from the product's shape alone)
 // that several workgroups form; the one that arrives last adds them in the order of k.  The result does not depend on who
@@ -116,9 +121,10 @@ struct Tile {
     static constexpr int BM = BM_, BN = BN_, NWM = NWM_, NWN = NWN_, STAGES = STAGES_;
     static constexpr int T = 64 * NWM * NWN, WI = BM / NWM / 16, WJ = BN / NWN / 16;
     static constexpr int STAGE = (BM + BN) * 128, LOADS = STAGE / 16 / T;
-    static constexpr int PARTS = WI >= 8 ? 4 : 1;
+    static constexpr int PARTS = WI >= 6 ? 4 : 1;
 };
 typedef Tile<256, 256, 2, 4, 2> Large;    // 132 KB of LDS, one workgroup to a CU
+typedef Tile<192, 256, 2, 4, 2> Flat;     // 112 KB, one: where tiles of 256 leave many CUs idle
 typedef Tile<128, 128, 2, 2, 2> Medium;   // 64 KB, two
 typedef Tile<64, 64, 2, 2, 4> Small;      // 64 KB, two
 
@@ -154,7 +160,8 @@ __device__ __forceinline__ int frag_off(int lane, int h) { return (lane & 15) * 
 
 // A step's products.  A row group's fragments are read one group ahead of their use, and the next step's loads are issued
 // among the products (`between`): the barriers of the compiler's scheduler keep both where they stand, or it gathers the reads
-// at the top of the step, where both waves of a SIMD then wait for them at once (1.7 us instead of ... a 256 x 256 step).
+// at the top of the step, where both waves of a SIMD then wait for them at once (4096 x 16384 times 4096^2 in fp16: 480 us with
+// them, 568 without).
 #define NT_STAY() __builtin_amdgcn_sched_barrier(0)
 
 template <int WI, int WJ, bool SPLIT, class Between>
@@ -353,20 +360,21 @@ __device__ __forceinline__ bool join(f4 (&acc)[WI][WJ], int piece, int n, float 
 
 // ---- results ---------------------------------------------------------------------------------------------------------------
 // A lane's accumulators are four numbers of one row: written from there, a row gets 32 or 64 bytes at a time, which costs twice
-// what whole lines cost.  So a wave passes its part of the tile through the LDS that the stages have left (16 KB a wave, its
+// what whole lines cost.  So a wave passes its part of the tile through the LDS that the stages have left (12 or 16 KB a wave, its
 // own: no barrier), up to 64 x 64 float32 at a time, and reads it back as eight neighbours of a row or of a column.  The
 // 16-byte chunks of row r lie at chunk ^ key(r), so that writes and both kinds of reads hit all banks evenly.
 template <int WI, int WJ>
 struct Patch {
-    static constexpr int COLS = WJ * 16, ROWS = WI < 4 ? WI * 16 : 64, PASSES = WI * 16 / ROWS;
+    static constexpr int COLS = WJ * 16, ROWS = WI % 4 == 0 ? 64 : WI % 3 == 0 ? 48 : WI * 16, PASSES = WI * 16 / ROWS;
+    static constexpr int EACH_WAVE = ROWS * COLS * 4 <= 12288 ? 12288 : 16384;   // bytes of LDS
     static constexpr int EIGHTS = ROWS * COLS / 512;   // groups of eight numbers to a lane
-    static_assert(ROWS * COLS * 4 <= 16384, "");
+    static_assert(ROWS * COLS * 4 <= EACH_WAVE && ROWS * PASSES == WI * 16 && ROWS * COLS % 512 == 0, "");
     char *lds;
     int lane;
     template <class CFG>
     __device__ __forceinline__ static Patch of(char *const (&st)[8], int wave, int lane) {
         constexpr int EACH = CFG::NWM * CFG::NWN / CFG::STAGES;
-        static_assert(CFG::STAGE >= EACH * 16384, "");
+        static_assert(CFG::STAGE >= EACH * EACH_WAVE, "");
         typedef __attribute__((address_space(3))) char *Lds;
         uint32_t from = 0;
 #pragma unroll
@@ -375,7 +383,7 @@ struct Patch {
             asm("" : "+s"(s));   // (the compiler would look these up in a table, which it cannot place)
             from = wave / EACH == k ? s : from;
         }
-        return {(char *)(Lds(uintptr_t(from + wave % EACH * 16384))), lane};
+        return {(char *)(Lds(uintptr_t(from + wave % EACH * EACH_WAVE))), lane};
     }
     __device__ __forceinline__ static void order() {   // a wave's LDS accesses run in order: only the compiler has to be told
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");

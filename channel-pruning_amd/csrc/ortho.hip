@@ -164,6 +164,7 @@ struct Inverse {
 };
 
 // ---- |U|_F, and the momentum: one pass over G (and M), bound by HBM -----------------------------------------------------------
+// (12.8 M numbers, G and M float32: 28.5 us for 153 MB, 5.4 TB/s; 67 M in bfloat16: 39 us for 134 MB.)
 // A workgroup sums rows_per rows of a chunk of `width` columns; the partial sums are added in one order by whoever needs the
 // norm.  Contiguous matrices are one row: their own rows' lengths would leave most of them unaligned.
 __global__ void __launch_bounds__(256) k_ortho_norm(Jobs js, Table t, float momentum, int nesterov, int *counts, int n_counts) {
@@ -278,6 +279,7 @@ __device__ __forceinline__ void load8(const char *row, int k, float (&v)[8]) {
 }
 
 // ---- X = U / (|U|_F + eps) in both orientations, zero in the padding: one 64 x 64 tile of G to a workgroup --------------------
+// Bound by HBM: 4096 x 16384 in bfloat16 90 us for 403 MB, 12.8 M numbers in float32 40 us for 204 MB.
 // sixteen numbers of a tile's row
 __device__ __forceinline__ void load_tile(const void *p, int dtype, int64_t ld, const Job &j, int r, int c, float (&v)[16]) {
     float a[8] = {}, b[8] = {};
@@ -335,6 +337,10 @@ __global__ void __launch_bounds__(256) k_ortho_load(Table tab, float momentum, i
 }
 
 // ---- the products ------------------------------------------------------------------------------------------------------------
+// All jobs' tiles of one of a step's three products in one launch.  Bound by the matrix instructions where matrices are large (4096 x
+// 16384 in fp16: first product 305 us, 0.90 PFLOP/s of the half that is formed -- 136 tiles of 256 x 256 divide badly over 256
+// CUs --, second 110, third 480, 1.15 PFLOP/s), by a launch's fixed costs where they are many and small (the 40 layers of a
+// pruned resnet50, 8.5 M numbers: 14, 8 and 23 us).
 struct Factors {
     float acc, a, diag;   // what the accumulator, A's entry and the diagonal count for in the result
     float keep;           // LAST: 1 - lr * weight_decay (cp_ortho_step)
@@ -471,7 +477,9 @@ __global__ void __launch_bounds__(CFG::T) k_ortho_product(Table tab, Factors f, 
 
 // ---- small matrices: the whole step in one workgroup ---------------------------------------------------------------------------
 // Where the short side fits 64 rows and the long side the registers of eight waves, seventeen launches of 4.3 us each do 1 us
-// of arithmetic.  Here a workgroup keeps X in registers from the first product to the last.
+// of arithmetic.  Here a workgroup keeps X in registers from the first product to the last (64 x 576 in bfloat16: 30 us, of which
+// 3.3 a step; 73 with the launches above).  Bound by the latency of a step's chain: a product, a sum over the waves through LDS, a
+// product of 64 x 64, a product.
 // A wave owns CT tiles of 16 columns, in the two forms that the matrix instruction's operands need: by columns (lane: column
 // j, eight rows; K = rows, for B X) and by rows (lane: row i, eight columns; K = columns, for X X^T).  The result of a product
 // IS such an operand (lane: column, four consecutive rows; or, with the operands exchanged, row and four columns) once K's
@@ -1051,7 +1059,7 @@ int pieces_of(const Job &j, int phase, bool split) {
 
 bool choose(Class &cl, int phase, Choice &best) {
     double least = 1e300;
-    const int forced = cp_knob(CP_KNOB_NT_TILE);
+    const int forced = cp_knob(CP_KNOB_NT_TILE) % 4;   // (it has no Flat)
     for (int cfg = 0; cfg < 3; ++cfg) {
         if (forced && forced - 1 != cfg) continue;
         int64_t groups = 0, total = 0, longest = 0;
