@@ -1,4 +1,5 @@
 // Matrices held in 8-bit floating point with one scale per block of 128 (cp_blocks), the cast that makes them and their product.
+#include <algorithm>
 #include <cfloat>
 #include <cmath>
 
@@ -413,8 +414,9 @@ __global__ void __launch_bounds__(CFG::T) k_matmul_blocks(Product p) {
 
 // Few rows of A: bound by reading B once.  A workgroup takes sixteen rows of B and its eight waves an eighth of k each, straight
 // from memory into the matrix instruction's registers (a lane holds 32 bytes of one row: the K order within a block is the same
-// for A and B, and that is all that a sum needs); their sums are added in the order of k.  Up to 32 rows: one row by 4096 x 4096
-// takes 5 us (17 MB), a call of it 7.3 (17 rows: 7.5; 64 x 64 tiles 12, 128 x 128 18).
+// for A and B, and that is all that a sum needs); their sums are added in the order of k.  Up to 80 rows, while the tiles' launch
+// costs more (form_of): one row by 4096 x 4096 takes 5.6 us (17 MB), a call of it 7.3 -- in 64 x 64 tiles, most of whose rows
+// would be padding, 12.
 template <int MT, int FA, int FB, bool COMMON, bool WIDE>
 __global__ void __launch_bounds__(512) k_matmul_blocks_rows(Product p) {
     __shared__ alignas(16) float sum[8][MT][64][4];
@@ -436,7 +438,7 @@ __global__ void __launch_bounds__(512) k_matmul_blocks_rows(Product p) {
     f4 acc[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[m] = f4{0.f, 0.f, 0.f, 0.f};
-    constexpr int U = MT == 1 ? 4 : 2;   // blocks whose loads are under way together
+    constexpr int U = MT == 1 ? 4 : MT == 2 ? 2 : 1;   // blocks whose loads are under way together
     for (int k = k0; k < k1; k += U) {
         nt::i4v qb[U][2], qa[U][MT][2];
         float sj[U][4], si[U][MT];
@@ -511,6 +513,7 @@ struct Form {
     size_t counts, parts;   // bytes
 };
 constexpr int kMaxJoined = 16384;   // workgroups of a launch that joins pieces
+constexpr int kFewRows = 80;         // of A, for k_matmul_blocks_rows
 constexpr int kChip = 256;          // CUs that a split is planned for
 
 Form form_of(const cp_blocks *A, const cp_blocks *B, int c_dtype) {
@@ -524,9 +527,19 @@ Form form_of(const cp_blocks *A, const cp_blocks *B, int c_dtype) {
     const int64_t steps = (A->cols + 127) / 128;
     const bool wide = wide_form(c_dtype);
     Form best = {};
-    const int forced = cp_knob(CP_KNOB_NT_TILE);
-    if (A->rows <= 32 && B->rows <= kMaxThreads / 512 * 16 && !forced) return {4, 0, 0, 1, 0, 0};
+    const bool few = A->rows <= kFewRows && B->rows <= kMaxThreads / 512 * 16;
+    int forced = cp_knob(CP_KNOB_NT_TILE);
+    if (forced == 5 && !few) forced = 0;
     double least = 1e300;
+    if (few && (!forced || forced == 5)) {
+        // sixteen rows of B to a workgroup: rounds of 256, each a part of a us per step.  77 x 1000 x 2048 in float32: 8.4 us, 9.5 in
+        // tiles; 64 x 4096 x 8192: 21.5, 16; 32 x 4096 x 4096 in bfloat16: 8.6, 10.4
+        best = {4, 0, 0, 1, 0, 0};
+        least = double((B->rows + 4095) / 4096) * steps * (0.07 + 0.0032 * A->rows) + 1.0;
+        // (no tile costs less than a 64 x 64 one in one piece, or in pieces of four steps)
+        const double one = std::min(steps * alone[wide][2], 4 * alone[wide][2] + joined[2] + 2 * piece[2]);
+        if (forced || least <= extra[2] + one) return best;
+    }
     for (int cfg = 0; cfg < 4; ++cfg) {
         const bool alone_on_cu = cfg == 0 || cfg == 3;
         if (wide && alone_on_cu) continue;
@@ -559,8 +572,11 @@ template <int FA, int FB, bool COMMON, bool WIDE>
 void launch_product(cp_ctx *ctx, const Product &p, const Form &f) {
     const int n = f.tiles_m * f.tiles_n * f.pieces;
     if (f.cfg == 4) {
-        if (p.M <= 16) k_matmul_blocks_rows<1, FA, FB, COMMON, WIDE><<<(p.N + 15) / 16, 512, 0, ctx->stream>>>(p);
-        else k_matmul_blocks_rows<2, FA, FB, COMMON, WIDE><<<(p.N + 15) / 16, 512, 0, ctx->stream>>>(p);
+        const int n = (p.N + 15) / 16;
+        if (p.M <= 16) k_matmul_blocks_rows<1, FA, FB, COMMON, WIDE><<<n, 512, 0, ctx->stream>>>(p);
+        else if (p.M <= 32) k_matmul_blocks_rows<2, FA, FB, COMMON, WIDE><<<n, 512, 0, ctx->stream>>>(p);
+        else if (p.M <= 64) k_matmul_blocks_rows<4, FA, FB, COMMON, WIDE><<<n, 512, 0, ctx->stream>>>(p);
+        else k_matmul_blocks_rows<5, FA, FB, COMMON, WIDE><<<n, 512, 0, ctx->stream>>>(p);
         return;
     }
     if constexpr (!WIDE) {   // the widened fragments of 256 x 256 do not fit into registers

@@ -1059,7 +1059,7 @@ int pieces_of(const Job &j, int phase, bool split) {
 
 bool choose(Class &cl, int phase, Choice &best) {
     double least = 1e300;
-    const int forced = cp_knob(CP_KNOB_NT_TILE) % 4;   // (it has no Flat)
+    const int knob = cp_knob(CP_KNOB_NT_TILE), forced = knob > 3 ? 0 : knob;   // (the others are the 8-bit products')
     for (int cfg = 0; cfg < 3; ++cfg) {
         if (forced && forced - 1 != cfg) continue;
         int64_t groups = 0, total = 0, longest = 0;

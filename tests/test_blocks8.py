@@ -204,7 +204,7 @@ def check_product(ctx, m, n, k, fa="e4m3", fb="e4m3", ta=1, tb=128, out="f32", b
     return C
 
 
-@pytest.fixture(params=[0, 1, 2, 3, 4])
+@pytest.fixture(params=[0, 1, 2, 3, 4, 5])
 def tile_shape(request, ctx):
     """Every shape of tile in turn (0: the library's choice)."""
     ctx.lib.cp_debug_knob(3, request.param)
