@@ -532,7 +532,7 @@ Form form_of(const cp_blocks *A, const cp_blocks *B, int c_dtype) {
     if (forced == 5 && !few) forced = 0;
     double least = 1e300;
     if (few && (!forced || forced == 5)) {
-        // sixteen rows of B to a workgroup: rounds of 256, each a part of a us per step.  77 x 1000 x 2048 in float32: 8.4 us, 9.5 in
+        // sixteen rows of B to a workgroup: rounds of 256, each a part of a us per step.  77 x 1000 x 2048 in float32: 8.1 us, 9.5 in
         // tiles; 64 x 4096 x 8192: 21.5, 16; 32 x 4096 x 4096 in bfloat16: 8.6, 10.4
         best = {4, 0, 0, 1, 0, 0};
         least = double((B->rows + 4095) / 4096) * steps * (0.07 + 0.0032 * A->rows) + 1.0;
