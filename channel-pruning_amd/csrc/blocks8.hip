@@ -356,8 +356,8 @@ __device__ __forceinline__ void write_c(const Product &p, const f4 (&acc)[WI][WJ
 // factor and a fused add for every number of the tile: bound by both together.  8192^3, every row with its own scales: 527 us, 2.09
 // PFLOP/s (a library product without any scales 358); common scales, 20000 x 512 x 4005: 67 us, 1.22 (its
 // 80 MB come from HBM one step ahead of their use).  WIDE (float32 and fp16 results):
-// the operands are widened in registers, 128 conversions to 64 matrix instructions of a wave, which cost as much again
-// (512 x 4005 x 20000: 112 us, 0.73 PFLOP/s); 256 x 256 tiles would need more registers than there are.
+// the operands are widened in registers and go through the fp16 instructions, twice as many: 512 x 4005 x 20000, 112 us, 0.73
+// PFLOP/s (104 if the conversions cost nothing); 256 x 256 tiles would need more registers than there are.
 template <class CFG, int FA, int FB, bool COMMON, bool WIDE>
 __global__ void __launch_bounds__(CFG::T) k_matmul_blocks(Product p) {
     constexpr int BM = CFG::BM, BN = CFG::BN, T = CFG::T, WI = CFG::WI, WJ = CFG::WJ;

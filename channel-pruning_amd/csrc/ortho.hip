@@ -477,7 +477,7 @@ __global__ void __launch_bounds__(CFG::T) k_ortho_product(Table tab, Factors f, 
 
 // ---- small matrices: the whole step in one workgroup ---------------------------------------------------------------------------
 // Where the short side fits 64 rows and the long side the registers of eight waves, seventeen launches of 4.3 us each do 1 us
-// of arithmetic.  Here a workgroup keeps X in registers from the first product to the last (64 x 576 in bfloat16: 30 us, of which
+// of arithmetic.  Here a workgroup keeps X in registers from the first product to the last (64 x 576 in bfloat16: 29 us, of which
 // 3.3 a step; 73 with the launches above).  Bound by the latency of a step's chain: a product, a sum over the waves through LDS, a
 // product of 64 x 64, a product.
 // A wave owns CT tiles of 16 columns, in the two forms that the matrix instruction's operands need: by columns (lane: column
@@ -580,11 +580,30 @@ __global__ void __launch_bounds__(64 * kSmallWaves) k_ortho_small(SmallJobs js) 
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[k][e] = float(q[e]);
             }
+            if constexpr (sizeof(V) > 16) return;   // (float32 needs no conversion, for which each load would be waited for)
+            if (j.cols < 8) return;
+            // the rows' last eight, of which the units have had some
+            const int had = -j.cols & 7;
+#pragma unroll
+            for (int k = UNITS; k < UNITS + ENDS; ++k) {
+                int r, c;
+                const bool in = place(k, r, c);
+                V q = {};
+                if (in) __builtin_memcpy(&q, static_cast<const char *>(p) + (r * ld + j.cols - 8) * int(sizeof(V) / 8), sizeof(V));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    v[k][e] = 0.f;
+#pragma unroll
+                    for (int h = 1; h < 8; ++h)
+                        if (e + h < 8) v[k][e] = had == h ? float(q[e + h]) : v[k][e];
+                }
+            }
         };
         typedef float f8 __attribute__((ext_vector_type(8)));
         if (dtype == CP_F32) whole(f8());
         else if (dtype == CP_BF16) whole(nt::b8());
         else whole(h8());
+        if (j.cols >= 8 && dtype != CP_F32) return;
 #pragma unroll
         for (int k = UNITS; k < UNITS + ENDS; ++k) {
             int r, c;
@@ -813,33 +832,43 @@ __global__ void __launch_bounds__(64 * kSmallWaves) k_ortho_small(SmallJobs js) 
         __syncthreads();
         constexpr int FOURS = RO * (CO / 4) / T, AT_ONCE = FOURS % 4 ? 2 : 4;   // of a thread; W's loads that are under way at once
         static_assert(RO * (CO / 4) % T == 0 && FOURS % AT_ONCE == 0, "");
-        for (int i0 = 0; i0 < FOURS; i0 += AT_ONCE) {
-            f4 v[AT_ONCE], w[AT_ONCE];
-            int row[AT_ONCE], col[AT_ONCE];
+        auto write = [&](auto type) {
+            typedef decltype(type) V;   // four numbers, at any element's address
+            for (int i0 = 0; i0 < FOURS; i0 += AT_ONCE) {
+                f4 v[AT_ONCE];
+                V w[AT_ONCE];
+                int row[AT_ONCE], col[AT_ONCE];
 #pragma unroll
-            for (int q = 0; q < AT_ONCE; ++q) {
-                const int i = (i0 + q) * T + tid, r = i / (CO / 4), c = i % (CO / 4) * 4;
-                // place in the long side: wave's tiles of this half
-                const int l = TALL ? r : c, at = (l / (CT * 8) * CT + half * (CT / 2)) * 16 + l % (CT * 8);
-                row[q] = TALL ? at : r;
-                col[q] = TALL ? c : at;
-                v[q] = *reinterpret_cast<const f4 *>(&os[r][c]);
-                if (j.M && row[q] < j.rows && col[q] + 4 <= j.cols) w[q] = load4_as_float(j.out, j.o_dtype, row[q] * j.ldo + col[q]);
-            }
+                for (int q = 0; q < AT_ONCE; ++q) {
+                    const int i = (i0 + q) * T + tid, r = i / (CO / 4), c = i % (CO / 4) * 4;
+                    // place in the long side: wave's tiles of this half
+                    const int l = TALL ? r : c, at = (l / (CT * 8) * CT + half * (CT / 2)) * 16 + l % (CT * 8);
+                    row[q] = TALL ? at : r;
+                    col[q] = TALL ? c : at;
+                    v[q] = *reinterpret_cast<const f4 *>(&os[r][c]);
+                    w[q] = V{};
+                    if (j.M && row[q] < j.rows && col[q] + 4 <= j.cols)
+                        w[q] = take_from<V>(static_cast<const char *>(j.out) + (row[q] * j.ldo + col[q]) * int(sizeof(V) / 4));
+                }
 #pragma unroll
-            for (int q = 0; q < AT_ONCE; ++q) {
-                if (row[q] >= j.rows || col[q] >= j.cols) continue;
-                const int64_t to = row[q] * j.ldo + col[q];
-                if (col[q] + 4 <= j.cols) {
-                    store4_as(j.out, j.o_dtype, to, j.M ? w[q] * js.keep - v[q] * j.lr : v[q]);
-                } else {
-                    for (int e = 0; col[q] + e < j.cols; ++e) {
-                        const float o = e == 0 ? v[q][0] : e == 1 ? v[q][1] : v[q][2];
-                        store_as(j.out, j.o_dtype, to + e, j.M ? js.keep * load_as_float(j.out, j.o_dtype, to + e) - j.lr * o : o);
+                for (int q = 0; q < AT_ONCE; ++q) {
+                    if (row[q] >= j.rows || col[q] >= j.cols) continue;
+                    const int64_t to = row[q] * j.ldo + col[q];
+                    if (col[q] + 4 <= j.cols) {
+                        const f4 o = j.M ? __builtin_convertvector(w[q], f4) * js.keep - v[q] * j.lr : v[q];
+                        put_to<V>(static_cast<char *>(j.out) + to * int(sizeof(V) / 4), __builtin_convertvector(o, V));
+                    } else {
+                        for (int e = 0; col[q] + e < j.cols; ++e) {
+                            const float o = e == 0 ? v[q][0] : e == 1 ? v[q][1] : v[q][2];
+                            store_as(j.out, j.o_dtype, to + e, j.M ? js.keep * load_as_float(j.out, j.o_dtype, to + e) - j.lr * o : o);
+                        }
                     }
                 }
             }
-        }
+        };
+        if constexpr (!SPLIT) write(nt::b4u());   // (pairs are there for the two other types)
+        else if (j.o_dtype == CP_F32) write(nt::f4u());
+        else write(nt::h4u());
     }
 }
 
