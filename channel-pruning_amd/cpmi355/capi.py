@@ -465,6 +465,8 @@ class Context:
         self._check(self.lib.cp_sync(self.h), "cp_sync")
 
     def set_stream(self, stream_ptr):
+        """Run on a caller's stream; 0 or None: the context's own, which torch's work does not wait for, nor it for torch's.
+        In order with torch: set_stream(torch.cuda.current_stream().cuda_stream or 1) -- 1 is the legacy default stream."""
         self._check(self.lib.cp_ctx_set_stream(self.h, stream_ptr), "cp_ctx_set_stream")
 
     # -- hot path -------------------------------------------------------------------

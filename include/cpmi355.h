@@ -64,7 +64,8 @@ int cp_ctx_destroy(cp_ctx *ctx);
  * contexts of cp_prune_layers.  Destroy it before `of`. */
 int cp_ctx_create_sibling(cp_ctx *of, cp_ctx **out);
 /* run on a caller-owned hipStream_t (e.g. torch.cuda.current_stream().cuda_stream);
- * NULL restores the ctx's own stream. */
+ * NULL restores the ctx's own stream, which no other stream waits for.  The legacy default stream, which torch uses unless
+ * told otherwise and gives as 0, is hipStreamLegacy (1). */
 int cp_ctx_set_stream(cp_ctx *ctx, void *hip_stream);
 int cp_sync(cp_ctx *ctx);
 

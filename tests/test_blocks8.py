@@ -338,6 +338,13 @@ def test_product_on_other_streams_and_contexts(ctx):
             ctx.matmul_blocks(A.b, B.b, c.ptr, 0)
         for c in outs:
             assert np.array_equal(c.raw(), want)
+    ctx.set_stream(1)                                                     # the legacy default stream
+    for c in outs:
+        ctx.to_device(c.before, c.buf)
+        ctx.matmul_blocks(A.b, B.b, c.ptr, 0)
+        assert np.array_equal(c.raw(), want)
+    ctx.sync()
+    ctx.set_stream(None)
     del A2, B2, outs2, c, d
     two.close()
 
