@@ -6,8 +6,12 @@
 //
 // Numbers.  Singular values stay in [0, u_k] with bounds u_k that the host derives from the coefficients, so every entry of X,
 // A and B is bounded too, and a power of two per step and matrix puts that bound at 2^14: fp16's whole range is used, with
-// headroom of four.  fp16 then holds 11 bits of an entry where bf16 would hold 8, at the same rate.  Results of 24 or 11 bits
-// carry a pair of fp16 (22 bits) and three products instead of one; the pair's dropped low * low term is below its rounding.
+// headroom of four.  Numbers are carried as pairs of fp16 (22 bits) and three products instead of one; the pair's dropped
+// low * low term is below its rounding.  Only where G and the result are both bf16 they are one fp16 each (11 bits, where bf16
+// would hold 8, at the same rate): a step amplifies what is lost in a small singular direction up to 3.44 times, so that the
+// 11 bits cost 0.5, 4 and 7 % of O where a rank-4 part is 10, 100 and 1000 times as strong as the rest (256 x 576) -- an eighth of
+// what G's own rounding to bf16 has cost there (3, 26 and 46 %).  float32, fp16 and the step's momentum have not lost that: they
+// get pairs (3e-5 in the worst of these), whatever the result's type.
 // Sums are float32 in the accumulators, |U|_F is summed in float64.
 #include <algorithm>
 #include <cmath>
@@ -866,7 +870,7 @@ __global__ void __launch_bounds__(64 * kSmallWaves) k_ortho_small(SmallJobs js) 
                 }
             }
         };
-        if constexpr (!SPLIT) write(nt::b4u());   // (pairs are there for the two other types)
+        if (!SPLIT || j.o_dtype == CP_BF16) write(nt::b4u());
         else if (j.o_dtype == CP_F32) write(nt::f4u());
         else write(nt::h4u());
     }
@@ -1013,7 +1017,8 @@ int check_requests(cp_ctx *ctx, const std::vector<Request> &rq, bool step, bool 
     return CP_OK;
 }
 
-bool is_split(const Request &r) { return r.o_dtype != CP_BF16; }
+// whether a job's numbers are carried as pairs: see the head of this file
+bool is_split(const Request &r) { return r.M || r.g_dtype != CP_BF16 || r.o_dtype != CP_BF16; }
 
 int64_t padded(int64_t v) { return (v + kPad - 1) / kPad * kPad; }
 

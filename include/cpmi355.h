@@ -293,8 +293,9 @@ int cp_matmul_blocks_workspace(const cp_blocks *A, const cp_blocks *B, int c_dty
  *   X = G / (|G|_F + eps);   `steps` times  X <- a X + b (X X^T) X + c (X X^T)^2 X
  * coef HOST [steps][3] = (a, b, c) per step, or NULL: (3.4445, -4.7750, 2.0315), which brings singular values into about
  * [0.7, 1.2].  G DEVICE [rows, cols] (g_dtype F32, BF16 or F16, row stride ldg), O DEVICE [rows, cols] (o_dtype likewise; may
- * be G itself).  All jobs of a call run in common launches.  Products are carried with 22 bits of mantissa where the result
- * is F32 or F16 and with 11 where it is BF16 (8), sums in float32, the norm in float64.  G = 0 gives O = 0; a NaN or an
+ * be G itself).  All jobs of a call run in common launches.  Products are carried with 22 bits of mantissa, or with 11
+ * where both G and O are BF16 (8) -- an eighth of what G's own rounding costs; O as F32 gives 22 --, sums in float32, the norm
+ * in float64.  G = 0 gives O = 0; a NaN or an
  * infinity in G makes that job's O NaN.  coef must keep |x| <= 1 below 16 in every step (checked), steps 1..32.  The shorter
  * side is at most 65536, the longer 2^20.  Outputs of a call must not overlap each other; an output may be another job's G (all
  * are read first).  The order of a job's sums depends on its shape and types, and, where its short side is at most 64, on
@@ -312,7 +313,7 @@ int cp_orthogonalise_workspace(int n_jobs, const cp_ortho_job *jobs, int steps, 
 /* One optimiser step on a set of layers' weights:
  *   M <- momentum M + G;   U = nesterov ? G + momentum M : M;   W <- (1 - lr weight_decay) W - lr gamma O(U)
  * G DEVICE (g_dtype F32, BF16 or F16), M DEVICE f32 in/out, W DEVICE (w_dtype F32, BF16 or F16) in/out, all [rows, cols];
- * gamma: the job's factor on lr (sqrt(max(1, rows / cols)) is usual).  O(U) as above, carried for W's type.  no M or W
+ * gamma: the job's factor on lr (sqrt(max(1, rows / cols)) is usual).  O(U) as above, carried with 22 bits.  No M or W
  * of a call may overlap another matrix of it (a G may serve several jobs).  Nothing is kept between calls but M. */
 typedef struct cp_ortho_step_job {
     const void *G;
