@@ -5,7 +5,7 @@ import pytest
 
 from cpmi355 import capi
 from lowbits import HALF, TYPES, Mat
-from test_ortho import distance, iterate, within
+from test_ortho import iterate, tile_shape, within  # noqa: F401
 
 gpu = pytest.mark.gpu
 
@@ -60,3 +60,103 @@ def test_step_of_an_ill_conditioned_momentum(ctx, rows, cols, top, gk, wk, neste
     want, far = distance32(U)
     moved = iterate(U + 2.0 ** -24 * (np.abs(m2) + np.abs(m) + np.abs(U)) * rs.choice([-1, 1], U.shape)) - want
     within(-W.get(), want, far + 4 * np.sqrt((moved ** 2).mean()), wk)
+
+
+# ---- a network's layers in one step --------------------------------------------------------------------------------------------
+
+
+class Layer:
+    """G, M and W of one layer on the device, and what a step has to make of them."""
+
+    def __init__(self, ctx, rs, rows, cols, gk, wk, gamma):
+        self.shape, self.gk, self.wk, self.gamma = (rows, cols), gk, wk, gamma
+        self.g = Mat(ctx, 1e-3 * dominated(rs, rows, cols, 3.0), gk, ld=cols + rs.randint(3))
+        self.m = Mat(ctx, 8e-3 * dominated(rs, rows, cols, 3.0), "f32", ld=cols + rs.randint(3), lead=rs.randint(2))
+        self.w = Mat(ctx, 0.05 * rs.randn(rows, cols), wk, ld=cols + rs.randint(3), lead=rs.randint(4))
+
+    def twin(self, ctx):
+        """The same layer in memory of its own."""
+        t = Layer.__new__(Layer)
+        t.__dict__.update(self.__dict__)
+        t.m, t.w = Mat(ctx, self.m.get(), "f32"), Mat(ctx, self.w.get(), self.wk)
+        return t
+
+    def job(self):
+        r, c = self.shape
+        return (self.g.ptr, TYPES[self.gk], r, c, self.m.ptr, self.w.ptr, TYPES[self.wk], self.gamma, self.g.ld, self.m.ld, self.w.ld)
+
+    def held(self):
+        return self.g.get(), self.m.get(), self.w.get()
+
+    def check(self, before, lr, momentum, nesterov, decay):
+        g, m, w = before
+        gamma = max(1, self.shape[0] / max(self.shape[1], 1)) ** 0.5 if self.gamma is None else self.gamma
+        m2 = momentum * m + g
+        U = g + momentum * m2 if nesterov else m2
+        O, far = distance32(U)
+        # U's float32 roundings (see test_step_of_an_ill_conditioned_momentum)
+        signs = np.where((np.arange(U.size).reshape(U.shape) * 2654435761 >> 7) & 1, 1.0, -1.0)
+        moved = iterate(U + 2.0 ** -24 * (np.abs(m2) + np.abs(m) + np.abs(U)) * signs) - O
+        far = abs(lr * gamma) * (far + 4 * np.sqrt((moved ** 2).mean()))
+        want = (1 - lr * decay) * w - lr * gamma * O
+        assert (np.abs(self.m.get() - m2) <= 2.0 ** -24 * (np.abs(m2) + np.abs(m)) + 1e-30).all()
+        # W: two float32 factors (each off by half a step), a product and a fused multiply-add, and the type's rounding
+        slack = 4 * 2.0 ** -24 * (np.abs(w) + np.abs(want)) + HALF[self.wk] * np.abs(want) + 2.0 ** -25
+        err = np.abs(self.w.get() - want)
+        assert (err <= 12 * far + slack).all() and np.sqrt((err ** 2).mean()) <= far + np.sqrt((slack ** 2).mean()), self.shape
+        assert self.m.untouched() and self.w.untouched() and np.array_equal(self.g.raw(), self.g.before)
+
+
+@gpu
+@pytest.mark.parametrize("rows,cols", [(130, 140), (140, 130), (70, 700), (700, 70), (300, 520), (520, 300)])
+@pytest.mark.parametrize("gk,wk", [("f32", "f32"), ("bf16", "bf16"), ("f32", "bf16"), ("f16", "f16")])
+def test_step_in_every_tile_shape(ctx, tile_shape, rows, cols, gk, wk):
+    layer = Layer(ctx, np.random.RandomState(rows + cols), rows, cols, gk, wk, None)
+    jobs = capi.OrthoStepJobs([layer.job()])
+    for nesterov in (True, False):
+        before = layer.held()
+        ctx.ortho_step(jobs, 0.02, nesterov=nesterov, weight_decay=0.1)
+        layer.check(before, 0.02, 0.95, nesterov, 0.1)
+
+
+def run_together(ctx, layers, alone):
+    """Two steps on all layers in one call, each against float64; `alone(layer)`: and against a call of its own, bit for bit."""
+    twins = [(a, a.twin(ctx)) for a in layers if alone(a)]
+    jobs = capi.OrthoStepJobs([a.job() for a in layers])
+    for _ in range(2):
+        before = [a.held() for a in layers]
+        ctx.ortho_step(jobs, 0.02, weight_decay=0.1)
+        for a, b in zip(layers, before):
+            if a.w.rows and a.w.cols:
+                a.check(b, 0.02, 0.95, True, 0.1)
+    for a, t in twins:
+        one = capi.OrthoStepJobs([(a.g.ptr, TYPES[a.gk], *a.shape, t.m.ptr, t.w.ptr, TYPES[a.wk], a.gamma, a.g.ld, t.m.ld, t.w.ld)])
+        for _ in range(2):
+            ctx.ortho_step(one, 0.02, weight_decay=0.1)
+        assert np.array_equal(a.m.get(), t.m.get()) and np.array_equal(a.w.get(), t.w.get()), a.shape
+
+
+@gpu
+@pytest.mark.parametrize("seed", [0, 1])
+def test_step_of_a_network(ctx, seed):
+    """More layers than a launch's records, tall and wide, large and small, of all types: float32, fp16 and bfloat16 weights
+    share the call's counters and pieces."""
+    rs = np.random.RandomState(20 + seed)
+    kinds = [("f32", "f32"), ("bf16", "bf16"), ("f32", "bf16"), ("bf16", "f32"), ("f16", "f16")]
+    shapes = [(int(16 * 24 ** rs.rand()), int(16 * 32 ** rs.rand())) for _ in range(44)]
+    shapes += [(70, 5000), (5000, 70), (1, 1), (400, 400), (1, 300), (300, 1)]
+    layers = [Layer(ctx, rs, *s, *kinds[i % 5], None if i % 3 else 0.7) for i, s in enumerate(shapes)]
+    run_together(ctx, layers, lambda a: min(a.shape) > 64)
+
+
+@gpu
+def test_step_of_many_small_layers(ctx):
+    """A call of small matrices alone, more than one kernel's records of a kind."""
+    rs = np.random.RandomState(30)
+    kinds = [("f32", "f32"), ("bf16", "bf16"), ("f32", "bf16"), ("bf16", "f32"), ("f16", "f16")]
+    shapes = [(int(rs.randint(1, 65)), int(rs.randint(1, 513))) for _ in range(60)]
+    shapes = [s if i % 2 else s[::-1] for i, s in enumerate(shapes)] + [(64, 512), (512, 64), (64, 64), (1, 1)]
+    shapes += [(48, 200)] * 30
+    layers = [Layer(ctx, rs, *s, *kinds[i % 5], None if i % 3 else 0.7) for i, s in enumerate(shapes)]
+    assert capi.ortho_workspace(capi.OrthoStepJobs([a.job() for a in layers])) == 0
+    run_together(ctx, layers, lambda a: True)
