@@ -209,6 +209,13 @@ def _ptr(x):
     return int(x)
 
 
+def _device_ptr(x, name):
+    """_ptr of what lies on the device: host arrays and host tensors are refused."""
+    if isinstance(x, np.ndarray) or (hasattr(x, "is_cuda") and not x.is_cuda):
+        raise ValueError("%s: memory on the device is needed (a DevBuf, a torch tensor on the device or an address)" % name)
+    return _ptr(x)
+
+
 _TORCH_CODES = {}      # torch dtype -> dtype code, filled when torch is first seen
 
 
@@ -220,7 +227,7 @@ def _torch_codes():
 
 def _matrix(x, dtype, rows, cols, ld, name):
     """(pointer, row stride in elements, device index or None) of a device matrix.  A torch tensor is held to the dtype code,
-    the shape and unit column stride, and gives its own row stride; a DevBuf to its size; an int is taken as it is."""
+    the shape and unit column stride, and gives its own row stride; a DevBuf to its size; an int, a device address, is taken as it is."""
     if hasattr(x, "stride"):
         codes = _TORCH_CODES or _torch_codes()
         if codes.get(x.dtype) != dtype:
@@ -241,7 +248,7 @@ def _matrix(x, dtype, rows, cols, ld, name):
         if rows and cols and ((rows - 1) * ld + cols) * (8 if dtype == CP_F64 else 4 if dtype == CP_F32 else 2) > x.nbytes:
             raise ValueError("%s: the buffer holds %d bytes, too few for [%d, %d]" % (name, x.nbytes, rows, cols))
         return x.ptr, ld, x.ctx.device
-    return _ptr(x), ld, None
+    return _device_ptr(x, name), ld, None
 
 
 class Blocks:
@@ -277,7 +284,7 @@ class Blocks:
                     raise ValueError("%s: the buffer holds %d bytes, %d needed" % (name, b.nbytes, need))
         self.q, self.scale, self.rows, self.cols, self.fmt, self.tile = q, scale, rows, cols, fmt, tile
         self.ld, self.lds = int(ld), int(lds)
-        self.c = BlocksStruct(_ptr(q), _ptr(scale), rows, cols, self.ld, self.lds, fmt, tile)
+        self.c = BlocksStruct(_device_ptr(q, "q"), _device_ptr(scale, "scale"), rows, cols, self.ld, self.lds, fmt, tile)
         self.ref = ctypes.byref(self.c)
         rc = load().cp_blocks_check(self.ref)
         if rc != 0:
@@ -607,9 +614,17 @@ class Context:
     def _elsewhere(self, device, name):
         raise ValueError("%s is on device %d, the context on %d" % (name, device, self.device))
 
-    @staticmethod
-    def _ws(ws):
-        return (None, 0) if ws is None else (_ptr(ws), int(ws.nbytes))
+    def _ws(self, ws):
+        """(pointer, bytes) of a workspace: a DevBuf or a contiguous tensor, of this device."""
+        if ws is None:
+            return None, 0
+        p = _device_ptr(ws, "ws")
+        if not hasattr(ws, "nbytes") or (hasattr(ws, "is_contiguous") and not ws.is_contiguous()):
+            raise ValueError("ws: a DevBuf or a contiguous tensor is needed")
+        device = ws.ctx.device if isinstance(ws, DevBuf) else ws.get_device()
+        if device != self.device:
+            self._elsewhere(device, "ws")
+        return p, int(ws.nbytes)
 
     def quant_blocks(self, x, x_dtype, out=None, out_t=None, ldx=None, flags=0):
         """x [rows, cols] -> the 8-bit matrices out [rows, cols] and / or out_t [cols, rows] (Blocks), in one read of x
@@ -637,7 +652,12 @@ class Context:
                 if bias.shape != (B.rows,) or (_TORCH_CODES or _torch_codes()).get(bias.dtype) != CP_F32 or not bias.is_contiguous() \
                         or bias.get_device() != self.device:
                     raise ValueError("bias: a contiguous float32 tensor [%d] on device %d is needed" % (B.rows, self.device))
-            bias = _ptr(bias)
+            elif isinstance(bias, DevBuf):
+                if bias.ctx.device != self.device:
+                    self._elsewhere(bias.ctx.device, "bias")
+                if bias.nbytes < 4 * B.rows:
+                    raise ValueError("bias: the buffer holds %d bytes, %d needed" % (bias.nbytes, 4 * B.rows))
+            bias = _device_ptr(bias, "bias")
         w, wb = (None, 0) if ws is None else self._ws(ws)
         rc = self.lib.cp_matmul_blocks(self.h, A.ref, B.ref, bias, p, c_dtype, ldc, w, wb)
         if rc:
