@@ -671,6 +671,12 @@ class Context:
         return n.value
 
     # -- orthogonalised updates ------------------------------------------------------------------
+    def _jobs(self, jobs, kind):
+        if not isinstance(jobs, kind):       # the lists' records differ
+            raise ValueError("jobs: %s is needed, got %s" % (kind.__name__, type(jobs).__name__))
+        if jobs.device not in (None, self.device):
+            self._elsewhere(jobs.device, "a job")
+
     @staticmethod
     def _coef(coef, steps):
         if coef is None:
@@ -681,8 +687,7 @@ class Context:
     def orthogonalise(self, jobs, steps=5, coef=None, eps=1e-7, ws=None):
         """O = the Newton-Schulz approximation of G's orthogonal polar factor, for every matrix of an OrthoJobs list in common
         launches (cp_orthogonalise).  coef: (a, b, c) or one row per step; None = (3.4445, -4.7750, 2.0315)."""
-        if jobs.device not in (None, self.device):
-            self._elsewhere(jobs.device, "a job")
+        self._jobs(jobs, OrthoJobs)
         q = self._coef(coef, steps)
         w, wb = self._ws(ws)
         self._check(self.lib.cp_orthogonalise(self.h, jobs.n, jobs.c, steps, None if q is None else q.ctypes.data, eps, w, wb),
@@ -691,8 +696,7 @@ class Context:
     def ortho_step(self, jobs, lr, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coef=None, eps=1e-7, ws=None):
         """One optimiser step on every layer of an OrthoStepJobs list: momentum, orthogonalisation, decay, weights
         (cp_ortho_step).  G is read, M and W are updated."""
-        if jobs.device not in (None, self.device):
-            self._elsewhere(jobs.device, "a job")
+        self._jobs(jobs, OrthoStepJobs)
         q = self._coef(coef, steps)
         w, wb = self._ws(ws)
         self._check(self.lib.cp_ortho_step(self.h, jobs.n, jobs.c, lr, momentum, int(nesterov), weight_decay, steps,
@@ -872,6 +876,8 @@ class Context:
 
 def ortho_workspace(jobs, steps=5, coef=None, eps=1e-7):
     """Context.ortho_workspace without a context: checks the jobs like the call itself, needs no device."""
+    if not isinstance(jobs, (OrthoJobs, OrthoStepJobs)):
+        raise ValueError("jobs: OrthoJobs or OrthoStepJobs is needed, got %s" % type(jobs).__name__)
     n = ctypes.c_size_t()
     q = Context._coef(coef, steps)
     lib = load()

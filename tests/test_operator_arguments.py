@@ -95,3 +95,19 @@ def test_bias_and_workspace_are_checked(no_ctx):
     for ok in (dict(), dict(bias=Buf(28)), dict(bias=4096), dict(ws=Buf(512)), dict(ws=Tensor((512,), "torch.uint8"))):
         with pytest.raises(capi.CpError):                # through to the library, which misses the context
             product(**ok)
+
+
+# ---- lists of the other call ---------------------------------------------------------------------------------------------------
+
+
+def test_a_list_of_the_other_call_is_refused(no_ctx):
+    """The records differ: read as the other's, a stride would be taken for an address."""
+    jobs, steps = capi.OrthoJobs([(4096, 0, 5, 130, 8192, 0)]), capi.OrthoStepJobs([(4096, 0, 5, 130, 8192, 16384, 0)])
+    for bad in (steps, [(4096, 0, 5, 130, 8192, 0)], None):
+        with pytest.raises(ValueError):
+            no_ctx.orthogonalise(bad)
+    for bad in (jobs, [(4096, 0, 5, 130, 8192, 16384, 0)], None):
+        with pytest.raises(ValueError):
+            no_ctx.ortho_step(bad, 0.1)
+    with pytest.raises(ValueError):
+        capi.ortho_workspace([(4096, 0, 5, 130, 8192, 0)])
