@@ -254,7 +254,7 @@ def _matrix(x, dtype, rows, cols, ld, name):
 class Blocks:
     """A matrix [rows, cols] held in 8-bit floating point (cp_blocks): bytes q [rows, ld] and float32 scales
     [ceil(cols / 128), lds], one per 128 columns of a row (tile=1) or of 128 rows (tile=128).  q / scale: torch tensors
-    (two-dimensional: their row strides are ld / lds), DevBufs or device addresses; kept alive by this object.  The bytes of a
+    (two-dimensional: their row strides are ld / lds, whatever is given has to agree), DevBufs or device addresses; kept alive by this object.  The bytes of a
     row from cols to the next multiple of 128 have to be zero."""
 
     def __init__(self, q, scale, rows, cols, fmt, tile, ld=None, lds=None):
@@ -273,10 +273,8 @@ class Blocks:
             if self.device not in (None, t.device.index):
                 raise ValueError("q and scale are on different devices")
             self.device = t.device.index
-        if ld is None:
-            ld = q.stride(0) if hasattr(q, "data_ptr") and q.shape[0] > 1 else max(up, 128)
-        if lds is None:
-            lds = scale.stride(0) if hasattr(scale, "data_ptr") and scale.shape[0] > 1 else max(tall, 1)
+        ld = self._stride(q, rows, ld, max(up, 128), "ld")
+        lds = self._stride(scale, kb, lds, max(tall, 1), "lds")
         for b, name, need in ((q, "q", (rows - 1) * ld + up if rows else 0), (scale, "scale", 4 * ((kb - 1) * lds + tall) if kb else 0)):
             if isinstance(b, DevBuf):
                 self.device = b.ctx.device
@@ -290,6 +288,16 @@ class Blocks:
         if rc != 0:
             raise CpError(rc, "cp_blocks_check", "rows %d, cols %d, ld %d, lds %d, fmt %d, tile %d"
                           % (rows, cols, self.ld, self.lds, fmt, tile))
+
+    @staticmethod
+    def _stride(t, rows, given, least, name):
+        """The row stride of a tensor's `rows` rows, the given one or the least."""
+        own = t.stride(0) if hasattr(t, "data_ptr") and t.shape[0] > 1 else None
+        if given is None:
+            return least if own is None else own
+        if own is not None and rows > 1 and given != own:
+            raise ValueError("%s: %d does not fit the tensor's row stride %d" % (name, given, own))
+        return given
 
     @classmethod
     def empty(cls, ctx, rows, cols, fmt, tile):

@@ -111,3 +111,25 @@ def test_a_list_of_the_other_call_is_refused(no_ctx):
             no_ctx.ortho_step(bad, 0.1)
     with pytest.raises(ValueError):
         capi.ortho_workspace([(4096, 0, 5, 130, 8192, 0)])
+
+
+# ---- 8-bit matrices in tensors --------------------------------------------------------------------------------------------------
+
+
+def held(rows=5, cols=130, fmt=capi.CP_E4M3, tile=1, q=None, scale=None, **kw):
+    q = Tensor((rows, 256), "torch.uint8") if q is None else q
+    scale = Tensor((2, rows if tile == 1 else -(-rows // 128)), "torch.float32") if scale is None else scale
+    return capi.Blocks(q, scale, rows, cols, fmt, tile, **kw)
+
+
+def test_strides_have_to_be_the_tensors():
+    """A stride of the caller's that is not the tensor's reads past its memory."""
+    b = held(q=Tensor((5, 256), "torch.uint8", (512, 1)), scale=Tensor((2, 5), "torch.float32", (9, 1)))
+    assert (b.ld, b.lds) == (512, 9)
+    b = held(q=Tensor((5, 256), "torch.uint8", (512, 1)), scale=Tensor((2, 5), "torch.float32", (9, 1)), ld=512, lds=9)
+    assert (b.ld, b.lds) == (512, 9)
+    for kw in (dict(ld=512), dict(ld=384), dict(lds=6), dict(lds=1 << 20)):
+        with pytest.raises(ValueError):
+            held(**kw)
+    held(rows=1, q=Tensor((1, 256), "torch.uint8"), ld=1024)                               # one row: its stride leads nowhere
+    capi.Blocks(Tensor((5, 128), "torch.uint8"), Tensor((1, 5), "torch.float32"), 5, 100, capi.CP_E4M3, 1, lds=80)   # one block column
