@@ -251,6 +251,9 @@ def _matrix(x, dtype, rows, cols, ld, name):
     return _device_ptr(x, name), ld, None
 
 
+_FLOAT8 = {"torch.float8_e4m3fn": CP_E4M3, "torch.float8_e5m2": CP_E5M2}
+
+
 class Blocks:
     """A matrix [rows, cols] held in 8-bit floating point (cp_blocks): bytes q [rows, ld] and float32 scales
     [ceil(cols / 128), lds], one per 128 columns of a row (tile=1) or of 128 rows (tile=128).  q / scale: torch tensors
@@ -262,7 +265,7 @@ class Blocks:
         kb, up = -(-cols // 128), -(-cols // 128) * 128
         tall = rows if tile == 1 else -(-rows // 128)
         self.device = None
-        for t, name, dts, need in ((q, "q", ("torch.uint8", "torch.float8_e4m3fn", "torch.float8_e5m2"), (rows, up)),
+        for t, name, dts, need in ((q, "q", ("torch.uint8", *_FLOAT8), (rows, up)),
                                    (scale, "scale", ("torch.float32",), (kb, tall))):
             if not hasattr(t, "data_ptr"):
                 continue
@@ -273,6 +276,8 @@ class Blocks:
             if self.device not in (None, t.device.index):
                 raise ValueError("q and scale are on different devices")
             self.device = t.device.index
+        if hasattr(q, "data_ptr") and str(q.dtype) != "torch.uint8" and _FLOAT8[str(q.dtype)] != fmt:
+            raise ValueError("q: a tensor of %s does not hold fmt %r" % (q.dtype, fmt))
         ld = self._stride(q, rows, ld, max(up, 128), "ld")
         lds = self._stride(scale, kb, lds, max(tall, 1), "lds")
         for b, name, need in ((q, "q", (rows - 1) * ld + up if rows else 0), (scale, "scale", 4 * ((kb - 1) * lds + tall) if kb else 0)):

@@ -133,3 +133,12 @@ def test_strides_have_to_be_the_tensors():
             held(**kw)
     held(rows=1, q=Tensor((1, 256), "torch.uint8"), ld=1024)                               # one row: its stride leads nowhere
     capi.Blocks(Tensor((5, 128), "torch.uint8"), Tensor((1, 5), "torch.float32"), 5, 100, capi.CP_E4M3, 1, lds=80)   # one block column
+
+
+def test_types_have_to_be_the_format():
+    held(q=Tensor((5, 256), "torch.float8_e4m3fn"))
+    held(q=Tensor((5, 256), "torch.float8_e5m2"), fmt=capi.CP_E5M2)
+    for t, fmt in (("torch.float8_e4m3fn", capi.CP_E5M2), ("torch.float8_e5m2", capi.CP_E4M3), ("torch.int8", capi.CP_E4M3),
+                   ("torch.float8_e4m3fnuz", capi.CP_E4M3)):
+        with pytest.raises(ValueError):
+            held(q=Tensor((5, 256), t), fmt=fmt)
