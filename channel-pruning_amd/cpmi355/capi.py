@@ -273,16 +273,14 @@ class Blocks:
                 raise ValueError("%s: a two-dimensional device tensor of %s is needed" % (name, " / ".join(dts)))
             if t.shape[0] < need[0] or t.shape[1] < need[1] or (t.shape[1] > 1 and t.stride(1) != 1):
                 raise ValueError("%s: at least %s with unit column stride is needed, got %s" % (name, need, tuple(t.shape)))
-            if self.device not in (None, t.device.index):
-                raise ValueError("q and scale are on different devices")
-            self.device = t.device.index
+            self._on(t.device.index)
         if hasattr(q, "data_ptr") and str(q.dtype) != "torch.uint8" and _FLOAT8[str(q.dtype)] != fmt:
             raise ValueError("q: a tensor of %s does not hold fmt %r" % (q.dtype, fmt))
         ld = self._stride(q, rows, ld, max(up, 128), "ld")
         lds = self._stride(scale, kb, lds, max(tall, 1), "lds")
         for b, name, need in ((q, "q", (rows - 1) * ld + up if rows else 0), (scale, "scale", 4 * ((kb - 1) * lds + tall) if kb else 0)):
             if isinstance(b, DevBuf):
-                self.device = b.ctx.device
+                self._on(b.ctx.device)
                 if b.nbytes < need:
                     raise ValueError("%s: the buffer holds %d bytes, %d needed" % (name, b.nbytes, need))
         self.q, self.scale, self.rows, self.cols, self.fmt, self.tile = q, scale, rows, cols, fmt, tile
@@ -293,6 +291,11 @@ class Blocks:
         if rc != 0:
             raise CpError(rc, "cp_blocks_check", "rows %d, cols %d, ld %d, lds %d, fmt %d, tile %d"
                           % (rows, cols, self.ld, self.lds, fmt, tile))
+
+    def _on(self, device):
+        if self.device not in (None, device):
+            raise ValueError("q and scale are on different devices")
+        self.device = device
 
     @staticmethod
     def _stride(t, rows, given, least, name):

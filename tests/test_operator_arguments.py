@@ -142,3 +142,11 @@ def test_types_have_to_be_the_format():
                    ("torch.float8_e4m3fnuz", capi.CP_E4M3)):
         with pytest.raises(ValueError):
             held(q=Tensor((5, 256), t), fmt=fmt)
+
+
+def test_both_parts_lie_on_one_device():
+    two, three = Tensor((2, 5), "torch.float32", device=1), Buf(1 << 16, device=1)
+    assert held(q=Tensor((5, 256), "torch.uint8", device=1), scale=three).device == 1
+    for kw in (dict(scale=two), dict(scale=three), dict(q=three), dict(q=Buf(1 << 16), scale=three), dict(q=Buf(1 << 16), scale=two)):
+        with pytest.raises(ValueError):
+            held(**kw)
