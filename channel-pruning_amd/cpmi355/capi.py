@@ -322,6 +322,13 @@ class _Jobs:
         self.n, self.keep, self.device = n, [], None
         self.c = (struct * max(n, 1))()
 
+    @staticmethod
+    def _size(rows, cols):
+        rows, cols = int(rows), int(cols)
+        if max(abs(rows), abs(cols)) >= 1 << 31:
+            raise ValueError("rows %d, cols %d: out of range" % (rows, cols))
+        return rows, cols
+
     def _take(self, x, dtype, rows, cols, ld, name):
         ptr, ld, dev = _matrix(x, dtype, rows, cols, ld, name)
         if dev is not None:
@@ -340,7 +347,8 @@ class OrthoJobs(_Jobs):
         _Jobs.__init__(self, OrthoJob, len(jobs))
         for a, (G, gd, rows, cols, O, od, *lds) in zip(self.c, jobs):
             ldg, ldo = lds or (None, None)
-            a.rows, a.cols, a.g_dtype, a.o_dtype = int(rows), int(cols), gd, od
+            a.rows, a.cols = self._size(rows, cols)
+            a.g_dtype, a.o_dtype = gd, od
             a.G, a.ldg = self._take(G, gd, rows, cols, ldg, "G")
             a.O, a.ldo = self._take(O, od, rows, cols, ldo, "O")
 
@@ -354,7 +362,8 @@ class OrthoStepJobs(_Jobs):
         _Jobs.__init__(self, OrthoStepJob, len(jobs))
         for a, (G, gd, rows, cols, M, W, wd, *more) in zip(self.c, jobs):
             gamma, ldg, ldm, ldw = (more + [None] * 4)[:4]
-            a.rows, a.cols, a.g_dtype, a.w_dtype = int(rows), int(cols), gd, wd
+            a.rows, a.cols = self._size(rows, cols)
+            a.g_dtype, a.w_dtype = gd, wd
             a.gamma = max(1.0, rows / max(cols, 1)) ** 0.5 if gamma is None else float(gamma)
             a.G, a.ldg = self._take(G, gd, rows, cols, ldg, "G")
             a.M, a.ldm = self._take(M, CP_F32, rows, cols, ldm, "M")

@@ -150,3 +150,15 @@ def test_both_parts_lie_on_one_device():
     for kw in (dict(scale=two), dict(scale=three), dict(q=three), dict(q=Buf(1 << 16), scale=three), dict(q=Buf(1 << 16), scale=two)):
         with pytest.raises(ValueError):
             held(**kw)
+
+
+# ---- sizes that a record does not hold ----------------------------------------------------------------------------------------
+
+
+def test_sizes_past_the_records_are_refused():
+    """2^32 + 64 rows are not 64 of them."""
+    for rows, cols in (((1 << 32) + 64, 4), (4, (1 << 32) + 64), (1 << 31, 4)):
+        with pytest.raises(ValueError):
+            capi.OrthoJobs([(4096, 0, rows, cols, 8192, 0)])
+        with pytest.raises(ValueError):
+            capi.OrthoStepJobs([(4096, 0, rows, cols, 8192, 16384, 0)])
