@@ -49,19 +49,22 @@ struct Job {
     float lr;                    // lr * gamma
 };
 
-// The phases' launches: job k's first workgroup of each, and the pieces of k that its tiles are cut into
+// The phases' launches: job k's first workgroup of each, and how the products' tiles are shared: the pieces of k that they are cut
+// into (at most 16, in the low bits) and, where there are several, the job's first slot among the launch's partial sums and counters
 // (LAST: the last step's third product, which writes O or W)
 enum { LOAD, GRAM, POLY, APPLY, LAST, PHASES };
+constexpr int kShareBits = 5;
 struct Place {
     int first[PHASES];
-    int16_t pieces[PHASES];
+    int share[PHASES - 1];
+    int pieces(int phase) const { return share[phase - 1] & ((1 << kShareBits) - 1); }
 };
 
 // A call's jobs in its workspace.  The first kernel carries them in its arguments and writes them there.
 struct Table {
     Job *job;
     int *first[PHASES];
-    int *pieces[PHASES];
+    int *share[PHASES - 1];
     int n;
 };
 
@@ -181,10 +184,8 @@ __global__ void __launch_bounds__(256) k_ortho_norm(Jobs js, Table t, float mome
         const int *from = reinterpret_cast<const int *>(&j);
         int *to = reinterpret_cast<int *>(t.job + js.base + which);
         for (int i = threadIdx.x; i < int(sizeof(Job) / 4); i += 256) to[i] = from[i];
-        if (threadIdx.x < PHASES) {
-            t.first[threadIdx.x][js.base + which] = js.place[which].first[threadIdx.x];
-            t.pieces[threadIdx.x][js.base + which] = js.place[which].pieces[threadIdx.x];
-        }
+        if (threadIdx.x < PHASES) t.first[threadIdx.x][js.base + which] = js.place[which].first[threadIdx.x];
+        if (threadIdx.x < PHASES - 1) t.share[threadIdx.x][js.base + which] = js.place[which].share[threadIdx.x];
     }
     for (int i = blockIdx.x * 256 + threadIdx.x; i < n_counts; i += gridDim.x * 256) counts[i] = 0;
     const int r0 = id / j.chunks * j.rows_per, rows = min(r0 + j.rows_per, j.sum_rows) - r0;
@@ -362,7 +363,8 @@ __global__ void __launch_bounds__(CFG::T) k_ortho_product(Table tab, Factors f, 
     const int ra = wm * WI * 16, rb = wn * WJ * 16;
     const int at = nt::xcd_order(blockIdx.x, gridDim.x), which = find_job(tab.first[PHASE], tab.n, at);
     const Job j = tab.job[which];
-    const int first = tab.first[PHASE][which], pieces = tab.pieces[PHASE][which];
+    const int first = tab.first[PHASE][which], share = tab.share[PHASE - 1][which];
+    const int pieces = share & ((1 << kShareBits) - 1), slot = share >> kShareBits;
     const bool tall = j.rows > j.cols;
     const bool swap = PHASE == LAST && tall;   // the result's rows are G's rows: four consecutive numbers lie in one of them
     const char *xt = f.xt ? j.xt1 : j.xt0;
@@ -396,7 +398,7 @@ __global__ void __launch_bounds__(CFG::T) k_ortho_product(Table tab, Factors f, 
         [&](const char *s, auto between) {
             nt::products16<WI, WJ, SPLIT>(s + ra * 128, s + (BM + rb) * 128, lane, acc, between);
         });
-    if (pieces > 1 && !nt::join<T>(acc, piece, pieces, parts + int64_t(first + tile) * (BM * BN), tiles, counts + first + tile, &flag, tid))
+    if (pieces > 1 && !nt::join<T>(acc, piece, pieces, parts + int64_t(slot + tile) * (BM * BN), tiles, counts + slot + tile, &flag, tid))
         return;
     typedef nt::Patch<WI, WJ> Patch;
     const Patch patch = Patch::template of<CFG>(st, wave, lane);
@@ -1033,7 +1035,7 @@ size_t job_bytes(const Request &r) {
 struct Choice {
     int cfg;           // 0 Large, 1 Medium, 2 Small
     int grid;
-    bool joins;
+    int slots;         // of partial sums: the workgroups of the jobs whose tiles are cut
 };
 
 // The jobs of one class (one fp16 a number, or pairs)
@@ -1097,28 +1099,32 @@ bool choose(Class &cl, int phase, Choice &best) {
     for (int cfg = 0; cfg < 3; ++cfg) {
         if (forced && forced - 1 != cfg) continue;
         int64_t groups = 0, total = 0, longest = 0;
-        Choice c = {cfg, 0, false};
+        bool joins = false;
         for (size_t k = 0; k < cl.jobs.size(); ++k) {
             const int64_t tiles = tiles_of(cl.jobs[k], phase, kEdge[cfg]), steps = steps_of(cl.jobs[k], phase);
-            const int p = cl.places[k].pieces[phase];
-            c.joins |= p > 1;
+            const int p = cl.places[k].pieces(phase);
+            joins |= p > 1;
             groups += tiles * p;
             total += tiles * steps;
             longest = std::max(longest, (steps + p - 1) / p);
         }
         if (groups * (cfg == 0 ? nt::Large::T : nt::Medium::T) > kMaxThreads) continue;
-        c.grid = int(groups);
-        const double cost = cost_of(cfg, cl.split, phase == LAST && cl.jobs[0].M, groups, total, longest, c.joins);
+        const double cost = cost_of(cfg, cl.split, phase == LAST && cl.jobs[0].M, groups, total, longest, joins);
         if (cost < least) {
             least = cost;
-            best = c;
+            best = {cfg, int(groups), 0};
         }
     }
     if (least == 1e300) return false;
     int at = 0;
     for (size_t k = 0; k < cl.jobs.size(); ++k) {
-        cl.places[k].first[phase] = at;
-        at += int(tiles_of(cl.jobs[k], phase, kEdge[best.cfg])) * cl.places[k].pieces[phase];
+        Place &p = cl.places[k];
+        const int pieces = p.pieces(phase), groups = int(tiles_of(cl.jobs[k], phase, kEdge[best.cfg])) * pieces;
+        p.first[phase] = at;
+        at += groups;
+        if (pieces == 1) continue;
+        p.share[phase - 1] = pieces | best.slots << kShareBits;
+        best.slots += groups;
     }
     return true;
 }
@@ -1139,7 +1145,7 @@ int small_tiles(const Request &r) {
     return std::min(r.rows, r.cols) <= 64 && each <= kSmallTiles[split] ? (each + 1) / 2 * 2 : 0;
 }
 
-size_t table_bytes(size_t n) { return cp_align_up(n * (sizeof(Job) + 2 * PHASES * sizeof(int)), 256); }
+size_t table_bytes(size_t n) { return cp_align_up(n * (sizeof(Job) + (2 * PHASES - 1) * sizeof(int)), 256); }
 
 int lay_out(cp_ctx *ctx, const std::vector<Request> &rq, bool crossed, double lr, Layout &lay) {
     lay.cls[0].split = false;
@@ -1193,7 +1199,7 @@ int lay_out(cp_ctx *ctx, const std::vector<Request> &rq, bool crossed, double lr
         Place p = {};
         p.first[LOAD] = int(cl.loads);
         cl.loads += int64_t(mp / 64) * int64_t(np / 64);
-        for (int phase = GRAM; phase < PHASES; ++phase) p.pieces[phase] = int16_t(pieces_of(j, phase, cl.split));
+        for (int phase = GRAM; phase < PHASES; ++phase) p.share[phase - 1] = pieces_of(j, phase, cl.split);
         cl.sum_groups.push_back((j.sum_rows + j.rows_per - 1) / j.rows_per * j.chunks);
         cl.jobs.push_back(j);
         cl.places.push_back(p);
@@ -1203,9 +1209,9 @@ int lay_out(cp_ctx *ctx, const std::vector<Request> &rq, bool crossed, double lr
         if (cl.loads * 256 > kMaxThreads || !choose(cl, GRAM, cl.gram) || !choose(cl, POLY, cl.poly) || !choose(cl, APPLY, cl.apply) || !choose(cl, LAST, cl.last))
             return cp_set_error(ctx, CP_ERR_UNSUPPORTED, "matrices of a call too large for one launch");
         for (const Choice *c : {&cl.gram, &cl.poly, &cl.apply, &cl.last})
-            if (c->joins) {
-                lay.counts = std::max(lay.counts, cp_align_up(size_t(c->grid) * sizeof(int), 256));
-                lay.parts = std::max(lay.parts, size_t(c->grid) * kEdge[c->cfg] * kEdge[c->cfg] * sizeof(float));
+            if (c->slots) {
+                lay.counts = std::max(lay.counts, cp_align_up(size_t(c->slots) * sizeof(int), 256));
+                lay.parts = std::max(lay.parts, size_t(c->slots) * kEdge[c->cfg] * kEdge[c->cfg] * sizeof(float));
             }
         lay.tables += table_bytes(cl.jobs.size());
     }
@@ -1229,10 +1235,8 @@ void place(Layout &lay, char *ws) {
         cl.table.n = int(n);
         cl.table.job = reinterpret_cast<Job *>(tables);
         int *p = reinterpret_cast<int *>(tables + n * sizeof(Job));
-        for (int k = 0; k < PHASES; ++k) {
-            cl.table.first[k] = p + 2 * k * n;
-            cl.table.pieces[k] = p + (2 * k + 1) * n;
-        }
+        for (int k = 0; k < PHASES; ++k) cl.table.first[k] = p + k * n;
+        for (int k = 0; k < PHASES - 1; ++k) cl.table.share[k] = p + (PHASES + k) * n;
         tables += table_bytes(n);
         for (Job &j : cl.jobs) {
             const size_t mn = size_t(j.mp) * j.ldn, mm = size_t(j.mp) * j.lds;

@@ -160,3 +160,41 @@ def test_step_of_many_small_layers(ctx):
     layers = [Layer(ctx, rs, *s, *kinds[i % 5], None if i % 3 else 0.7) for i, s in enumerate(shapes)]
     assert capi.ortho_workspace(capi.OrthoStepJobs([a.job() for a in layers])) == 0
     run_together(ctx, layers, lambda a: True)
+
+
+# ---- workspaces ------------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("one,many", [((128, 20000), [(4096, 4096)] * 40), ((100, 50000), [(2048, 8192)] * 200), ((70, 9000), [(512, 512)] * 30)])
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+def test_a_layer_cut_along_k_brings_its_own_pieces_only(one, many, kind):
+    """The partial sums of one layer's tiles, not slots for every workgroup of the launch it joins."""
+    def need(shapes):
+        T, at, jobs = TYPES[kind], 1 << 40, []
+        for r, c in shapes:
+            jobs.append((at, T, r, c, at + (1 << 34), T))
+            at += 1 << 36
+        return capi.ortho_workspace(capi.OrthoJobs(jobs))
+
+    # its matrices (what it needs alone), and 16 pieces of each of its 256 x 256 tiles of the first product, of 256 KB
+    pieces = 16 * (-(-one[0] // 256)) * (-(-one[0] // 256)) << 18
+    assert need(many) < need(many + [one]) <= need(many) + need([one]) + pieces + 65536
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+def test_mixed_call_stays_in_its_workspace(ctx, tile_shape, kind):
+    """Layers whose tiles are cut among others whose are not: the same bits as each alone, nothing behind the workspace."""
+    rs = np.random.RandomState(40)
+    shapes = [(150, 140), (70, 9000), (300, 260), (6000, 130), (200, 70), (129, 4500)]
+    T = TYPES[kind]
+    Gs, Os = [Mat(ctx, dominated(rs, *s, 2.0), kind) for s in shapes], [Mat(ctx, np.zeros(s), kind) for s in shapes]
+    jobs = capi.OrthoJobs([(G.ptr, T, *s, O.ptr, T) for G, O, s in zip(Gs, Os, shapes)])
+    need = ctx.ortho_workspace(jobs)
+    ws = ctx.to_device(np.full(need + 4096, 0xff, dtype=np.uint8))
+    assert ctx.lib.cp_orthogonalise(ctx.h, jobs.n, jobs.c, 5, None, 1e-7, ws.ptr, need) == 0
+    assert (ctx.to_host(ws, (need + 4096,), np.uint8)[need:] == 0xff).all()
+    for G, O, s in zip(Gs, Os, shapes):
+        one = Mat(ctx, np.zeros(s), kind)
+        ctx.orthogonalise(capi.OrthoJobs([(G.ptr, T, *s, one.ptr, T)]))
+        assert O.untouched() and np.array_equal(one.raw(), O.raw())
