@@ -135,6 +135,8 @@ SIGNATURES = {
     "cp_prune_layers": (_c_int, [_c_int, ctypes.POINTER(_vp), _vp, _vp]),
     "cp_result_host": (_c_int, [_vp, ctypes.POINTER(_vp), ctypes.POINTER(_vp), ctypes.POINTER(_c_int),
                                 ctypes.POINTER(_c_int)]),
+    "cp_ctx_after_stream": (_c_int, [_vp, _vp]),
+    "cp_ctx_before_stream": (_c_int, [_vp, _vp]),
     "cp_blocks_check": (_c_int, [_vp]),
     "cp_quant_blocks": (_c_int, [_vp, _vp, _c_int, _c_i64, _c_i64, _c_i64, _c_int, _vp, _vp]),
     "cp_matmul_blocks": (_c_int, [_vp, _vp, _vp, _vp, _vp, _c_int, _c_i64, _vp, ctypes.c_size_t]),
@@ -225,6 +227,19 @@ def _torch_codes():
     return _TORCH_CODES
 
 
+def torch_stream(device):
+    """torch's current stream on a device as a handle for set_stream (the legacy default stream: 1)."""
+    import torch
+    try:
+        return torch._C._cuda_getCurrentRawStream(device) or 1          # 0.1 us; the public way takes 2.7
+    except AttributeError:
+        return torch.cuda.current_stream(device).cuda_stream or 1
+
+
+def _is_tensor(x):
+    return hasattr(x, "data_ptr")
+
+
 def _matrix(x, dtype, rows, cols, ld, name):
     """(pointer, row stride in elements, device index or None) of a device matrix.  A torch tensor is held to the dtype code,
     the shape and unit column stride, and gives its own row stride; a DevBuf to its size; an int, a device address, is taken as it is."""
@@ -265,6 +280,7 @@ class Blocks:
         kb, up = -(-cols // 128), -(-cols // 128) * 128
         tall = rows if tile == 1 else -(-rows // 128)
         self.device = None
+        self.tensors = _is_tensor(q) or _is_tensor(scale)
         for t, name, dts, need in ((q, "q", ("torch.uint8", *_FLOAT8), (rows, up)),
                                    (scale, "scale", ("torch.float32",), (kb, tall))):
             if not hasattr(t, "data_ptr"):
@@ -319,7 +335,7 @@ class _Jobs:
     """An array of job records and what keeps their memory alive."""
 
     def __init__(self, struct, n):
-        self.n, self.keep, self.device = n, [], None
+        self.n, self.keep, self.device, self.tensors = n, [], None, False
         self.c = (struct * max(n, 1))()
 
     @staticmethod
@@ -336,6 +352,7 @@ class _Jobs:
                 raise ValueError("%s is on another device than the job before it" % name)
             self.device = dev
         self.keep.append(x)
+        self.tensors = self.tensors or _is_tensor(x)
         return ptr, ld
 
 
@@ -403,6 +420,8 @@ class DevBuf:
 class Context:
     """One device + one stream (cp_ctx).  Create it inside the process that uses it."""
 
+    _given = None       # the caller's stream of set_stream
+
     def __init__(self, device=0, priority=None):
         """priority: HIP priority of the context's stream (< 0 = higher); None = the environment's CP_CTX_PRIORITY (default 0)"""
         self.lib = load()
@@ -425,6 +444,7 @@ class Context:
         h = _vp()
         self._check(self.lib.cp_ctx_create_sibling(self.h, ctypes.byref(h)), "cp_ctx_create_sibling")
         other.h, other.device, other.pid = h.value, self.device, self.pid
+        other._given = self._given
         other._parent = self       # the stream belongs to `self`: keep it alive as long as the sibling
         return other
 
@@ -497,9 +517,32 @@ class Context:
         self._check(self.lib.cp_sync(self.h), "cp_sync")
 
     def set_stream(self, stream_ptr):
-        """Run on a caller's stream; 0 or None: the context's own, which torch's work does not wait for, nor it for torch's.
-        In order with torch: set_stream(torch.cuda.current_stream().cuda_stream or 1) -- 1 is the legacy default stream."""
+        """Run on a caller's stream (1: the legacy default stream); 0 or None: the context's own.  Nothing is put in order by this
+        call: with torch's work, use_torch_stream does it."""
         self._check(self.lib.cp_ctx_set_stream(self.h, stream_ptr), "cp_ctx_set_stream")
+        self._given = getattr(stream_ptr, "value", stream_ptr) or None
+
+    def use_torch_stream(self):
+        """Run on torch's current stream, behind what this context has enqueued so far (its scratch is free then).  To be called
+        again where that stream may have changed; costs next to nothing where it has not.  (On its own stream a context
+        puts every call with torch tensors in order with torch's current stream, by two events: about 10 us a call.)"""
+        s = torch_stream(self.device)
+        if s != self._given:
+            self._check(self.lib.cp_ctx_before_stream(self.h, s), "cp_ctx_before_stream")
+            self.set_stream(s)
+
+    def _enter(self, *tensors):
+        """Before a call on the context's own stream: if any part is a torch tensor, what torch's stream holds is waited for.
+        -> that stream, for _leave, or None."""
+        if not any(tensors):
+            return None
+        s = torch_stream(self.device)
+        self._check(self.lib.cp_ctx_after_stream(self.h, s), "cp_ctx_after_stream")
+        return s
+
+    def _leave(self, s):
+        """Behind the call: torch's stream waits for it."""
+        self._check(self.lib.cp_ctx_before_stream(self.h, s), "cp_ctx_before_stream")
 
     # -- hot path -------------------------------------------------------------------
     def patch_gather(self, fmap, B, C, H, W, xs, ys, k, pad, stride, relu, X_out, row0):
@@ -661,7 +704,10 @@ class Context:
         for d, name in ((dev, "x"), (out and out.device, "out"), (out_t and out_t.device, "out_t")):
             if d is not None and d != self.device:
                 self._elsewhere(d, name)
+        s = None if self._given else self._enter(_is_tensor(x), out and out.tensors, out_t and out_t.tensors)
         rc = self.lib.cp_quant_blocks(self.h, p, x_dtype, rows, cols, ldx, flags, out and out.ref, out_t and out_t.ref)
+        if s:
+            self._leave(s)
         if rc:
             self._check(rc, "cp_quant_blocks")
 
@@ -669,6 +715,7 @@ class Context:
         """C [M, N] = A [M, K] B [N, K]^T (+ bias float32 [N]) of two Blocks (cp_matmul_blocks).  ws: None or a device buffer
         of matmul_blocks_workspace() bytes (needed under stream capture)."""
         p, ldc, dev = _matrix(C, c_dtype, A.rows, B.rows, ldc, "C")
+        tensors = _is_tensor(C) or A.tensors or B.tensors or _is_tensor(bias) or _is_tensor(ws)
         for d, name in ((dev, "C"), (A.device, "A"), (B.device, "B")):
             if d is not None and d != self.device:
                 self._elsewhere(d, name)
@@ -684,7 +731,10 @@ class Context:
                     raise ValueError("bias: the buffer holds %d bytes, %d needed" % (bias.nbytes, 4 * B.rows))
             bias = _device_ptr(bias, "bias")
         w, wb = (None, 0) if ws is None else self._ws(ws)
+        s = None if self._given else self._enter(tensors)
         rc = self.lib.cp_matmul_blocks(self.h, A.ref, B.ref, bias, p, c_dtype, ldc, w, wb)
+        if s:
+            self._leave(s)
         if rc:
             self._check(rc, "cp_matmul_blocks")
 
@@ -715,8 +765,11 @@ class Context:
         self._jobs(jobs, OrthoJobs)
         q = self._coef(coef, steps)
         w, wb = self._ws(ws)
-        self._check(self.lib.cp_orthogonalise(self.h, jobs.n, jobs.c, steps, None if q is None else q.ctypes.data, eps, w, wb),
-                    "cp_orthogonalise")
+        s = None if self._given else self._enter(jobs.tensors, _is_tensor(ws))
+        rc = self.lib.cp_orthogonalise(self.h, jobs.n, jobs.c, steps, None if q is None else q.ctypes.data, eps, w, wb)
+        if s:
+            self._leave(s)
+        self._check(rc, "cp_orthogonalise")
 
     def ortho_step(self, jobs, lr, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coef=None, eps=1e-7, ws=None):
         """One optimiser step on every layer of an OrthoStepJobs list: momentum, orthogonalisation, decay, weights
@@ -724,8 +777,12 @@ class Context:
         self._jobs(jobs, OrthoStepJobs)
         q = self._coef(coef, steps)
         w, wb = self._ws(ws)
-        self._check(self.lib.cp_ortho_step(self.h, jobs.n, jobs.c, lr, momentum, int(nesterov), weight_decay, steps,
-                                           None if q is None else q.ctypes.data, eps, w, wb), "cp_ortho_step")
+        s = None if self._given else self._enter(jobs.tensors, _is_tensor(ws))
+        rc = self.lib.cp_ortho_step(self.h, jobs.n, jobs.c, lr, momentum, int(nesterov), weight_decay, steps,
+                                    None if q is None else q.ctypes.data, eps, w, wb)
+        if s:
+            self._leave(s)
+        self._check(rc, "cp_ortho_step")
 
     def ortho_workspace(self, jobs, steps=5, coef=None, eps=1e-7):
         """Bytes of scratch that a call on these jobs (OrthoJobs or OrthoStepJobs) needs."""

@@ -113,6 +113,7 @@ struct cp_ctx {
     bool refit_pending = false;       // set by a deferred refit: factor + solve still to be launched by the batch
     cp_refit_deferred deferred = {};
     cp_precompute pre;
+    hipEvent_t ev_order = nullptr;    // cp_ctx_after_stream, cp_ctx_before_stream
     hipEvent_t ev_fork = nullptr, ev_join = nullptr;   // hand-offs to / from the shared CU-masked stream of the long GEMMs
     int itq_sweeps = 0;               // Jacobi sweeps of the last cp_itq_iterate (all alternations)
     int itq_ns_steps = 0, itq_sign_alternations = 0;   // Newton-Schulz steps / alternations that took the sign-function route

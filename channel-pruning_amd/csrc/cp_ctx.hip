@@ -144,6 +144,7 @@ extern "C" int cp_ctx_destroy(cp_ctx *ctx) {
     if (ctx->ev_epoch) hipEventDestroy(ctx->ev_epoch);
     for (int i = 0; i < 2 * CP_MAX_STAGES; ++i)
         if (ctx->ev[i]) hipEventDestroy(ctx->ev[i]);
+    if (ctx->ev_order) hipEventDestroy(ctx->ev_order);
     if (ctx->ev_fork) hipEventDestroy(ctx->ev_fork);
     if (ctx->ev_join) hipEventDestroy(ctx->ev_join);
     if (ctx->own_stream) hipStreamDestroy(ctx->own_stream);
@@ -155,6 +156,32 @@ extern "C" int cp_ctx_set_stream(cp_ctx *ctx, void *hip_stream) {
     if (!ctx) return CP_ERR_ARG;
     ctx->stream = hip_stream ? reinterpret_cast<hipStream_t>(hip_stream) : ctx->own_stream;
     return CP_OK;
+}
+
+// `later` waits for what `earlier` holds now
+static int stream_order(cp_ctx *ctx, hipStream_t earlier, hipStream_t later) {
+    if (earlier == later) return CP_OK;
+    CP_HIP(ctx, hipSetDevice(ctx->device));
+    if (!ctx->ev_order) CP_HIP(ctx, hipEventCreateWithFlags(&ctx->ev_order, hipEventDisableTiming));
+    CP_HIP(ctx, hipEventRecord(ctx->ev_order, earlier));
+    CP_HIP(ctx, hipStreamWaitEvent(later, ctx->ev_order, 0));
+    return CP_OK;
+}
+static hipStream_t stream_of(void *s) { return s == hipStreamLegacy ? nullptr : reinterpret_cast<hipStream_t>(s); }
+
+extern "C" int cp_ctx_after_stream(cp_ctx *ctx, void *hip_stream) {
+    if (!ctx) return CP_ERR_ARG;
+    return stream_order(ctx, stream_of(hip_stream), stream_of(ctx->stream));
+}
+
+extern "C" int cp_ctx_before_stream(cp_ctx *ctx, void *hip_stream) {
+    if (!ctx) return CP_ERR_ARG;
+    const hipStream_t own = stream_of(ctx->stream), other = stream_of(hip_stream);
+    hipStreamCaptureStatus a = hipStreamCaptureStatusNone, b = hipStreamCaptureStatusNone;
+    CP_HIP(ctx, hipSetDevice(ctx->device));
+    if (own) CP_HIP(ctx, hipStreamIsCapturing(own, &a));   // (the default stream is never captured)
+    if (other) CP_HIP(ctx, hipStreamIsCapturing(other, &b));
+    return a == b ? stream_order(ctx, own, other) : CP_OK;
 }
 
 extern "C" int cp_sync(cp_ctx *ctx) {

@@ -67,6 +67,12 @@ int cp_ctx_create_sibling(cp_ctx *of, cp_ctx **out);
  * NULL restores the ctx's own stream, which no other stream waits for.  The legacy default stream, which torch uses unless
  * told otherwise and gives as 0, is hipStreamLegacy (1). */
 int cp_ctx_set_stream(cp_ctx *ctx, void *hip_stream);
+/* What the context enqueues from now on runs behind what hip_stream (NULL or hipStreamLegacy: the legacy default stream) holds
+ * now.  On a stream under capture the context's stream joins the capture. */
+int cp_ctx_after_stream(cp_ctx *ctx, void *hip_stream);
+/* What hip_stream runs from now on is behind what the context has enqueued.  Does nothing where one of the two streams is under
+ * capture and the other is not: a graph cannot wait for work outside of it. */
+int cp_ctx_before_stream(cp_ctx *ctx, void *hip_stream);
 int cp_sync(cp_ctx *ctx);
 
 /* ---- device memory helpers (so a ctypes-only host needs nothing else) ------------ */

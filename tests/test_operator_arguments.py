@@ -9,7 +9,7 @@ from cpmi355 import capi
 @pytest.fixture
 def no_ctx():
     c = capi.Context.__new__(capi.Context)
-    c.lib, c.h, c.device = capi.load(), None, 0
+    c.lib, c.h, c.device, c._given = capi.load(), None, 0, 1
     return c
 
 
