@@ -263,7 +263,7 @@ def _capi():
     from cpmi355 import capi
     if _ctx is None:
         _ctx = capi.Context(0)
-        _ctx.set_stream(torch.cuda.current_stream().cuda_stream or 1)      # in order with torch's work (0 is the legacy default stream, 1)
+    _ctx.use_torch_stream()                                                # in order with torch's work, whatever stream it is on now
     return capi, _ctx
 
 
