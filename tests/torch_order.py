@@ -132,6 +132,27 @@ for name, ctx in (("own", own), ("follows", follows)):
         assert same(e, r), turn
     print("captured:", name, flush=True)
 
+# the timed programs, first on the default stream, then on another
+from perf import operators as ops  # noqa: E402
+ops.own = True
+case = dict(op="step", shapes="64x495,300x200", w="f32", g="f32", nesterov=True)
+first = {k: v.clone() for k, v in ops.run(ops.prepare(case, 7)).items()}
+torch.cuda.synchronize()
+with torch.cuda.stream(side[0]):
+    st = ops.prepare(case, 7)
+    G = [g.clone() for g in st["G"]]
+    for g in st["G"]:
+        g.zero_()
+    delay()
+    for g, h in zip(st["G"], G):
+        g.copy_(h)
+    out = ops.run(st)
+    got = {k: v.clone() for k, v in out.items()}
+    for v in out.values():
+        v.zero_()
+    torch.cuda.synchronize()
+    assert all(torch.equal(first[k], got[k]) for k in first)
+print("perf/operators on another stream", flush=True)
 torch.cuda.synchronize()
 for c in (own, follows):
     c.close()
