@@ -352,8 +352,8 @@ __device__ __forceinline__ void write_c(const Product &p, const f4 (&acc)[WI][WJ
 }
 
 // One tile of C, or a piece of k of it, to a workgroup.  COMMON: B's rows share their scales in blocks of 128 (weights), so that a
-// wave multiplies each sum by one factor; else by a row's and a column's.  Beside the matrix instructions a step has that
-// factor and a fused add for every number of the tile: bound by both together.  8192^3, every row with its own scales: 527 us, 2.09
+// wave's sums take a row's factor; else a row's and a column's.  Beside the matrix instructions a step has those
+// factors in a fused add for every number of the tile (and a product): bound by both together.  8192^3, every row with its own scales: 527 us, 2.09
 // PFLOP/s (a library product without any scales 358); common scales, 20000 x 512 x 4005: 67 us, 1.22 (its
 // 80 MB come from HBM one step ahead of their use).  WIDE (float32 and fp16 results):
 // the operands are widened in registers and go through the fp16 instructions, twice as many: 512 x 4005 x 20000, 112 us, 0.73
@@ -468,7 +468,7 @@ __global__ void __launch_bounds__(512) k_matmul_blocks_rows(Product p) {
                 fa.set(qa[u][m][0], qa[u][m][1]);
                 const f4 t = nt::block_product<FA, FB, WIDE>(fa, fb);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) acc[m][r] = fmaf(t[r], si[u][m] * sj[u][COMMON ? 0 : r], acc[m][r]);
+                for (int r = 0; r < 4; ++r) acc[m][r] = fmaf(t[r] * si[u][m], sj[u][COMMON ? 0 : r], acc[m][r]);
             }
         }
     }

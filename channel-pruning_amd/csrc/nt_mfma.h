@@ -236,13 +236,22 @@ struct Frag8 {
     }
 };
 
-// the products of one block of sixteen rows of A and of B, from zero
-template <int FA, int FB, bool WIDE>
-__device__ __forceinline__ f4 block_product(const Frag8<FA, WIDE> &a, const Frag8<FB, WIDE> &b) {
+// a scale as a power of two, in the form of the matrix instruction's own scales, and the rest (a user's scale may be anything)
+__device__ __forceinline__ float part_of(float scale, int &power) {
+    const uint32_t e = __float_as_uint(scale) >> 23 & 0xff;
+    power = int(min(max(e, 1u), 254u));
+    return ldexpf(scale, 127 - power);
+}
+
+// the products of one block of sixteen rows of A and of B, from zero.  SCALED: times 2^(power - 127)
+template <int FA, int FB, bool WIDE, bool SCALED = false>
+__device__ __forceinline__ f4 block_product(const Frag8<FA, WIDE> &a, const Frag8<FB, WIDE> &b, int power = 127) {
     f4 z = {0.f, 0.f, 0.f, 0.f};
     if (WIDE) {
 #pragma unroll
         for (int h = 0; h < 4; ++h) z = __builtin_amdgcn_mfma_f32_16x16x32_f16(b.w[h], a.w[h], z, 0, 0, 0);
+    } else if constexpr (SCALED) {
+        z = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b.v, a.v, z, FB, FA, 0, power, 0, 127);
     } else {
         z = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b.v, a.v, z, FB, FA, 0, 0, 0, 0);
     }
@@ -250,7 +259,10 @@ __device__ __forceinline__ f4 block_product(const Frag8<FA, WIDE> &a, const Frag
 }
 
 // The 8-bit step: the products of one block of 128 start from zero and join the accumulators times both blocks' scales.
-// sa [16 WI] and sb ([16 WJ], or one value where COMMON) are this wave's scales of the step.
+// sa [16 WI] and sb ([16 WJ], or one value where COMMON) are this wave's scales of the step.  The product of two scales may lie
+// outside float32 where the result does not (operands of 1e-19; blocks of 1e30 and 1e14 that share no column): a sum is taken
+// times one, then times the other.  COMMON on the 8-bit instructions has no time for a second product (8192^3: 505 us instead of 430): there the
+// instruction takes the power of two of B's scale, and what is left of it joins A's (439 us).
 // WIDE: the 8-bit matrix instructions align the eight products of a group to the largest and drop what lies below 2^-13 of
 // its power of two (measured: 2^16 + 4 gives 2^16 within a group, 2^16 + 8 is exact, and across groups all of float32 counts).
 // A bfloat16 result rounds off 2^-8 and takes them as they are; float32 and fp16 results are formed with the fp16
@@ -263,14 +275,18 @@ __device__ __forceinline__ void products8(const char *a, const char *b, const fl
     Frag8<FA, WIDE> af[2];
     f4 sj[WJ], t[2][WJ];
     float si[2];
-    const float common = COMMON ? sb[0] : 1.f;
+    constexpr bool SCALED = COMMON && !WIDE;
+    int power = 127;
+    float common = COMMON ? sb[0] : 1.f;
+    if constexpr (SCALED) common = part_of(common, power);
     auto join = [&](int i, int j) {   // a row group's products join the accumulators while the next one's are formed
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-            acc[i][j][r] = fmaf(t[i & 1][j][r], COMMON ? si[i & 1] : si[i & 1] * sj[j][r], acc[i][j][r]);
+            acc[i][j][r] = SCALED ? fmaf(t[i & 1][j][r], si[i & 1], acc[i][j][r])
+                                  : fmaf(t[i & 1][j][r] * si[i & 1], COMMON ? common : sj[j][r], acc[i][j][r]);
     };
     af[0].load(a, o0, o1);
-    si[0] = sa[lane & 15] * common;
+    si[0] = sa[lane & 15] * (SCALED ? common : 1.f);
 #pragma unroll
     for (int j = 0; j < WJ; ++j) {
         bf[j].load(b + j * 2048, o0, o1);
@@ -290,14 +306,14 @@ __device__ __forceinline__ void products8(const char *a, const char *b, const fl
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int j = 0; j < WJ; ++j) {
-            t[u][j] = block_product<FA, FB, WIDE>(af[u], bf[j]);
+            t[u][j] = block_product<FA, FB, WIDE, SCALED>(af[u], bf[j], power);
             if (i > 0) join(i - 1, j);
             // a matrix instruction, then the vector instructions that fit beside it
             __builtin_amdgcn_sched_group_barrier(0x008, WIDE ? 4 : 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x002, COMMON ? 4 : 8, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, SCALED ? 4 : 8, 0);
         }
         __builtin_amdgcn_s_setprio(0);
-        if (i + 1 < WI) si[u ^ 1] = COMMON ? next * common : sa[(i + 1) * 16 + (lane & 15)];
+        if (i + 1 < WI) si[u ^ 1] = COMMON ? next * (SCALED ? common : 1.f) : sa[(i + 1) * 16 + (lane & 15)];
         NT_STAY();
     }
 #pragma unroll

@@ -283,7 +283,8 @@ int cp_quant_blocks(cp_ctx *ctx, const void *x, int x_dtype, int64_t rows, int64
 /* C[i, j] = sum_k A[i, k] B[j, k] (+ bias[j]): A [M, K], B [N, K], C DEVICE [M, N] (c_dtype F32, BF16 or F16, row stride
  * ldc elements), bias DEVICE f32 [N] or NULL.  With x [M, c k^2], w [n, c k^2], dy [M, n]: y = x w^T, dx = dy (w^T)^T,
  * dw = dy^T (x^T)^T, the operands in the orientation that cp_quant_blocks' out / out_t give.  The products of a block are
- * summed in float32 and joined in float32 times both scales; one rounding to c_dtype at the end.  (For BF16 the matrix unit
+ * summed in float32 and joined in float32 times both scales, whose own product may be past float32 (a block's sum times one of
+ * them may not: magnitudes below 2^104 are safe in any case); one rounding to c_dtype at the end.  (For BF16 the matrix unit
  * adds products eight at a time, each cut below 2^-13 of the largest; F32 and F16 results keep all of float32.)  The order of
  * the sums depends on the shape alone.  C must not overlap the operands.  K = 0: C = bias (or 0).  Asynchronous.
  * ws: DEVICE scratch of cp_matmul_blocks_workspace() bytes, 256-byte aligned, or NULL: the context's own, which a call under
