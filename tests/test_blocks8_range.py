@@ -62,3 +62,28 @@ def test_scales_of_every_size(ctx, tile_shape, tb, out):
     want, tol = product_bound(A.real, B.real, out)
     got = formed(ctx, A, B, out)
     assert (np.abs(got - want) <= tol).all(), float((np.abs(got - want) / tol).max())
+
+
+@gpu
+@pytest.mark.parametrize("m,n", SHAPES)
+@pytest.mark.parametrize("ta,tb", [(1, 1), (1, 128), (128, 128)])
+@pytest.mark.parametrize("out", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("fa", ["e4m3", "e5m2"])
+def test_nan_stays_in_its_row_and_column(ctx, tile_shape, m, n, ta, tb, out, fa):
+    """An infinity or a NaN in A or B becomes a NaN there: the result's row or column is NaN, everything else is as it was."""
+    rs = np.random.RandomState(m + n)
+    a, b = rs.randn(m, 300), rs.randn(n, 300)
+    a[m // 2, 5], a[m - 1, 299], b[n - 1, 130] = np.nan, -np.inf, np.inf
+    mats = []
+    for x, f, t in ((a, fa, ta), (b, "e4m3", tb)):
+        X, h = Mat(ctx, x, "f32"), Held(ctx, *x.shape, f, t)
+        ctx.quant_blocks(X.ptr, capi.CP_F32, h.b)
+        mats.append(h)
+    got = formed(ctx, *mats, out)
+    bad = np.zeros((m, n), dtype=bool)
+    bad[[m // 2, m - 1]], bad[:, n - 1] = True, True
+    assert np.array_equal(np.isnan(got), bad)
+    for x in (a, b):
+        x[~np.isfinite(x)] = 0                                   # (a block's scale is that of its finite values)
+    want, tol = product_bound(Held.of(ctx, a, fa, ta).real, Held.of(ctx, b, "e4m3", tb).real, out)
+    assert (np.abs(got - want)[~bad] <= tol[~bad]).all()
