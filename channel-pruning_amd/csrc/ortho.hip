@@ -961,17 +961,27 @@ struct Region {
     size_t size;
     size_t job;
     bool read;   // G
+    int64_t width() const { return cols * int64_t(size); }
     uintptr_t end() const { return at + (size_t(rows - 1) * ld + cols) * size; }
 };
 
-// whether two matrices share an element: rows of one stride interleave as column ranges of one wider matrix do
+// whether two matrices share a byte
 bool overlap(const Region &p, const Region &q) {
     if (p.at >= q.end() || q.at >= p.end()) return false;
-    if (p.ld != q.ld || p.size != q.size) return true;
-    const Region &lo = p.at <= q.at ? p : q, &hi = p.at <= q.at ? q : p;
-    if ((hi.at - lo.at) % lo.size) return true;
-    const int64_t d = int64_t((hi.at - lo.at) / lo.size) % lo.ld;   // hi's first column, counted from lo's
-    return d < lo.cols || d + hi.cols > lo.ld;
+    if (p.ld == q.ld && p.size == q.size) {   // rows of one stride interleave as column ranges of one wider matrix do
+        const Region &lo = p.at <= q.at ? p : q, &hi = p.at <= q.at ? q : p;
+        const int64_t stride = lo.ld * int64_t(lo.size), d = int64_t(hi.at - lo.at) % stride;   // hi's first byte, counted from a row of lo
+        return d < lo.width() || d + hi.width() > stride;
+    }
+    // every row of the one with fewer against the first row of the other that ends behind its begin
+    const Region &few = p.rows <= q.rows ? p : q, &many = p.rows <= q.rows ? q : p;
+    const int64_t stride = many.ld * int64_t(many.size);
+    for (int64_t i = 0; i < few.rows; ++i) {
+        const int64_t begin = int64_t(few.at) + i * few.ld * int64_t(few.size) - int64_t(many.at);
+        const int64_t row = begin < many.width() ? 0 : (begin - many.width()) / stride + 1;
+        if (row < many.rows && row * stride < begin + few.width()) return true;
+    }
+    return false;
 }
 
 struct Request {

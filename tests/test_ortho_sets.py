@@ -198,3 +198,49 @@ def test_mixed_call_stays_in_its_workspace(ctx, tile_shape, kind):
         one = Mat(ctx, np.zeros(s), kind)
         ctx.orthogonalise(capi.OrthoJobs([(G.ptr, T, *s, one.ptr, T)]))
         assert O.untouched() and np.array_equal(one.raw(), O.raw())
+
+
+# ---- which matrices of a call may lie where ---------------------------------------------------------------------------------------
+
+
+def cells(at, rows, cols, ld, size):
+    return {at + (i * ld + j) * size + b for i in range(rows) for j in range(cols) for b in range(size)}
+
+
+def test_outputs_are_refused_exactly_where_they_share_memory():
+    """Interleaved matrices of any strides and types, against sets of their bytes."""
+    rs = np.random.RandomState(50)
+    seen = [0, 0]
+    for _ in range(4000):
+        jobs, bytes_ = [], []
+        for i in range(2):
+            kind = ("f32", "bf16")[rs.randint(2)]
+            size = 4 if kind == "f32" else 2
+            rows, cols = rs.randint(1, 7), rs.randint(1, 6)
+            ld = cols + (rs.randint(0, 20) if rs.rand() < 0.7 else 0)
+            at = 1 << 20 if i == 0 else (1 << 20) + int(rs.randint(-60, 60)) * size
+            jobs.append(((1 << 30) + (i << 20), 0, rows, cols, at, TYPES[kind], None, ld))
+            bytes_.append(cells(at, rows, cols, ld, size))
+        jobs = [j[:6] + (j[3], j[7]) for j in jobs]
+        share = bool(bytes_[0] & bytes_[1])
+        seen[share] += 1
+        if share:
+            with pytest.raises(capi.CpError):
+                capi.ortho_workspace(capi.OrthoJobs(jobs))
+        else:
+            capi.ortho_workspace(capi.OrthoJobs(jobs))
+    assert min(seen) > 1000
+
+
+def test_a_tall_matrix_between_the_rows_of_a_wide_one():
+    """2^18 rows of three numbers at a stride of their own, beside 2^18 rows of another stride that meet them in one place only."""
+    n = 1 << 18
+    def call(ld, at):
+        return capi.ortho_workspace(capi.OrthoJobs([(1 << 40, 0, n, 3, 1 << 42, 0, 3, 12), (1 << 41, 0, n, 3, (1 << 42) + 4 * at, 0, 3, ld)]))
+    call(24, 3)                                                  # every second gap
+    call(12, 9)                                                  # the same stride
+    call(36, 4)
+    call(12 * n - 1, 3)                                          # its second row lies behind the other matrix
+    for ld, at in ((25, 3), (36, 10), (24, 1), (6 * n - 1, 3)):
+        with pytest.raises(capi.CpError):
+            call(ld, at)
