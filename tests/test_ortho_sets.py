@@ -5,7 +5,7 @@ import pytest
 
 from cpmi355 import capi
 from lowbits import HALF, TYPES, Mat
-from test_ortho import iterate, tile_shape, within  # noqa: F401
+from test_ortho import distance, iterate, tile_shape, within  # noqa: F401
 
 gpu = pytest.mark.gpu
 
@@ -244,3 +244,59 @@ def test_a_tall_matrix_between_the_rows_of_a_wide_one():
     for ld, at in ((25, 3), (36, 10), (24, 1), (6 * n - 1, 3)):
         with pytest.raises(capi.CpError):
             call(ld, at)
+
+
+# ---- special values in the kernel of small matrices ---------------------------------------------------------------------------------
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,cols", [(40, 130), (64, 500), (1, 77), (33, 33)])
+def test_special_small_matrices(ctx, kind, rows, cols):
+    rs = np.random.RandomState(rows)
+    T = TYPES[kind]
+    gone = rs.randn(rows, cols)
+    gone[1::3], gone[:, 1::5] = 0, 0
+    lowrank = rs.randn(rows, 2) @ rs.randn(2, cols)
+    spread = rs.randn(rows, cols) * np.logspace(0, -4, rows)[:, None]
+    good = [gone, lowrank, spread, np.eye(rows, cols), np.zeros((rows, cols))]
+    bad = []
+    for v in (np.nan, np.inf, -np.inf):
+        b = rs.randn(rows, cols)
+        b[rows // 2, cols - 1] = v
+        bad.append(b)
+    for turn in (lambda x: x, lambda x: x.T):
+        mats = [turn(x) for x in good + bad]
+        for eps in (1e-7, 0.0):
+            Gs, Os = [Mat(ctx, x, kind) for x in mats], [Mat(ctx, np.ones(x.shape), kind) for x in mats]
+            jobs = capi.OrthoJobs([(G.ptr, T, *x.shape, O.ptr, T) for G, O, x in zip(Gs, Os, mats)])
+            assert ctx.ortho_workspace(jobs) == 0                # the small kernel, all of them in one call
+            ctx.orthogonalise(jobs, eps=eps)
+            for i, (G, O) in enumerate(zip(Gs, Os)):
+                assert O.untouched()
+                if i >= len(good):
+                    assert np.isnan(O.get()).all()
+                elif i == 4:
+                    assert (O.get() == 0).all()
+                else:
+                    want, far = distance(G.get(), kind, eps=eps)
+                    within(O.get(), want, far, kind)
+                if i == 0:
+                    assert (O.get()[(G.get() == 0).all(1)] == 0).all() and (O.get()[:, (G.get() == 0).all(0)] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("wk", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,cols", [(40, 130), (130, 40), (140, 200), (200, 140)])
+def test_a_gradient_that_is_not_finite_spoils_its_own_layer_only(ctx, wk, rows, cols):
+    rs = np.random.RandomState(60)
+    layers = [Layer(ctx, rs, rows, cols, "f32", wk, None) for _ in range(3)]
+    g = layers[1].g.get()
+    g[2, 3] = np.inf
+    layers[1].g = Mat(ctx, g, "f32")
+    before = [a.held() for a in layers]
+    ctx.ortho_step(capi.OrthoStepJobs([a.job() for a in layers]), 0.02, weight_decay=0.1)
+    for i in (0, 2):
+        layers[i].check(before[i], 0.02, 0.95, True, 0.1)
+    m = layers[1].m.get()
+    assert np.isinf(m[2, 3]) and np.isfinite(np.delete(m.reshape(-1), 2 * cols + 3)).all() and np.isnan(layers[1].w.get()).all()
