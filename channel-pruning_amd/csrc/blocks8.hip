@@ -414,8 +414,8 @@ __global__ void __launch_bounds__(CFG::T) k_matmul_blocks(Product p) {
 
 // Few rows of A: bound by reading B once.  A workgroup takes sixteen rows of B and its eight waves an eighth of k each, straight
 // from memory into the matrix instruction's registers (a lane holds 32 bytes of one row: the K order within a block is the same
-// for A and B, and that is all that a sum needs); their sums are added in the order of k.  Up to 80 rows, while the tiles' launch
-// costs more (form_of): one row by 4096 x 4096 takes 5.6 us (17 MB), a call of it 7.3 -- in 64 x 64 tiles, most of whose rows
+// for A and B, and that is all that a sum needs); their sums are added in the order of k.  Up to 128 rows (the waves' sums take 64 KB
+// of LDS then), while the tiles' launch costs more (form_of): one row by 4096 x 4096 takes 5.6 us (17 MB), a call of it 7.3 -- in 64 x 64 tiles, most of whose rows
 // would be padding, 12.
 template <int MT, int FA, int FB, bool COMMON, bool WIDE>
 __global__ void __launch_bounds__(512) k_matmul_blocks_rows(Product p) {
@@ -513,7 +513,7 @@ struct Form {
     size_t counts, parts;   // bytes
 };
 constexpr int kMaxJoined = 16384;   // workgroups of a launch that joins pieces
-constexpr int kFewRows = 80;         // of A, for k_matmul_blocks_rows
+constexpr int kRowGroups = 8;        // of sixteen rows of A, for k_matmul_blocks_rows
 constexpr int kChip = 256;          // CUs that a split is planned for
 
 Form form_of(const cp_blocks *A, const cp_blocks *B, int c_dtype) {
@@ -527,13 +527,15 @@ Form form_of(const cp_blocks *A, const cp_blocks *B, int c_dtype) {
     const int64_t steps = (A->cols + 127) / 128;
     const bool wide = wide_form(c_dtype);
     Form best = {};
-    const bool few = A->rows <= kFewRows && B->rows <= kMaxThreads / 512 * 16;
+    const bool few = A->rows <= 16 * kRowGroups && B->rows <= kMaxThreads / 512 * 16;
     int forced = cp_knob(CP_KNOB_NT_TILE);
     if (forced == 5 && !few) forced = 0;
     double least = 1e300;
     if (few && (!forced || forced == 5)) {
-        // sixteen rows of B to a workgroup: rounds of 256, each a part of a us per step.  77 x 1000 x 2048 in float32: 8.1 us, 9.5 in
-        // tiles; 64 x 4096 x 8192: 21.5, 16; 32 x 4096 x 4096 in bfloat16: 8.6, 10.4
+        // sixteen rows of B to a workgroup: rounds of 256, each a part of a us per step.  us for 16, 32, 64, 80, 96, 128 rows, against
+        // 64 x 64 tiles:  4096 x 512 bfloat16 4.3 4.2 4.7 4.3 4.4 5.0, 4.5-4.6;  1000 x 2048 float32 5.6 5.0 7.1 8.0 9.1 11.0, 8.5-9.6;
+        // 4096 x 2048 float32 5.7 5.2 7.2 8.3 9.3 11.3, 10.5-13.1;  bfloat16 5.2 5.0 7.0 8.1 9.1 11.1, 7.6-8.0;
+        // 4096 x 8192 bfloat16 9.7 13 21 24 28 35, 11-15.  Over 576 shapes the choice takes 1.01 of the better form's time.
         best = {4, 0, 0, 1, 0, 0};
         least = double((B->rows + 4095) / 4096) * steps * (0.07 + 0.0032 * A->rows) + 1.0;
         // (no tile costs less than a 64 x 64 one in one piece, or in pieces of four steps)
@@ -568,16 +570,19 @@ __global__ void __launch_bounds__(256) k_zero(int *p, int n) {
     for (int i = blockIdx.x * 256 + threadIdx.x; i < n; i += gridDim.x * 256) p[i] = 0;
 }
 
+// the least number of row groups that holds A
+template <int MT, int FA, int FB, bool COMMON, bool WIDE>
+void launch_rows(cp_ctx *ctx, const Product &p) {
+    if constexpr (MT > 1)
+        if (p.M <= 16 * (MT - 1)) return launch_rows<MT - 1, FA, FB, COMMON, WIDE>(ctx, p);
+    k_matmul_blocks_rows<MT, FA, FB, COMMON, WIDE><<<(p.N + 15) / 16, 512, 0, ctx->stream>>>(p);
+}
+
 template <int FA, int FB, bool COMMON, bool WIDE>
 void launch_product(cp_ctx *ctx, const Product &p, const Form &f) {
     const int n = f.tiles_m * f.tiles_n * f.pieces;
     if (f.cfg == 4) {
-        const int n = (p.N + 15) / 16;
-        if (p.M <= 16) k_matmul_blocks_rows<1, FA, FB, COMMON, WIDE><<<n, 512, 0, ctx->stream>>>(p);
-        else if (p.M <= 32) k_matmul_blocks_rows<2, FA, FB, COMMON, WIDE><<<n, 512, 0, ctx->stream>>>(p);
-        else if (p.M <= 64) k_matmul_blocks_rows<4, FA, FB, COMMON, WIDE><<<n, 512, 0, ctx->stream>>>(p);
-        else k_matmul_blocks_rows<5, FA, FB, COMMON, WIDE><<<n, 512, 0, ctx->stream>>>(p);
-        return;
+        return launch_rows<kRowGroups, FA, FB, COMMON, WIDE>(ctx, p);
     }
     if constexpr (!WIDE) {   // the widened fragments of 256 x 256 do not fit into registers
         if (f.cfg == 0) return (void)(k_matmul_blocks<nt::Large, FA, FB, COMMON, WIDE><<<n, nt::Large::T, 0, ctx->stream>>>(p));
