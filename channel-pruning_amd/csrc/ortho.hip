@@ -901,11 +901,11 @@ struct Plan {
     double sx[kMaxSteps + 1], sa[kMaxSteps], sb[kMaxSteps];   // scales of X before step k, of A and B in it
 };
 
-// the power of two that puts a bound at 2^14
+// the power of two that puts a bound at 2^14 (what shrinks below 2^-86 is below float32's numbers after a step or two)
 double scale_for(double bound) {
     int e;
-    std::frexp(std::max(bound, 1e-30), &e);
-    return std::ldexp(1.0, std::min(14 - e, 30));
+    std::frexp(std::max(bound, 1e-60), &e);
+    return std::ldexp(1.0, std::min(14 - e, 100));
 }
 
 // largest |p(x)| on [0, u], p(x) = x^odd (a + b x^2 + c x^4): at an end or where the derivative, a quadratic in x^2, is zero

@@ -300,3 +300,22 @@ def test_a_gradient_that_is_not_finite_spoils_its_own_layer_only(ctx, wk, rows, 
         layers[i].check(before[i], 0.02, 0.95, True, 0.1)
     m = layers[1].m.get()
     assert np.isinf(m[2, 3]) and np.isfinite(np.delete(m.reshape(-1), 2 * cols + 3)).all() and np.isnan(layers[1].w.get()).all()
+
+
+# ---- coefficients and factors at the ends of their ranges -----------------------------------------------------------------------------
+
+
+@gpu
+@pytest.mark.parametrize("rows,cols", [(40, 130), (140, 200)])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("steps,a", [(3, 1e-6), (5, 2e-5)])
+def test_coefficients_that_shrink_every_number(ctx, rows, cols, kind, steps, a):
+    """X <- a X, a power of which is what is left of G / |G|_F: numbers as small as float32's and bfloat16's own, at full precision."""
+    rs = np.random.RandomState(3)
+    G, O = Mat(ctx, rs.randn(rows, cols), kind), Mat(ctx, np.ones((rows, cols)), kind)
+    ctx.orthogonalise(capi.OrthoJobs([(G.ptr, TYPES[kind], rows, cols, O.ptr, TYPES[kind])]), steps=steps, coef=(a, 0.0, 0.0), eps=0.0)
+    want = iterate(G.get(), steps=steps, coef=[(a, 0.0, 0.0)] * steps, eps=0.0)
+    # per step: X and B rounded (11 or 22 bits of the largest number, which is at most eight times the mean), float32 sums
+    bits = 11 if kind == "bf16" else 22
+    err = np.sqrt(((O.get() - want) ** 2).mean()) / np.sqrt((want ** 2).mean())
+    assert err <= (2 * steps + 2) * 2.0 ** -bits + HALF[kind], err
