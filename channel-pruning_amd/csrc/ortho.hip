@@ -14,6 +14,7 @@
 // get pairs (3e-5 in the worst of these), whatever the result's type.
 // Sums are float32 in the accumulators, |U|_F is summed in float64.
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 
 #include "cp_common.h"
@@ -1317,6 +1318,10 @@ void launch_small(hipStream_t st, const std::vector<SmallJob> &jobs, SmallJobs &
 
 int run(cp_ctx *ctx, const std::vector<Request> &rq, bool crossed, const Plan &pl, double lr, double momentum, int nesterov, double decay,
         double eps, void *given, size_t given_bytes) {
+    // (no more than that: lr, decay and gamma are finite, so that a NaN is not among them)
+    bool fits = std::fabs(momentum) <= FLT_MAX && std::fabs(1.0 - lr * decay) <= FLT_MAX;
+    for (const Request &r : rq) fits &= std::fabs(lr * r.gamma) <= FLT_MAX;
+    if (!fits) return cp_set_error(ctx, CP_ERR_ARG, "momentum, 1 - lr weight_decay or lr gamma is past float32");
     Layout lay;
     CP_TRY(lay_out(ctx, rq, crossed, lr, lay));
     CP_HIP(ctx, hipSetDevice(ctx->device));

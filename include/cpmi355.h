@@ -320,7 +320,8 @@ int cp_orthogonalise_workspace(int n_jobs, const cp_ortho_job *jobs, int steps, 
 /* One optimiser step on a set of layers' weights:
  *   M <- momentum M + G;   U = nesterov ? G + momentum M : M;   W <- (1 - lr weight_decay) W - lr gamma O(U)
  * G DEVICE (g_dtype F32, BF16 or F16), M DEVICE f32 in/out, W DEVICE (w_dtype F32, BF16 or F16) in/out, all [rows, cols];
- * gamma: the job's factor on lr (sqrt(max(1, rows / cols)) is usual).  O(U) as above, carried with 22 bits.  No M or W
+ * gamma: the job's factor on lr (sqrt(max(1, rows / cols)) is usual).  momentum, lr gamma and 1 - lr weight_decay have to be
+ * float32 numbers.  O(U) as above, carried with 22 bits.  No M or W
  * of a call may overlap another matrix of it (a G may serve several jobs).  Nothing is kept between calls but M. */
 typedef struct cp_ortho_step_job {
     const void *G;

@@ -319,3 +319,17 @@ def test_coefficients_that_shrink_every_number(ctx, rows, cols, kind, steps, a):
     bits = 11 if kind == "bf16" else 22
     err = np.sqrt(((O.get() - want) ** 2).mean()) / np.sqrt((want ** 2).mean())
     assert err <= (2 * steps + 2) * 2.0 ** -bits + HALF[kind], err
+
+
+@gpu
+def test_factors_past_float32_are_refused(ctx):
+    """lr gamma, the momentum and the decay's factor are float32 in the kernels: an infinity there would leave NaN in W."""
+    W, M, G = (Mat(ctx, np.ones((3, 4)), "f32") for _ in range(3))
+    def call(lr, gamma=1.0, **kw):
+        ctx.ortho_step(capi.OrthoStepJobs([(G.ptr, 0, 3, 4, M.ptr, W.ptr, 0, gamma)]), lr, **kw)
+    for bad in (dict(lr=1e39), dict(lr=-1e39), dict(lr=1e20, gamma=1e20), dict(lr=1e-3, momentum=1e39), dict(lr=1e20, weight_decay=1e20)):
+        with pytest.raises(capi.CpError):
+            call(**bad)
+    assert np.array_equal(W.raw(), W.before) and np.array_equal(M.raw(), M.before)
+    call(1e38, 1e-38)
+    assert np.isfinite(W.get()).all()
