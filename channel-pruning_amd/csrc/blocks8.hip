@@ -34,9 +34,10 @@ int check_blocks(cp_ctx *ctx, const cp_blocks *m, const char *name) {
 // an 8 x 8 patch in registers, so x is read once for both orientations; a wave's patches form 64 x 64, which makes the
 // segments that it writes 64 bytes long in either.  Bound by HBM, as long as the arithmetic stays short: the largest magnitudes
 // are found on the bit patterns; a thread makes the factors of one row or column, not of its patch's sixteen; and what only
-// infinities and NaN need is done in tiles that hold one.  f32 [20000, 4608] both ways: 107 us for 559 MB (5.2 TB/s; a large copy
-// reaches 4.9), bf16 [4096, 25088]: 86 us for 411 MB, bf16 [20000, 4005], whose rows begin anywhere: 82 us for 324 MB.  (No cut to +-fmax is needed: a finite x times the inverse exceeds
-// fmax by two roundings at most, and rounds to it.)
+// infinities and NaN need is done in tiles that hold one.  f32 [20000, 4608] both ways: 106 us for 559 MB (5.2 TB/s; adding two large
+// float32 matrices, which also reads two bytes for each that it writes, reaches 5.7, a copy 4.97), bf16 [4096, 25088]: 87 us for 411 MB,
+// bf16 [20000, 4005], whose rows begin anywhere: 82 us for 324 MB; the same on six inputs in turn, none of which is in a cache.
+// (No cut to +-fmax is needed: a finite x times the inverse exceeds fmax by two roundings at most, and rounds to it.)
 struct Held {
     uint8_t *q;
     float *scale;
@@ -354,7 +355,7 @@ __device__ __forceinline__ void write_c(const Product &p, const f4 (&acc)[WI][WJ
 // One tile of C, or a piece of k of it, to a workgroup.  COMMON: B's rows share their scales in blocks of 128 (weights), so that a
 // wave's sums take a row's factor; else a row's and a column's.  Beside the matrix instructions a step has those
 // factors in a fused add for every number of the tile (and a product): bound by both together.  8192^3, every row with its own scales: 527 us, 2.09
-// PFLOP/s (a library product without any scales 358); common scales, 20000 x 512 x 4005: 67 us, 1.22 (its
+// PFLOP/s (a library product without any scales 358), common scales 439; those, 20000 x 512 x 4005: 70 us, 1.17 (its
 // 80 MB come from HBM one step ahead of their use).  WIDE (float32 and fp16 results):
 // the operands are widened in registers and go through the fp16 instructions, twice as many: 512 x 4005 x 20000, 112 us, 0.73
 // PFLOP/s (104 if the conversions cost nothing); 256 x 256 tiles would need more registers than there are.

@@ -172,7 +172,8 @@ struct Inverse {
 };
 
 // ---- |U|_F, and the momentum: one pass over G (and M), bound by HBM -----------------------------------------------------------
-// (12.8 M numbers, G and M float32: 28.5 us for 153 MB, 5.4 TB/s; 67 M in bfloat16: 39 us for 134 MB.)
+// (12.8 M numbers, G and M float32: 28.5 us for 153 MB, 5.4 TB/s, and 29.5 on six sets of layers in turn, 5.2; adding two large
+// matrices reaches 5.7.  67 M in bfloat16: 39 us for 134 MB; reading alone, a large maximum takes 3.7 TB/s.)
 // A workgroup sums rows_per rows of a chunk of `width` columns; the partial sums are added in one order by whoever needs the
 // norm.  Contiguous matrices are one row: their own rows' lengths would leave most of them unaligned.
 __global__ void __launch_bounds__(256) k_ortho_norm(Jobs js, Table t, float momentum, int nesterov, int *counts, int n_counts) {
@@ -346,7 +347,7 @@ __global__ void __launch_bounds__(256) k_ortho_load(Table tab, float momentum, i
 // All jobs' tiles of one of a step's three products in one launch.  Bound by the matrix instructions where matrices are large (4096 x
 // 16384 in fp16: first product 305 us, 0.90 PFLOP/s of the half that is formed -- 136 tiles of 256 x 256 divide badly over 256
 // CUs --, second 110, third 480, 1.15 PFLOP/s), by a launch's fixed costs where they are many and small (the 40 layers of a
-// pruned resnet50, 8.5 M numbers: 14, 8 and 23 us).
+// pruned resnet50, 8.5 M numbers in pairs: 25, 13 and 41 us).
 struct Factors {
     float acc, a, diag;   // what the accumulator, A's entry and the diagonal count for in the result
     float keep;           // LAST: 1 - lr * weight_decay (cp_ortho_step)
