@@ -525,7 +525,7 @@ class Context:
     def use_torch_stream(self):
         """Run on torch's current stream, behind what this context has enqueued so far (its scratch is free then).  To be called
         again where that stream may have changed; costs next to nothing where it has not.  (On its own stream a context
-        puts every call with torch tensors in order with torch's current stream, by two events: about 10 us a call.)"""
+        puts every call with torch tensors in order with torch's current stream, by two events: 23 us a call, this 0.4.)"""
         s = torch_stream(self.device)
         if s != self._given:
             self._check(self.lib.cp_ctx_before_stream(self.h, s), "cp_ctx_before_stream")
